@@ -13,6 +13,8 @@ Public surface (mirrors faster_cosyvoice.token2wav.flashinfer_dit / flashinfer_f
                           -- stream_step / stream_step_batched (Flow half) over the packed path
   load_flow               -- the MI355X flow from a flow.pt state dict
   HiFTVocoder             -- the HiFT vocoder (CausalHiFTGenerator counterpart), packed batches
+  fused_linear, qk_norm_rope, prefix_attention
+                          -- decoder-layer operators of the model that writes the speech tokens
 """
 
 from .estimator import DiTEstimator, rope_tables
@@ -21,10 +23,12 @@ from .solver import apply_mi355x, euler_schedule, solve_euler_batched, solve_eul
 from .streaming import CFMDecoder, StreamingFlow
 from .checkpoint import load_flow
 from .hift import HiFTVocoder
+from .lm import fused_linear, prefix_attention, qk_norm_rope
 from . import synthetic
 
 __all__ = ["CFMDecoder", "DiTEstimator", "FlowFrontEnd", "HiFTVocoder", "StreamingFlow",
            "apply_mi355x",
            "euler_schedule",
-           "flow_inference_batched", "flow_inference_batched_streaming", "load_flow", "rope_tables",
+           "flow_inference_batched", "flow_inference_batched_streaming", "fused_linear", "load_flow",
+           "prefix_attention", "qk_norm_rope", "rope_tables",
            "solve_euler_batched", "solve_euler_packed", "synthetic"]

@@ -1,4 +1,5 @@
-"""ctypes bindings of libfcvdit.so (declared in include/fcv_dit.h, fcv_flow.h and fcv_hift.h).
+"""ctypes bindings of libfcvdit.so (declared in include/fcv_dit.h, fcv_flow.h, fcv_hift.h and
+fcv_lm.h).
 
 The library is the only compute path: if it is missing, importing the estimator raises,
 there is no fallback.  Error codes map to the exceptions the reference raises for the same
@@ -9,7 +10,7 @@ RuntimeError for state errors).
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_float, c_int32, c_size_t, c_void_p
+from ctypes import POINTER, c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfcvdit.so"
@@ -64,6 +65,36 @@ class FcvHiftDims(ctypes.Structure):
         ("hop_len", c_int32), ("conv_pre_look_right", c_int32), ("f0_channels", c_int32),
         ("lrelu_slope", c_float), ("audio_limit", c_float), ("noise_samples", c_int32),
     ]
+
+
+class FcvLmLinear(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "residual", "y")]
+                + [(n, c_int64) for n in ("ldx", "ldw", "ldr", "ldy")]
+                + [(n, c_int32) for n in ("m", "n", "k", "dtype", "bias_dtype", "residual_dtype",
+                                          "y_dtype", "activation")])
+
+
+class FcvLmQkNormRope(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("qkv", "positions", "cache_rows", "rope_cos", "rope_sin",
+                                         "q_weight", "k_weight", "q_out", "k_cache", "v_cache")]
+                + [(n, c_int64) for n in ("qkv_row", "q_row", "k_session", "k_row", "k_head",
+                                          "v_session", "v_row", "v_head")]
+                + [(n, c_int32) for n in ("tokens", "n_heads", "n_kv_heads", "head_dim", "rope_dim",
+                                          "max_pos", "sessions", "capacity", "dtype",
+                                          "weight_dtype", "interleaved")]
+                + [("eps", c_float)])
+
+
+class FcvLmAttention(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("q", "prefix_k", "prefix_v", "k_cache", "v_cache", "cu_q",
+                                         "lengths", "slots", "out", "lse")]
+                + [(n, c_int64) for n in ("q_row", "q_head", "out_row", "out_head", "pk_row",
+                                          "pk_head", "pv_row", "pv_head", "k_session", "k_row",
+                                          "k_head", "v_session", "v_row", "v_head")]
+                + [(n, c_int32) for n in ("tokens", "batch", "n_heads", "n_kv_heads", "head_dim",
+                                          "prefix_len", "sessions", "capacity", "max_q",
+                                          "max_length", "dtype")]
+                + [("scale", c_float)])
 
 
 # (name, restype, argtypes) of every exported entry point
@@ -130,6 +161,12 @@ SIGNATURES = {
                                               c_void_p, c_void_p, c_void_p, c_size_t, c_int32,
                                               c_void_p]),
     "fcv_hift_graph_stats": (c_int32, [c_void_p, POINTER(c_int32), POINTER(c_int32)]),
+    # include/fcv_lm.h
+    "fcv_lm_linear_workspace_bytes": (c_size_t, [POINTER(FcvLmLinear)]),
+    "fcv_lm_linear": (c_int32, [POINTER(FcvLmLinear), c_void_p, c_size_t, c_void_p]),
+    "fcv_lm_qk_norm_rope": (c_int32, [POINTER(FcvLmQkNormRope), c_void_p]),
+    "fcv_lm_prefix_attention_workspace_bytes": (c_size_t, [POINTER(FcvLmAttention)]),
+    "fcv_lm_prefix_attention": (c_int32, [POINTER(FcvLmAttention), c_void_p, c_size_t, c_void_p]),
 }
 
 STAGES = ("qkv", "attention", "out_proj", "ff1", "ff2", "ln_mod", "conv", "adaln", "in_proj",

@@ -20,7 +20,8 @@ LIB_NAME = "libfcvdit.so"
 ARCH = "gfx950"
 
 SOURCES = ["gemm.hip", "gemv.hip", "attention.hip", "conv.hip", "elementwise.hip", "frontend.hip",
-           "hift.hip", "hift_split.hip", "hift_capi.hip", "capi.hip"]
+           "hift.hip", "hift_split.hip", "hift_capi.hip", "linear.hip", "qk_norm_rope.hip",
+           "prefix_attention.hip", "capi.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -51,7 +52,7 @@ def library_path() -> Path:
 # not in others, so an element's fp16 bits would depend on the GEMM tile shape, and with it on
 # the batch a document is packed with.
 EXACT_SOURCES = {"gemm.hip", "gemv.hip", "attention.hip", "conv.hip", "elementwise.hip", "capi.hip",
-                 "hift_split.hip"}
+                 "hift_split.hip", "linear.hip", "qk_norm_rope.hip", "prefix_attention.hip"}
 EXACT_FLAGS = ["-ffp-contract=off"]
 
 

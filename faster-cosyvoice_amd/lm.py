@@ -1,0 +1,321 @@
+"""Operators of the language model that writes the speech tokens, on libfcvdit.so
+(include/fcv_lm.h): the linear layer with its epilogue, per-head norms with the rotation and the
+cache append, and attention of a batch whose requests share one voice's prompt.
+
+The reference runs that model in an engine of its own (faster_cosyvoice/llm/engine.py:94-141);
+these are what a decoder layer beside Token2Wav needs:
+
+    qkv = fused_linear(x, w_qkv, b_qkv)
+    q = qk_norm_rope(qkv, positions, cos, sin, k_cache, v_cache, rows, n_heads=32)
+    o = prefix_attention(q, k_cache, v_cache, lengths, prefix_k=voice_k, prefix_v=voice_v)
+    x = fused_linear(o.flatten(1), w_out, residual=x)
+
+Calls are asynchronous on the current stream of the tensors' device, compute no gradients, and may
+be captured into a graph: lengths, positions and rows are device tensors, and workspaces come from
+torch's allocator, which keeps a capture's in the capture's own pool.  Wrong shapes, types and
+layouts raise ``ValueError`` before anything is launched; values inside device tensors are not
+looked at on the host (include/fcv_lm.h says what the kernels make of each).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}  # FCV_LM_F16, FCV_LM_BF16
+_F32 = 2                                         # FCV_LM_F32
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def _launch(fn, device: torch.device, *args) -> None:
+    """Call a library entry on ``device``'s current stream, with ``device`` current."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _launch(fn, device, *args)
+    rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        _lib.check(rc)
+
+
+def _dtype(t: torch.Tensor, name: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None or not t.is_cuda:
+        raise ValueError(f"{name} must be a float16 or bfloat16 tensor on the GPU, got "
+                         f"{t.dtype} on {t.device}")
+    return code
+
+
+def _side(t: torch.Tensor, name: str, like: torch.Tensor, code: int) -> int:
+    """The type code of a tensor that may be of ``like``'s type or fp32."""
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+    if t.dtype == like.dtype:
+        return code
+    if t.dtype == torch.float32:
+        return _F32
+    raise ValueError(f"{name} must be {like.dtype} or float32, got {t.dtype}")
+
+
+def _indices(t: torch.Tensor, name: str, n: int, like: torch.Tensor) -> int:
+    if t.dtype != torch.int32 or t.device != like.device or t.shape != (n,) \
+            or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} on {like.device}")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, name: str, width: int) -> tuple[int, int]:
+    """Row count and stride of a tensor seen as rows of its last dimension."""
+    if t.shape[-1] != width:
+        raise ValueError(f"{name} must have {width} columns, got {tuple(t.shape)}")
+    if t.dim() != 2:
+        try:
+            t = t.view(-1, width)
+        except RuntimeError as e:
+            raise ValueError(f"{name}'s leading dimensions {tuple(t.shape[:-1])} do not lie at one "
+                             "stride: make it contiguous") from e
+    n, ld = t.shape[0], t.stride(0)
+    if width > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+    return n, ld if n > 1 else max(ld, width)
+
+
+@torch.no_grad()
+def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                 activation: str | None = None, residual: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None,
+                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual``: products on the matrix cores with fp32 sums, one
+    rounding at the end.
+
+    ``x`` ``[..., K]`` and ``weight`` ``[N, K]`` are fp16 or bf16 (the same), ``bias`` ``[N]`` and
+    ``residual`` ``[..., N]`` are of that type or fp32; the result is of ``out_dtype`` (``x``'s by
+    default, or fp32) or goes to ``out``, which may be ``residual`` itself and overlaps no other
+    input.  ``activation``: ``"relu"``, ``"silu"``, ``"gelu"`` (erf), ``"gelu_tanh"`` or none.
+    Rows may lie at any stride; rows that start on 16-byte boundaries are read faster."""
+    code = _dtype(x, "x")
+    if weight.dtype != x.dtype or weight.device != x.device or weight.dim() != 2:
+        raise ValueError(f"weight must be a {x.dtype} matrix on {x.device}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    n, k = weight.shape
+    if n < 1 or k < 1:
+        raise ValueError(f"weight is empty: {tuple(weight.shape)}")
+    m, ldx = _rows(x, "x", k)
+    _, ldw = _rows(weight, "weight", k)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}")
+    shape = x.shape[:-1] + (n,)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype if out_dtype is None else out_dtype,
+                          device=x.device)
+        if out_dtype is not None:
+            out_code = _side(out, "out", x, code)
+        else:
+            out_code = code
+        ldy = n
+    else:
+        if out.shape != shape:
+            raise ValueError(f"out must have shape {tuple(shape)}, got {tuple(out.shape)}")
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"out is {out.dtype}, not {out_dtype}")
+        out_code = _side(out, "out", x, code)
+        _, ldy = _rows(out, "out", n)
+        if m > 1 and ldy < n:
+            raise ValueError("out's rows overlap")
+    bias_ptr, bias_code = None, code
+    if bias is not None:
+        bias_code = _side(bias, "bias", x, code)
+        if bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
+            raise ValueError(f"bias must be a contiguous vector of {n}")
+        bias_ptr = bias.data_ptr()
+    res_ptr, res_code, ldr = None, code, 0
+    if residual is not None:
+        res_code = _side(residual, "residual", x, code)
+        if residual.shape != shape:
+            raise ValueError(f"residual must have shape {tuple(shape)}, got "
+                             f"{tuple(residual.shape)}")
+        _, ldr = _rows(residual, "residual", n)
+        res_ptr = residual.data_ptr()
+    if m == 0:
+        return out
+    lib = _lib.load()
+    args = _lib.FcvLmLinear(x.data_ptr(), weight.data_ptr(), bias_ptr, res_ptr, out.data_ptr(),
+                            ldx, ldw, ldr, ldy, m, n, k, code, bias_code, res_code, out_code, act)
+    need = lib.fcv_lm_linear_workspace_bytes(args)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        _launch(lib.fcv_lm_linear, x.device, args, ws.data_ptr(), need)
+    else:
+        _launch(lib.fcv_lm_linear, x.device, args, None, 0)
+    return out
+
+
+def _cache(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    if t.dtype != like.dtype or t.device != like.device or t.dim() != 4 or t.numel() == 0:
+        raise ValueError(f"{name} must be a {like.dtype} tensor [sessions, capacity, kv heads, "
+                         f"head dim] on {like.device}")
+    if t.stride(3) != 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+
+
+@torch.no_grad()
+def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                 k_cache: torch.Tensor, v_cache: torch.Tensor, cache_rows: torch.Tensor, *,
+                 n_heads: int, q_weight: torch.Tensor | None = None,
+                 k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                 interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """RMS norms of queries and keys per head, the position rotation and the cache append, in one
+    pass over the packed projection ``qkv`` ``[T, (n_heads + 2 kv heads) * head dim]``.
+
+    The caches are ``[sessions, capacity, kv heads, head dim]`` (64 or 128) at any strides; token
+    ``t``'s key and value go to row ``cache_rows[t]`` of them, counted over sessions and capacity
+    (a negative row or one past the end: nowhere).  ``cos``/``sin`` are fp32 tables
+    ``[positions, rotated / 2]``; ``interleaved`` rotates pairs ``(2 i, 2 i + 1)``, otherwise
+    ``(i, i + rotated / 2)``.  ``q_weight``/``k_weight`` ``[head dim]`` scale the norms; without
+    them heads are not normed.  Returns the queries ``[T, n_heads, head dim]``.  A prompt that a
+    batch shares is written with one session's caches (``prefix[None]``)."""
+    code = _dtype(qkv, "qkv")
+    _cache(k_cache, "k_cache", qkv)
+    _cache(v_cache, "v_cache", qkv)
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ")
+    sessions, capacity, n_kv, dim = k_cache.shape
+    if dim not in (64, 128):
+        raise ValueError(f"head dim must be 64 or 128, got {dim}")
+    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * dim or n_heads < 1:
+        raise ValueError(f"qkv must be [tokens, {(n_heads + 2 * n_kv) * dim}], got "
+                         f"{tuple(qkv.shape)}")
+    tokens, qkv_row = _rows(qkv, "qkv", qkv.shape[1])
+    pos_ptr = _indices(positions, "positions", tokens, qkv)
+    row_ptr = _indices(cache_rows, "cache_rows", tokens, qkv)
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if t.dtype != torch.float32 or t.device != qkv.device or t.dim() != 2 \
+                or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 table on {qkv.device}")
+    if cos.shape != sin.shape or cos.shape[0] < 1:
+        raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be equal tables")
+    w_code = code
+    if q_weight is not None and k_weight is not None:
+        w_code = _side(q_weight, "q_weight", qkv, code)
+        if _side(k_weight, "k_weight", qkv, code) != w_code:
+            raise ValueError("q_weight and k_weight must have one type")
+        for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+            if t.shape != (dim,) or t.stride(0) != 1:
+                raise ValueError(f"{name} must be a contiguous vector of {dim}")
+    elif q_weight is not k_weight:
+        raise ValueError("q_weight and k_weight come together")
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if any(t.shape[i] > 1 and t.stride(i) == 0 for i in range(3)):
+            raise ValueError(f"{name} is expanded: its rows share memory")
+    if out is None:
+        out = torch.empty(tokens, n_heads, dim, dtype=qkv.dtype, device=qkv.device)
+    elif out.dtype != qkv.dtype or out.device != qkv.device or out.shape != (tokens, n_heads, dim) \
+            or out.stride(2) != 1 or (n_heads > 1 and out.stride(1) != dim):
+        raise ValueError(f"out must be a {qkv.dtype} tensor {(tokens, n_heads, dim)} on "
+                         f"{qkv.device} whose heads are contiguous")
+    if tokens == 0:
+        return out
+    ks, vs = k_cache.stride(), v_cache.stride()
+    args = _lib.FcvLmQkNormRope(
+        qkv.data_ptr(), pos_ptr, row_ptr, cos.data_ptr(), sin.data_ptr(),
+        None if q_weight is None else q_weight.data_ptr(),
+        None if k_weight is None else k_weight.data_ptr(), out.data_ptr(), k_cache.data_ptr(),
+        v_cache.data_ptr(), qkv_row, out.stride(0) if tokens > 1 else n_heads * dim, ks[0], ks[1],
+        ks[2], vs[0], vs[1], vs[2], tokens, n_heads, n_kv, dim, 2 * cos.shape[1], cos.shape[0],
+        sessions, capacity, code, w_code, bool(interleaved), eps)
+    _launch(_lib.load().fcv_lm_qk_norm_rope, qkv.device, args)
+    return out
+
+
+@torch.no_grad()
+def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     lengths: torch.Tensor, *, prefix_k: torch.Tensor | None = None,
+                     prefix_v: torch.Tensor | None = None, cu_q: torch.Tensor | None = None,
+                     max_q: int | None = None, slots: torch.Tensor | None = None,
+                     max_length: int | None = None, scale: float | None = None,
+                     out: torch.Tensor | None = None, return_lse: bool = False):
+    """Causal attention of a batch of sequences that share one prompt: every query of ``q``
+    ``[T, heads, head dim]`` sees all of ``prefix_k``/``prefix_v`` ``[P, kv heads, head dim]`` and
+    its own sequence's cached keys up to itself; the prompt is read once for the whole batch.
+
+    The caches are ``[sessions, capacity, kv heads, head dim]`` (64 or 128) at any strides;
+    sequence ``b`` reads session ``slots[b]`` (``b`` without ``slots``), its ``lengths[b]`` keys
+    include those of its new tokens.  Its queries are rows ``cu_q[b] .. cu_q[b + 1] - 1``; without
+    ``cu_q`` every sequence has ``T / len(lengths)``.  Rows past ``cu_q[-1]`` are not read, and
+    their rows of ``out`` stay as they are (whatever the memory held, without ``out``).  ``max_q`` and ``max_length`` bound the queries and keys of a sequence and shape the
+    launch (they default to ``T`` and the capacity); batches that pass them are still computed.
+    ``scale`` defaults to ``head dim ** -0.5``.  A query that sees no key gives zeros.  Returns
+    the output, or with ``return_lse`` also the log sums of exponentials, fp32 ``[T, heads]``."""
+    code = _dtype(q, "q")
+    _cache(k_cache, "k_cache", q)
+    _cache(v_cache, "v_cache", q)
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ")
+    sessions, capacity, n_kv, dim = k_cache.shape
+    if dim not in (64, 128):
+        raise ValueError(f"head dim must be 64 or 128, got {dim}")
+    if q.dim() != 3 or q.shape[2] != dim or q.shape[1] % n_kv or q.shape[1] < 1:
+        raise ValueError(f"q must be [tokens, heads, {dim}] with heads a multiple of {n_kv}, got "
+                         f"{tuple(q.shape)}")
+    if q.stride(2) != 1:
+        raise ValueError("q's last dimension must be contiguous")
+    tokens, heads, _ = q.shape
+    batch = lengths.numel()
+    if batch < 1:
+        raise ValueError("lengths is empty")
+    len_ptr = _indices(lengths, "lengths", batch, q)
+    cu_ptr = None if cu_q is None else _indices(cu_q, "cu_q", batch + 1, q)
+    if cu_q is None:
+        if tokens % batch:
+            raise ValueError(f"without cu_q the {tokens} rows of q must divide by the {batch} "
+                             "sequences")
+        max_q = max(tokens // batch, 1)
+    elif max_q is None:
+        max_q = max(tokens, 1)
+    slot_ptr = None if slots is None else _indices(slots, "slots", batch, q)
+    if slots is None and batch > sessions:
+        raise ValueError(f"{batch} sequences need slots: the caches hold {sessions} sessions")
+    prefix_len, pk_ptr, pv_ptr, pk, pv = 0, None, None, (0, 0), (0, 0)
+    if (prefix_k is None) != (prefix_v is None):
+        raise ValueError("prefix_k and prefix_v come together")
+    if prefix_k is not None:
+        for t, name in ((prefix_k, "prefix_k"), (prefix_v, "prefix_v")):
+            if t.dtype != q.dtype or t.device != q.device or t.dim() != 3 \
+                    or t.shape[1:] != (n_kv, dim) or t.stride(2) != 1:
+                raise ValueError(f"{name} must be a {q.dtype} tensor [keys, {n_kv}, {dim}] on "
+                                 f"{q.device}, its last dimension contiguous")
+        if prefix_k.shape != prefix_v.shape:
+            raise ValueError("prefix_k and prefix_v differ in length")
+        prefix_len = prefix_k.shape[0]
+        if prefix_len:
+            pk_ptr, pv_ptr = prefix_k.data_ptr(), prefix_v.data_ptr()
+            pk, pv = prefix_k.stride(), prefix_v.stride()
+    if out is None:
+        out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.device != q.device or out.shape != q.shape \
+            or out.stride(2) != 1:
+        raise ValueError(f"out must be a {q.dtype} tensor {tuple(q.shape)} on {q.device}, its last "
+                         "dimension contiguous")
+    elif any(out.shape[i] > 1 and out.stride(i) == 0 for i in range(2)):
+        raise ValueError("out is expanded: its rows share memory")
+    lse = None
+    if return_lse:
+        lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device)
+    if tokens == 0:
+        return (out, lse) if return_lse else out
+    ks, vs = k_cache.stride(), v_cache.stride()
+    args = _lib.FcvLmAttention(
+        q.data_ptr(), pk_ptr, pv_ptr, k_cache.data_ptr(), v_cache.data_ptr(), cu_ptr, len_ptr,
+        slot_ptr, out.data_ptr(), None if lse is None else lse.data_ptr(), q.stride(0),
+        q.stride(1), out.stride(0), out.stride(1), pk[0], pk[1], pv[0], pv[1], ks[0], ks[1], ks[2],
+        vs[0], vs[1], vs[2], tokens, batch, heads, n_kv, dim, prefix_len, sessions, capacity,
+        max_q, capacity if max_length is None else max_length, code,
+        dim ** -0.5 if scale is None else scale)
+    lib = _lib.load()
+    need = lib.fcv_lm_prefix_attention_workspace_bytes(args)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _launch(lib.fcv_lm_prefix_attention, q.device, args, ws.data_ptr(), need)
+    return (out, lse) if return_lse else out
