@@ -116,6 +116,13 @@ __device__ __forceinline__ void lds_dma16(const void* base, uint32_t voff, uint3
                : "s"(lds), "v"(voff), "s"(base)
                : "memory", "m0");
 }
+// The same from an address of each lane's own.
+__device__ __forceinline__ void lds_dma16_at(const void* addr, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(addr)
+               : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 }  // namespace fcv
