@@ -20,9 +20,11 @@ struct Half {
   typedef f16 T;
   static constexpr short kOne = 0x3C00;        // 1.0
   static constexpr short kInf = 0x7C00;        // +inf, and the exponent's mask
-  // Softmax weights are held at 2^kShift times their size: 2^15 keeps weights down to 2^-29 of the
-  // row's largest in fp16's normal range (many small weights can carry most of a long row's sum).
-  static constexpr float kShift = 15.0f;
+  // Softmax: a row's running maximum follows the true one when that is kLag (in powers of two) above
+  // it, so that sums are rescaled seldom, and weights are held at 2^kShift times their size.  fp16:
+  // no weight passes 2^15, and one is in the normal range down to 2^-25 of the row's largest (many
+  // small weights can carry most of a long row's sum).
+  static constexpr float kShift = 11.0f, kLag = 4.0f;
   static __device__ __forceinline__ float to_f32(short b) { return (float)__builtin_bit_cast(f16, b); }
   static __device__ __forceinline__ short from_f32(float v) {
     return __builtin_bit_cast(short, f2h(v));
@@ -41,7 +43,7 @@ struct Bf16 {
   typedef __bf16 T;
   static constexpr short kOne = 0x3F80;
   static constexpr short kInf = 0x7F80;
-  static constexpr float kShift = 0.0f;        // bf16 has fp32's range
+  static constexpr float kShift = 0.0f, kLag = 8.0f;  // bf16 has fp32's range
   static __device__ __forceinline__ float to_f32(short b) {
     return __uint_as_float((uint32_t)(uint16_t)b << 16);
   }

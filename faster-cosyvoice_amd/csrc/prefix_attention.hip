@@ -20,17 +20,22 @@ namespace fcv {
 namespace lm {
 namespace {
 
-constexpr int kRows = 32;   // queries of a row tile
-constexpr int kKeys = 32;   // keys of a wave's tile
 constexpr int kWaves = 4;
+constexpr int kFewRows = 32;    // queries of a row tile whose waves share the keys out
+constexpr int kFewKeys = 32;    // keys of a wave's tile there
+constexpr int kManyRows = 128;  // queries of a row tile whose waves share its queries out, 32 each
+constexpr int kManyKeys = 64;   // keys of a workgroup's tile there
+constexpr int kMaxParts = 64;   // lanes of the joining wave
 constexpr float kLog2e = 1.4426950408889634f;
 
-// How a call is split.  Parts 0 .. np - 1 are ranges of the prefix, np .. np + no - 1 of a
-// sequence's own keys.
+// How a call is split.  Parts 0 .. np - 1 are ranges of the prefix for the rows of all sequences
+// together, np .. np + no - 1 ranges of a sequence's own keys, or (np = 0, fused) of the prefix and its
+// own keys behind one another.
 struct Shape {
-  int prefix_tiles, np;      // row tiles over the whole batch; ranges of the prefix
-  int own_tiles, no;         // row tiles of a sequence; ranges of its keys
-  int prefix_step, own_step; // keys of a range (own_step at least: longer caches widen it)
+  bool prefix_many, own_many;  // tiles of 128 rows, else of 32
+  bool fused, direct;          // direct: one part, written to the output
+  int prefix_tiles, np, prefix_step;
+  int own_tiles, no, own_step; // own_step: keys of a range at least (longer caches widen it)
   int64_t prefix_blocks, own_blocks;
   __host__ __device__ int parts() const { return np + no; }
 };
@@ -43,9 +48,21 @@ struct Args {
   float scale2;   // scale * log2(e)
 };
 
+// A value that is the same in all lanes, as a scalar.
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const short* scalar(const short* p) {
+  const uint64_t u = (uint64_t)p;
+  return (const short*)((uint64_t)(uint32_t)scalar((int)u) | (uint64_t)(uint32_t)scalar((int)(u >> 32)) << 32);
+}
+
 __device__ __forceinline__ float half_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 template <int N>
@@ -97,153 +114,205 @@ __device__ __forceinline__ s16x8 v_fragment(const short* sv, int lane, int st, i
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// One tile of 32 keys from LDS.  `limit` (per lane) is the first key of the tile that the lane's
+// Whether the lane reads an infinity or a NaN among the values of a tile of 32 KT keys.
+template <class E, int D, int KT>
+__device__ __forceinline__ bool not_finite(const short* sv, int lane) {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+  u16x8 top = {};
+#pragma unroll 4
+  for (int i = 0; i < KT * D / 16; ++i)
+    top = __builtin_elementwise_max(
+        top, *reinterpret_cast<const u16x8*>(sv + (i * 64 + lane) * 8) & (unsigned short)0x7fff);
+  unsigned short most = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) most = most > top[e] ? most : top[e];
+  return most >= (unsigned short)E::kInf;
+}
+
+// One tile of 32 KT keys from LDS.  `limit` (per lane) is the first key of the tile that the lane's
 // query does not see; all_visible says that no lane has one.
-template <class E, int D>
-__device__ __forceinline__ void tile32(const short* sk, const short* sv, const s16x8 (&qf)[D / 16],
-                                       State<D>& st, int lane, int limit, bool all_visible,
-                                       float scale2) {
+template <class E, int D, int KT>
+__device__ __forceinline__ void tile(const short* sk, const short* sv, const s16x8 (&qf)[D / 16],
+                                     State<D>& st, int lane, int limit, bool all_visible,
+                                     float scale2) {
   const int ql = lane & 31, hl = lane >> 5;
-  f32x16 s;
+  f32x16 s[KT];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+  for (int t = 0; t < KT; ++t) {
 #pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) {
-    const s16x8 kf =
-        *reinterpret_cast<const s16x8*>(sk + ql * D + swz<D>(ql, ks * 2 + hl) * 8);
-    s = E::mfma32(kf, qf[ks], s);
+    for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const int row = t * 32 + ql;
+      const s16x8 kf = *reinterpret_cast<const s16x8*>(sk + row * D + swz<D>(row, ks * 2 + hl) * 8);
+      s[t] = E::mfma32(kf, qf[ks], s[t]);
+    }
   }
   if (!all_visible) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      s[e] = (e >> 2) * 8 + hl * 4 + (e & 3) < limit ? s[e] : -INFINITY;
-  }
-  float top = s[0];
+    for (int t = 0; t < KT; ++t)
 #pragma unroll
-  for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-  const float m_new = fmaxf(st.m, half_max(top) * scale2);
-  // a query that has seen no finite score yet keeps m = -inf and subtracts 0
-  const float base = m_new == -INFINITY ? 0.0f : m_new;
-  const float corr = hw_exp2(st.m - base);
-  const float shift = E::kShift - base;
-  st.m = m_new;
+      for (int e = 0; e < 16; ++e)
+        s[t][e] = t * 32 + (e >> 2) * 8 + hl * 4 + (e & 3) < limit ? s[t][e] : -INFINITY;
+  }
+  float top = s[0][0];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
+  top = half_max(top) * scale2;
+  if (__any(top > st.m + E::kLag)) {
+    const float m_new = top > st.m + E::kLag ? top : st.m;
+    // a query that has seen no finite score yet keeps m = -inf (and sums of 0)
+    const float corr = hw_exp2(st.m - (m_new == -INFINITY ? 0.0f : m_new));
+    st.m = m_new;
+    st.l *= corr;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) st.acc[dt][e] *= corr;
+  }
+  const float shift = E::kShift - (st.m == -INFINITY ? 0.0f : st.m);
   float sum = 0.0f;
-  s16x8 pf[2];
+  s16x8 pf[2 * KT];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const float w = hw_exp2(fmaf(s[e], scale2, shift));
-    sum += w;
-    // 16-bit weights (relative error 2^-9 bf16, 2^-12 fp16, each with its own sign): what the
-    // matrix instruction takes; the sum keeps the unrounded ones
-    pf[e >> 3][e & 7] = E::from_f32(w);
-  }
-  st.l = fmaf(st.l, corr, sum);
+  for (int t = 0; t < KT; ++t)
 #pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt) {
+    for (int e = 0; e < 16; ++e) {
+      const float w = hw_exp2(fmaf(s[t][e], scale2, shift));
+      sum += w;
+      // 16-bit weights (relative error 2^-9 bf16, 2^-12 fp16, each with its own sign): what the
+      // matrix instruction takes; the sum keeps the unrounded ones
+      pf[t * 2 + (e >> 3)][e & 7] = E::from_f32(w);
+    }
+  st.l += sum;
+  if (!all_visible && __any(not_finite<E, D, KT>(sv, lane))) {
+    // 0 * inf and 0 * NaN: a value that is not finite is taken out of the product, and the queries that
+    // see its key get +-big * big = +-inf instead (both for a NaN), in bf16, which spans fp32's range
+    constexpr short kBig = 0x7F00;  // 2^127
 #pragma unroll
-    for (int e = 0; e < 16; ++e) st.acc[dt][e] *= corr;
-    s16x8 vf[2];
+    for (int dt = 0; dt < D / 32; ++dt) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) vf[k] = v_fragment<D>(sv, lane, k, dt);
-    if (!all_visible) {
-      // 0 * inf and 0 * NaN: a value that is not finite is taken out of the product and given to
-      // the queries that see its key
-      bool bad = false;
+      for (int k = 0; k < 2 * KT; ++k) {
+        // one at a time, nothing of it computed ahead: this must not cost the usual path registers
+        int lane_here = lane, limit_here = limit;
+        asm volatile("" : "+v"(lane_here), "+v"(limit_here));
+        s16x8 vf = v_fragment<D>(sv, lane_here, k, dt), up = {}, down = {}, seen;
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) bad |= (vf[k][e] & E::kInf) == E::kInf;
-      if (__any(bad)) {
-        f32x16 up, down, nan;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) up[e] = down[e] = nan[e] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          s16x8 seen, is_up = {}, is_down = {}, is_nan = {};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int key = k * 16 + (e >> 2) * 8 + hl * 4 + (e & 3);
-            seen[e] = key < limit ? E::kOne : (short)0;
-            const short b = vf[k][e];
-            if ((b & E::kInf) != E::kInf) continue;
-            if ((b & 0x7fff) != E::kInf) is_nan[e] = E::kOne;
-            else if (b < 0) is_down[e] = E::kOne;
-            else is_up[e] = E::kOne;
-            vf[k][e] = 0;
-          }
-          up = E::mfma32(is_up, seen, up);
-          down = E::mfma32(is_down, seen, down);
-          nan = E::mfma32(is_nan, seen, nan);
+        for (int e = 0; e < 8; ++e) {
+          const short v = vf[e];
+          const bool bad = (v & E::kInf) == E::kInf, nan = bad && (v & 0x7fff) != E::kInf;
+          vf[e] = bad ? (short)0 : v;
+          up[e] = nan || (bad && v > 0) ? kBig : (short)0;
+          down[e] = nan || (bad && v < 0) ? (short)(kBig | 0x8000) : (short)0;
+          seen[e] = k * 16 + (e >> 2) * 8 + (lane_here >> 5) * 4 + (e & 3) < limit_here ? kBig : (short)0;
         }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (nan[e] > 0.0f) st.acc[dt][e] += NAN;
-          if (up[e] > 0.0f) st.acc[dt][e] += INFINITY;
-          if (down[e] > 0.0f) st.acc[dt][e] -= INFINITY;
-        }
+        st.acc[dt] = E::mfma32(vf, pf[k], st.acc[dt]);
+        st.acc[dt] = Bf16::mfma32(up, seen, st.acc[dt]);
+        st.acc[dt] = Bf16::mfma32(down, seen, st.acc[dt]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) st.acc[dt] = E::mfma32(vf[k], pf[k], st.acc[dt]);
+    return;
   }
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int k = 0; k < 2 * KT; ++k)
+      st.acc[dt] = E::mfma32(v_fragment<D>(sv, lane, k, dt), pf[k], st.acc[dt]);
 }
+
+// The queries of a row tile: rows first .. first + count - 1 of the (token, head of the group) pairs of
+// one key head, token-major from token0 on.
+struct Rows {
+  int kvh, group, token0, first, count;
+  __device__ __forceinline__ int token(int r) const { return token0 + (first + r) / group; }
+  __device__ __forceinline__ int head(int r) const { return kvh * group + (first + r) % group; }
+};
+
+template <int D>
+__device__ __forceinline__ void load_q(const FcvLmAttention& p, const Rows& rows, int r, int hl,
+                                       s16x8 (&qf)[D / 16]) {
+  const int row = min(r, rows.count - 1);
+  const short* q = static_cast<const short*>(p.q) + rows.token(row) * p.q_row + rows.head(row) * p.q_head;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+    qf[ks] = *reinterpret_cast<const s16x8*>(q + ks * 16 + hl * 8);
+}
+
+// Copies of one wave: N times 64 / (D / 8) rows, from row `row0` on, of tiles of keys (or values) with a
+// row stride in elements.  The lanes' offsets are worked out once; rows past the range's last one are
+// read as that one (and get no weight).
+template <int D, int N>
+struct Copies {
+  static constexpr int kRows = 64 / (D / 8);
+  uint32_t off[N];
+  static __device__ __forceinline__ uint32_t chunk(int r, int lane) {
+    return swz<D>(r, lane % (D / 8)) * 16;
+  }
+  __device__ __forceinline__ void init(uint32_t row_bytes, int row0, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = row0 + i * kRows + lane / (D / 8);
+      off[i] = r * row_bytes + chunk(r, lane);
+    }
+  }
+  // left: rows of the range from the tile's first on
+  __device__ __forceinline__ void issue(const short* tile, uint32_t row_bytes, int tile_rows, int left,
+                                        int row0, int lane, uint32_t lds) const {
+    const short* base = scalar(tile);
+    if (left >= tile_rows) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) lds_dma16(base, off[i], lds + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = row0 + i * kRows + lane / (D / 8);
+        lds_dma16(base, min(r, left - 1) * row_bytes + chunk(r, lane), lds + i * 1024);
+      }
+    }
+  }
+};
 
 // A row tile of up to 32 queries against keys [k0, k1) of a segment; the four waves take the range's
 // tiles in turn, each through LDS buffers of its own (no barrier), and are joined at the end.
-//
-// first_row .. first_row + n_rows - 1 are (token, head of the group) pairs, token-major; own: query i
-// of the tile's tokens sees keys up to first_pos + its token.
+// first_pos: the position of the sequence's first new token; own is false for the prefix.
 template <class E, int D>
-__device__ void few_rows(const Args& a, short* smem, int kvh, int token0, int first_row, int n_rows,
-                         const Segment& seg, int k0, int k1, bool own, int first_pos, int part) {
-  constexpr int kChunks = D / 8;                     // 16-byte chunks of a row
-  constexpr int kCopyRows = 64 / kChunks;            // rows of one copy
-  constexpr int kCopies = kKeys / kCopyRows;         // copies of a K or V tile
-  constexpr int kTileElems = kKeys * D;
+__device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Segment& seg, int k0, int k1,
+                         bool own, int first_pos, int part) {
+  constexpr int kCopies = kFewKeys / Copies<D, 1>::kRows;
+  constexpr int kTileElems = kFewKeys * D;
   const FcvLmAttention& p = a.p;
-  const int group = p.n_heads / p.n_kv_heads;
   const int lane = threadIdx.x & 63, ql = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  const int my_row = first_row + min(ql, n_rows - 1);
-  const int my_token = token0 + my_row / group, my_head = kvh * group + my_row % group;
   s16x8 qf[D / 16];
-  {
-    const short* q = static_cast<const short*>(p.q) + my_token * p.q_row + my_head * p.q_head;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
-      qf[ks] = *reinterpret_cast<const s16x8*>(q + ks * 16 + hl * 8);
-  }
+  load_q<D>(p, rows, ql, hl, qf);
   // first key past the query's view; the wave's smallest decides which tiles need the mask
-  const int limit = own ? min(k1, first_pos + my_row / group + 1) : k1;
+  const int limit = own ? min(k1, first_pos + rows.token(min(ql, rows.count - 1)) - rows.token0 + 1) : k1;
   int low = limit;
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) low = min(low, __shfl_xor(low, off, kWave));
 
   short* ring = smem + wave * 4 * kTileElems;
-  const uint32_t ring_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)ring;
-  const int copy_row = lane / kChunks, copy_pos = lane % kChunks;
+  const uint32_t ring_lds =
+      scalar((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)ring);
+  const uint32_t k_bytes = (uint32_t)seg.k_row * 2, v_bytes = (uint32_t)seg.v_row * 2;
+  Copies<D, kCopies> kc, vc;
+  kc.init(k_bytes, 0, lane);
+  vc.init(v_bytes, 0, lane);
   auto fetch = [&](int kt, int stage) {
-    const short* kb = seg.k + (int64_t)kt * seg.k_row;
-    const short* vb = seg.v + (int64_t)kt * seg.v_row;
     const uint32_t at = ring_lds + stage * 2 * kTileElems * 2;
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int r = i * kCopyRows + copy_row;
-      // keys past the range are read as its last one and get no weight
-      const uint32_t key = (uint32_t)(min(kt + r, k1 - 1) - kt);
-      const uint32_t chunk = (uint32_t)swz<D>(r, copy_pos) * 16;
-      lds_dma16(kb, key * (uint32_t)(seg.k_row * 2) + chunk, at + i * 1024);
-      lds_dma16(vb, key * (uint32_t)(seg.v_row * 2) + chunk, at + kTileElems * 2 + i * 1024);
-    }
+    kc.issue(seg.k + (int64_t)kt * seg.k_row, k_bytes, kFewKeys, k1 - kt, 0, lane, at);
+    vc.issue(seg.v + (int64_t)kt * seg.v_row, v_bytes, kFewKeys, k1 - kt, 0, lane, at + kTileElems * 2);
   };
 
   State<D> st;
   st.reset();
-  int kt = k0 + wave * kKeys, stage = 0;
+  int kt = k0 + wave * kFewKeys, stage = 0;
   if (kt < k1) fetch(kt, 0);
-  for (; kt < k1; kt += kWaves * kKeys, stage ^= 1) {
-    const int next = kt + kWaves * kKeys;
+  for (; kt < k1; kt += kWaves * kFewKeys, stage ^= 1) {
+    const int next = kt + kWaves * kFewKeys;
     if (next < k1) {
       fetch(next, stage ^ 1);
       wait_vmem<2 * kCopies>();
@@ -251,99 +320,205 @@ __device__ void few_rows(const Args& a, short* smem, int kvh, int token0, int fi
       wait_vmem<0>();
     }
     const short* sk = ring + stage * 2 * kTileElems;
-    tile32<E, D>(sk, sk + kTileElems, qf, st, lane, limit - kt, kt + kKeys <= low, a.scale2);
+    tile<E, D, 1>(sk, sk + kTileElems, qf, st, lane, limit - kt, kt + kFewKeys <= low, a.scale2);
     // the tile's reads have returned before its buffer is filled again
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 
   // join the waves: O is [wave][dim][query], a lane's own column
-  const auto lr = __builtin_amdgcn_permlane32_swap(__float_as_uint(st.l), __float_as_uint(st.l), false, false);
-  const float l_wave = __uint_as_float(lr[0]) + __uint_as_float(lr[1]);
+  const float l_wave = half_sum(st.l);
   __syncthreads();  // every wave is done with its buffers
-  float* so = reinterpret_cast<float*>(smem);        // [kWaves][D][kRows]
-  float2* ss = reinterpret_cast<float2*>(so + kWaves * D * kRows);  // [kWaves][kRows]
-  if (hl == 0) ss[wave * kRows + ql] = float2{st.m, l_wave};
+  float* so = reinterpret_cast<float*>(smem);                          // [kWaves][D][kFewRows]
+  float2* ss = reinterpret_cast<float2*>(so + kWaves * D * kFewRows);  // [kWaves][kFewRows]
+  if (hl == 0) ss[wave * kFewRows + ql] = float2{st.m, l_wave};
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int d = dt * 32 + (e >> 2) * 8 + hl * 4 + (e & 3);
-      so[(wave * D + d) * kRows + ql] = st.acc[dt][e];
+      so[(wave * D + d) * kFewRows + ql] = st.acc[dt][e];
     }
   __syncthreads();
   const int64_t rows_all = (int64_t)p.tokens * p.n_heads;
-  for (int i = threadIdx.x; i < n_rows * D; i += 256) {
+  for (int i = threadIdx.x; i < rows.count * D; i += 256) {
     const int r = i / D, d = i % D;
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ss[w * kRows + r].x);
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ss[w * kFewRows + r].x);
     const float base = m == -INFINITY ? 0.0f : m;
     float o = 0.0f, l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float2 s = ss[w * kRows + r];
+      const float2 s = ss[w * kFewRows + r];
       const float f = hw_exp2(s.x - base);
       l = fmaf(s.y, f, l);
-      o = fmaf(so[(w * D + d) * kRows + r], f, o);
+      o = fmaf(so[(w * D + d) * kFewRows + r], f, o);
     }
-    const int row = first_row + r;
-    const int64_t at = (int64_t)part * rows_all + (int64_t)(token0 + row / group) * p.n_heads +
-                       kvh * group + row % group;
+    const int64_t at = part * rows_all + (int64_t)rows.token(r) * p.n_heads + rows.head(r);
     a.part_o[at * D + d] = o;
     if (d == 0) a.part_s[at] = float2{m, l};
   }
   __syncthreads();  // the next row tile fills the buffers again
 }
 
+// A row tile of up to 128 queries, 32 a wave, against keys [k0, k1) of the prefix and [o0, o1) of the
+// sequence's own; all waves share a tile of 64 keys in LDS, the next one on its way.
 template <class E, int D>
-__global__ __launch_bounds__(256) void prefix_attention_kernel(const Args a) {
-  __shared__ __attribute__((aligned(1024))) short smem[kWaves * 4 * kKeys * D + kWaves * kRows * 4];
+__device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Segment& prefix, int k0,
+                          int k1, const Segment& own, int o0, int o1, int first_pos, int part) {
+  constexpr int kCopies = kManyKeys / Copies<D, 1>::kRows / kWaves;  // a wave's, of K and of V
+  constexpr int kTileElems = kManyKeys * D;
+  const FcvLmAttention& p = a.p;
+  const int lane = threadIdx.x & 63, ql = lane & 31, hl = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int my = min(wave * 32 + ql, rows.count - 1);
+
+  s16x8 qf[D / 16];
+  load_q<D>(p, rows, my, hl, qf);
+  const int limit = min(o1, first_pos + rows.token(my) - rows.token0 + 1);
+  int low = limit, high = limit;
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) {
+    low = min(low, __shfl_xor(low, off, kWave));
+    high = max(high, __shfl_xor(high, off, kWave));
+  }
+
+  const int row0 = wave * kCopies * Copies<D, 1>::kRows;
+  const uint32_t lds = scalar(
+      (int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem + wave * kCopies * 1024));
+  State<D> st;
+  st.reset();
+  int stage = 0;
+#pragma unroll 1
+  for (int g = 0; g < 2; ++g) {
+    const Segment seg = g == 0 ? prefix : own;
+    const int begin = g == 0 ? k0 : o0, end = g == 0 ? k1 : o1;
+    if (begin >= end) continue;
+    const uint32_t k_bytes = (uint32_t)seg.k_row * 2, v_bytes = (uint32_t)seg.v_row * 2;
+    Copies<D, kCopies> kc, vc;
+    kc.init(k_bytes, row0, lane);
+    vc.init(v_bytes, row0, lane);
+    auto fetch = [&](int kt, int to) {
+      const uint32_t at = lds + to * 2 * kTileElems * 2;
+      kc.issue(seg.k + (int64_t)kt * seg.k_row, k_bytes, kManyKeys, end - kt, row0, lane, at);
+      vc.issue(seg.v + (int64_t)kt * seg.v_row, v_bytes, kManyKeys, end - kt, row0, lane, at + kTileElems * 2);
+    };
+    fetch(begin, stage);
+    for (int kt = begin; kt < end; kt += kManyKeys, stage ^= 1) {
+      wait_vmem<0>();
+      // every wave's copies of this tile have landed, and every wave has read the one before
+      __syncthreads();
+      if (kt + kManyKeys < end) fetch(kt + kManyKeys, stage ^ 1);
+      if (g == 1 && kt >= high) continue;  // none of the wave's queries sees the tile
+      const short* sk = smem + stage * 2 * kTileElems;
+      tile<E, D, kManyKeys / 32>(sk, sk + kTileElems, qf, st, lane, (g == 0 ? end : limit) - kt,
+                                 kt + kManyKeys <= (g == 0 ? end : low), a.scale2);
+    }
+  }
+
+  const float l = half_sum(st.l);
+  const int r = wave * 32 + ql;
+  if (r < rows.count) {
+    const int token = rows.token(r), head = rows.head(r);
+    if (a.s.direct) {
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      short* out = static_cast<short*>(p.out) + token * p.out_row + head * p.out_head;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          s16x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = E::from_f32(st.acc[dt][4 * g + e] * inv);
+          *reinterpret_cast<s16x4*>(out + dt * 32 + g * 8 + hl * 4) = v;
+        }
+      if (p.lse && hl == 0)
+        p.lse[(int64_t)token * p.n_heads + head] = (st.m - E::kShift + log2f(l)) * 0.6931471805599453f;
+    } else {
+      const int64_t at = (int64_t)part * p.tokens * p.n_heads + (int64_t)token * p.n_heads + head;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(a.part_o + at * D + dt * 32 + g * 8 + hl * 4) =
+              f32x4{st.acc[dt][4 * g], st.acc[dt][4 * g + 1], st.acc[dt][4 * g + 2], st.acc[dt][4 * g + 3]};
+      if (hl == 0) a.part_s[at] = float2{st.m, l};
+    }
+  }
+  __syncthreads();  // the next row tile fills the buffers again
+}
+
+template <int D>
+constexpr int lds_elems() {
+  // few: [kWaves][2][K, V][32][D], and the join's sums behind as many bytes of O; many: [2][K, V][64][D]
+  return kWaves * 4 * kFewKeys * D + kWaves * kFewRows * 4;
+}
+
+template <class E, int D, bool FEW>
+__global__ __launch_bounds__(256, FEW ? 1 : 2) void prefix_attention_kernel(const Args a) {
+  __shared__ __attribute__((aligned(1024))) short smem[FEW ? lds_elems<D>() : 4 * kManyKeys * D];
   const FcvLmAttention& p = a.p;
   const Shape& s = a.s;
   const int group = p.n_heads / p.n_kv_heads;
   int64_t b = blockIdx.x;
-  if (b < s.prefix_blocks) {
-    // key head fastest: the row tiles of one head and range are dealt to one XCD and share its L2
-    const int kvh = (int)(b % p.n_kv_heads);
-    b /= p.n_kv_heads;
-    const int part = (int)(b % s.np), tile = (int)(b / s.np);
-    const int live = p.cu_q ? min(max(p.cu_q[p.batch], 0), p.tokens) : p.tokens;
-    const int first = tile * kRows, rows = min(kRows, live * group - first);
-    if (rows <= 0) return;
-    const int k0 = part * s.prefix_step, k1 = min(k0 + s.prefix_step, p.prefix_len);
-    const Segment seg = {static_cast<const short*>(p.prefix_k) + kvh * p.pk_head,
-                         static_cast<const short*>(p.prefix_v) + kvh * p.pv_head, p.pk_row, p.pv_row};
-    few_rows<E, D>(a, smem, kvh, 0, first, rows, seg, k0, k1, false, 0, part);
-    return;
-  }
-  b -= s.prefix_blocks;
-  const int kvh = (int)(b % p.n_kv_heads);
+  const bool stacked = b < s.prefix_blocks;
+  if (!stacked) b -= s.prefix_blocks;
+  // key head fastest: the row tiles of one head and range are dealt to one XCD and share its L2
+  const int kvh = scalar((int)(b % p.n_kv_heads));
   b /= p.n_kv_heads;
-  const int range = (int)(b % s.no);
-  b /= s.no;
-  const int seq = (int)(b % p.batch), tile0 = (int)(b / p.batch);
-  int t0, t1;
-  if (p.cu_q) {
-    t0 = min(max(p.cu_q[seq], 0), p.tokens);
-    t1 = min(max(p.cu_q[seq + 1], t0), p.tokens);
+  const int ranges = stacked ? s.np : s.no;
+  const int range = scalar((int)(b % ranges));
+  b /= ranges;
+
+  // the rows token0 .. of all sequences or of one, and its keys
+  int token0 = 0, tokens, slot = 0, length = 0, first_tile = (int)b;
+  if (stacked) {
+    tokens = p.cu_q ? min(max(p.cu_q[p.batch], 0), p.tokens) : p.tokens;
   } else {
-    const int n = p.tokens / p.batch;
-    t0 = seq * n;
-    t1 = t0 + n;
+    const int seq = scalar((int)(b % p.batch));
+    first_tile = (int)(b / p.batch);
+    if (p.cu_q) {
+      token0 = min(max(p.cu_q[seq], 0), p.tokens);
+      tokens = min(max(p.cu_q[seq + 1], token0), p.tokens) - token0;
+    } else {
+      tokens = p.tokens / p.batch;
+      token0 = seq * tokens;
+    }
+    slot = p.slots ? p.slots[seq] : seq;
+    length = min(max(p.lengths[seq], 0), p.capacity);
+    if (slot < 0 || slot >= p.sessions) slot = length = 0;
   }
-  const int slot = p.slots ? p.slots[seq] : seq;
-  int length = min(max(p.lengths[seq], 0), p.capacity);
-  if (slot < 0 || slot >= p.sessions) length = 0;
-  const int step = max(s.own_step, (length + s.no - 1) / s.no);
-  const int k0 = min(range * step, length), k1 = min(k0 + step, length);
-  const Segment seg = {
-      static_cast<const short*>(p.k_cache) + (length ? slot * p.k_session : 0) + kvh * p.k_head,
-      static_cast<const short*>(p.v_cache) + (length ? slot * p.v_session : 0) + kvh * p.v_head,
-      p.k_row, p.v_row};
-  const int n_rows = (t1 - t0) * group;
-  for (int first = tile0 * kRows; first < n_rows; first += s.own_tiles * kRows)
-    few_rows<E, D>(a, smem, kvh, t0, first, min(kRows, n_rows - first), seg, k0, k1, true,
-                   length - (t1 - t0), s.np + range);
+  const Segment prefix = {static_cast<const short*>(p.prefix_k) + kvh * p.pk_head,
+                          static_cast<const short*>(p.prefix_v) + kvh * p.pv_head, p.pk_row, p.pv_row};
+  const Segment own = {static_cast<const short*>(p.k_cache) + slot * p.k_session + kvh * p.k_head,
+                       static_cast<const short*>(p.v_cache) + slot * p.v_session + kvh * p.v_head,
+                       p.k_row, p.v_row};
+  // keys [c0, c1) of the prefix (if it is read here) and the sequence's own behind it
+  const int prefix_len = stacked || s.fused ? p.prefix_len : 0;
+  const int total = prefix_len + length;  // below 2^31: both are at most 2^30
+  const int step = stacked ? s.prefix_step : max(s.own_step, (total + s.no - 1) / s.no);
+  const int c0 = (int)min((int64_t)range * step, (int64_t)total);
+  const int c1 = (int)min((int64_t)c0 + step, (int64_t)total);
+  const int part = stacked ? range : s.np + range;
+  const bool many = !FEW || (stacked ? s.prefix_many : s.own_many);
+  const int tile_rows = many ? kManyRows : kFewRows;
+  const int n_rows = tokens * group, first_pos = length - tokens;
+  const int tiles = (n_rows + tile_rows - 1) / tile_rows;
+  const int stride = stacked ? s.prefix_tiles : s.own_tiles;
+  for (int i = scalar(first_tile); i < tiles; i += stride) {
+    const int index = tiles - 1 - i;  // the last tiles see the most keys and go first
+    const int first = index * tile_rows;
+    const Rows rows = {kvh, group, token0, first, min(tile_rows, n_rows - first)};
+    if (many) {
+      // own keys past the tile's last query are not visited
+      const int seen = stacked ? 0 : min(length, first_pos + (first + rows.count - 1) / group + 1);
+      many_rows<E, D>(a, smem, rows, prefix, min(c0, prefix_len), min(c1, prefix_len), own,
+                      max(c0 - prefix_len, 0), min(max(c1 - prefix_len, 0), seen), first_pos, part);
+    } else if constexpr (FEW) {
+      const Segment seg = stacked ? prefix : own;
+      few_rows<E, D>(a, smem, rows, seg, c0, c1, !stacked, first_pos, part);
+    }
+  }
 }
 
 // Joins the parts of each (token, head): one wave to a row, lane l holds dims 2 l, 2 l + 1.
@@ -354,6 +529,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)live * p.n_heads) return;
   const int lane = threadIdx.x & 63, parts = a.s.parts();
+  static_assert(kMaxParts == kWave, "a lane to a part");
   const int64_t rows_all = (int64_t)p.tokens * p.n_heads;
   float2 mine = {-INFINITY, 0.0f};
   if (lane < parts) mine = a.part_s[lane * rows_all + row];
@@ -394,22 +570,37 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 Shape shape_of(const FcvLmAttention& p) {
   Shape s{};
   const int group = p.n_heads / p.n_kv_heads;
-  s.prefix_tiles = ceil_div((int64_t)p.tokens * group, kRows);
-  if (p.prefix_len > 0) {
-    const int blocks = s.prefix_tiles * p.n_kv_heads;
-    const int want = std::max(1, std::min({ceil_div(2 * kCus, blocks), ceil_div(p.prefix_len, 256), 32}));
-    s.prefix_step = ceil_div(ceil_div(p.prefix_len, want), kWaves * kKeys) * kWaves * kKeys;
+  const int64_t seq_rows = std::min<int64_t>(p.max_q, std::max(p.tokens, 1)) * group;
+  const int64_t all_rows = (int64_t)p.tokens * group;
+  const int max_length = std::min(std::max(p.max_length, 1), p.capacity);
+  // Ranges of about equal work, so that the blocks fill the CUs twice.
+  auto cut = [](int keys, int64_t blocks, int least, int unit, int most) {
+    const int64_t want = std::min<int64_t>({(2 * kCus + blocks - 1) / blocks, ceil_div(keys, least), most});
+    return ceil_div(ceil_div(keys, std::max<int64_t>(want, 1)), unit) * unit;
+  };
+  s.own_many = seq_rows > kFewRows;
+  // A sequence with at least a tile of rows of its own reads the prefix with them: nothing is gained by
+  // stacking its rows with others'.
+  s.fused = p.prefix_len == 0 || seq_rows >= kManyRows || (p.batch == 1 && s.own_many);
+  if (!s.fused) {
+    s.prefix_many = all_rows > kFewRows;
+    s.prefix_tiles = ceil_div(all_rows, s.prefix_many ? kManyRows : kFewRows);
+    s.prefix_step = cut(p.prefix_len, (int64_t)s.prefix_tiles * p.n_kv_heads, 256, 128, 32);
     s.np = ceil_div(p.prefix_len, s.prefix_step);
+    s.prefix_blocks = (int64_t)s.prefix_tiles * p.n_kv_heads * s.np;
   }
-  s.own_tiles = std::max(1, ceil_div((int64_t)p.max_q * group, kRows));
-  s.no = std::max(1, std::min(ceil_div(p.max_length, 256), 32));
-  s.own_step = ceil_div(std::max(1, p.max_length), s.no);
-  s.prefix_blocks = (int64_t)s.prefix_tiles * p.n_kv_heads * s.np;
-  s.own_blocks = (int64_t)s.own_tiles * p.n_kv_heads * s.no * p.batch;
+  s.own_tiles = std::max(1, ceil_div(seq_rows, s.own_many ? kManyRows : kFewRows));
+  const int keys = (s.fused ? p.prefix_len : 0) + max_length;
+  const int64_t blocks = (int64_t)s.own_tiles * p.n_kv_heads * p.batch;
+  s.own_step = s.own_many ? cut(keys, blocks, 512, kManyKeys, 32) : cut(keys, blocks, 256, kWaves * kFewKeys, 32);
+  s.no = ceil_div(keys, s.own_step);
+  s.own_blocks = blocks * s.no;
+  s.direct = s.own_many && s.parts() == 1;
   return s;
 }
 
 int64_t sums_bytes(const FcvLmAttention& p, const Shape& s) {
+  if (s.direct) return 0;
   return ((int64_t)s.parts() * p.tokens * p.n_heads * 8 + 255) / 256 * 256;
 }
 
@@ -456,7 +647,11 @@ int check(const FcvLmAttention* p) {
 template <class E, int D>
 void launch(const Args& a, hipStream_t stream) {
   const unsigned blocks = (unsigned)(a.s.prefix_blocks + a.s.own_blocks);
-  hipLaunchKernelGGL((prefix_attention_kernel<E, D>), dim3(blocks), dim3(256), 0, stream, a);
+  if (a.s.own_many && (a.s.np == 0 || a.s.prefix_many))
+    hipLaunchKernelGGL((prefix_attention_kernel<E, D, false>), dim3(blocks), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((prefix_attention_kernel<E, D, true>), dim3(blocks), dim3(256), 0, stream, a);
+  if (a.s.direct) return;
   const int64_t rows = (int64_t)a.p.tokens * a.p.n_heads;
   hipLaunchKernelGGL((join_kernel<E, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
 }
@@ -468,6 +663,7 @@ void launch(const Args& a, hipStream_t stream) {
 extern "C" size_t fcv_lm_prefix_attention_workspace_bytes(const FcvLmAttention* args) {
   if (fcv::lm::check(args) || args->tokens == 0) return 0;
   const fcv::lm::Shape s = fcv::lm::shape_of(*args);
+  if (s.direct) return 0;
   return (size_t)(fcv::lm::sums_bytes(*args, s) +
                   (int64_t)s.parts() * args->tokens * args->n_heads * args->head_dim * 4);
 }
@@ -481,7 +677,8 @@ extern "C" int fcv_lm_prefix_attention(const FcvLmAttention* args, void* workspa
   FCV_CHECK(need == 0 || workspace, FCV_ERR_INVALID, "null workspace");
   FCV_CHECK(workspace_bytes >= need, FCV_ERR_INVALID,
             "workspace too small: need " + std::to_string(need) + " bytes");
-  FCV_CHECK(aligned(workspace, 256), FCV_ERR_INVALID, "workspace must be 256-byte aligned");
+  FCV_CHECK(need == 0 || aligned(workspace, 256), FCV_ERR_INVALID,
+            "workspace must be 256-byte aligned");
   Args a{*args, shape_of(*args), nullptr, nullptr, args->scale * kLog2e};
   a.part_s = static_cast<float2*>(workspace);
   a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_bytes(*args, a.s));

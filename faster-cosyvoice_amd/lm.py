@@ -316,6 +316,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         dim ** -0.5 if scale is None else scale)
     lib = _lib.load()
     need = lib.fcv_lm_prefix_attention_workspace_bytes(args)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _launch(lib.fcv_lm_prefix_attention, q.device, args, ws.data_ptr(), need)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _launch(lib.fcv_lm_prefix_attention, q.device, args, ws.data_ptr(), need)
+    else:
+        _launch(lib.fcv_lm_prefix_attention, q.device, args, None, 0)
     return (out, lse) if return_lse else out

@@ -45,8 +45,8 @@ def norm_rope(y, size, dim, normed, dtype):
 
 def attention(out, mass, score, keys, dim, dtype, v_max):
     """Scores are off by (dim + 4) U score; twice that relative in a weight (numerator and
-    denominator).  A weight is rounded to T: eps(T) / 2 relative.  fp16 weights are held at 2^15
-    times their size, so one below fp16's normal numbers (2^-14) is below 2^-29 of the row's
+    denominator).  A weight is rounded to T: eps(T) / 2 relative.  fp16 weights are held at 2^11
+    times their size, so one below fp16's normal numbers (2^-14) is below 2^-25 of the row's
     largest and off by at most that, read as zero or not.  Sums of `keys` weights and of the parts:
     (keys + 64) U."""
     score, keys = score[..., None], keys[..., None]
@@ -54,7 +54,7 @@ def attention(out, mass, score, keys, dim, dtype, v_max):
     rel = eps + 2 * ((dim + 4) * score + 8 + keys + 64) * U
     err = rel * mass
     if dtype == torch.float16:
-        err = err + keys * 2.0 ** -29 * v_max
+        err = err + keys * 2.0 ** -25 * v_max
     return (err + rounding(out.abs() + err, dtype)) * (1 + 2 ** -8)
 
 

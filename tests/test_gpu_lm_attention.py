@@ -187,8 +187,8 @@ def test_strides_and_padding(fcv):
     q = torch.full((11, hq, dim), float("nan"), dtype=dtype, device=DEV)
     q[:6] = a["q"]
     out = torch.full((11, hq, dim + 8), 7.0, dtype=dtype, device=DEV)
-    got = fcv.prefix_attention(**dict(a, q=q), max_q=3, out=out[..., :dim])
-    assert got.data_ptr() == out.data_ptr() and torch.equal(got[:6], want)
+    got, _ = check(fcv, dict(a, q=q), "padded", max_q=3, out=out[..., :dim])
+    assert got.data_ptr() == out.data_ptr()
     assert (out[6:] == 7).all() and (out[..., dim:] == 7).all()
     # two sequences that read one session, and one prefix head for all (stride 0)
     c = dict(a, slots=a["slots"].clone())
