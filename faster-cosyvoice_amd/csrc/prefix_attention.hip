@@ -65,16 +65,21 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+__device__ __forceinline__ uint32_t lds_base(short* smem) {
+  return (uint32_t)scalar((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem);
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vmem() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// LDS position of 16-byte chunk c of row r: 16 consecutive rows read at one chunk index, and the
-// 4 x 16 blocks of the transposed reads, spread over all banks.
+// LDS position of 16-byte chunk c of row r.  The keys' reads (16 rows at one chunk index) and the
+// transposed reads of values (four rows at four neighbouring chunks) both touch all banks: the row's low
+// bits choose the group of four chunks, its next two the chunk in the group.
 template <int D>
 __device__ __forceinline__ int swz(int r, int c) {
-  return D == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15);
+  return D == 64 ? c ^ ((r & 2) << 1 | ((r >> 2) & 3)) : c ^ ((r & 3) << 2 | ((r >> 2) & 3));
 }
 
 // The keys and values of one head of the prefix or of one session.
@@ -99,55 +104,89 @@ struct State {
   }
 };
 
-// V^T fragment of MFMA step st (16 keys) and dims 32 dt .. + 31: slot j of lane l is value
-// [16 st + 8 (j / 4) + 4 (l / 32) + j % 4][32 dt + l % 32], the keys of P's slots.
+// LDS addresses of a tile's fragments, for the tile whose keys (or values) start at byte `base`, a
+// multiple of 256.  In swz, a row's bits and a chunk's are joined by exclusive or, so that a lane's
+// addresses differ from its first by constants in the low byte and in the instruction's offset.
+typedef __attribute__((address_space(3))) const s16x8* lds16;
+typedef __attribute__((address_space(3))) s16x4* lds8;
+
+// K fragment of step ks (16 dims) of keys 32 t .. + 31: lane l holds key 32 t + l % 32, dims 16 ks +
+// 8 (l / 32) .. + 7.
 template <int D>
-__device__ __forceinline__ s16x8 v_fragment(const short* sv, int lane, int st, int dt) {
-  const int i = lane & 15, g = lane >> 4;
-  const int row = st * 16 + (g >> 1) * 4 + (i >> 2);
-  const int chunk = dt * 4 + (g & 1) * 2 + ((i & 3) >> 1);
-  typedef __attribute__((address_space(3))) s16x4* lds4;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lds4)(sv + row * D + swz<D>(row, chunk) * 8 + (i & 1) * 4));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lds4)(sv + (row + 8) * D + swz<D>(row + 8, chunk) * 8 + (i & 1) * 4));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+struct KeyFragments {
+  uint32_t at;
+  __device__ __forceinline__ KeyFragments(uint32_t base, int lane)
+      : at(base + (lane & 31) * (2 * D) + swz<D>(lane & 31, lane >> 5) * 16) {}
+  __device__ __forceinline__ s16x8 get(int t, int ks) const {
+    return *(lds16)((at ^ (uint32_t)(ks << 5)) + t * 64 * D);
+  }
+};
+
+// V^T fragment of step k (16 keys) and dims 32 dt .. + 31: slot j of lane l is value
+// [16 k + 8 (j / 4) + 4 (l / 32) + j % 4][32 dt + l % 32], the keys of P's slots.
+template <int D>
+struct ValueFragments {
+  uint32_t at;
+  __device__ __forceinline__ ValueFragments(uint32_t base, int lane) {
+    const int i = lane & 15, g = lane >> 4, row = (g >> 1) * 4 + (i >> 2);
+    at = base + row * (2 * D) + swz<D>(row, (g & 1) * 2 + ((i & 3) >> 1)) * 16 + (i & 1) * 8;
+  }
+  __device__ __forceinline__ s16x8 get(int k, int dt) const {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)((at ^ (uint32_t)(dt << 6)) + k * 32 * D));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds8)((at ^ (uint32_t)(dt << 6 | 32)) + k * 32 * D + 16 * D));  // eight rows on
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+// v with zeros in the place of infinities and NaN, whose presence is noted in `found`.
+template <class E>
+__device__ __forceinline__ s16x8 finite_only(const s16x8& v, uint32_t& found) {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u16x8 size = __builtin_bit_cast(u16x8, v) & (unsigned short)0x7fff;
+  const u16x8 past = __builtin_elementwise_sub_sat(size, (u16x8)(unsigned short)(E::kInf - 1));
+  const u32x4 p = __builtin_bit_cast(u32x4, past);
+  found |= (p[0] | p[1]) | (p[2] | p[3]);
+  const u16x8 keep = __builtin_elementwise_min(past, (u16x8)(unsigned short)1) - (unsigned short)1;
+  return __builtin_bit_cast(s16x8, __builtin_bit_cast(u16x8, v) & keep);
 }
 
-// Whether the lane reads an infinity or a NaN among the values of a tile of 32 KT keys.
-template <class E, int D, int KT>
-__device__ __forceinline__ bool not_finite(const short* sv, int lane) {
-  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
-  u16x8 top = {};
-#pragma unroll 4
-  for (int i = 0; i < KT * D / 16; ++i)
-    top = __builtin_elementwise_max(
-        top, *reinterpret_cast<const u16x8*>(sv + (i * 64 + lane) * 8) & (unsigned short)0x7fff);
-  unsigned short most = 0;
+// What the finite_only of a row's visible keys [from, to) took from value dims d .. d + 3: the row gets
+// it back once its sums are done (a 0 weight on a hidden infinity would be NaN).  Seldom runs.
+template <class E>
+__device__ __forceinline__ f32x4 not_finite4(const short* v, int64_t v_row, int from, int to, int d) {
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int key = from; key < to; ++key) {
+    const s16x4 x = *reinterpret_cast<const s16x4*>(v + key * v_row + d);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) most = most > top[e] ? most : top[e];
-  return most >= (unsigned short)E::kInf;
+    for (int e = 0; e < 4; ++e)
+      if ((x[e] & E::kInf) == E::kInf) sum[e] += E::to_f32(x[e]);
+  }
+  return sum;
 }
 
 // One tile of 32 KT keys from LDS.  `limit` (per lane) is the first key of the tile that the lane's
-// query does not see; all_visible says that no lane has one.
-template <class E, int D, int KT>
-__device__ __forceinline__ void tile(const short* sk, const short* sv, const s16x8 (&qf)[D / 16],
-                                     State<D>& st, int lane, int limit, bool all_visible,
-                                     float scale2) {
-  const int ql = lane & 31, hl = lane >> 5;
+// query does not see; all_visible says that no lane has one.  With hide, values that are not finite are
+// left out and noted in `found`.
+// keys_read() is called once the keys have been read, values_here() before the first value is.
+template <class E, int D, int KT, class F, class G>
+__device__ __forceinline__ void tile(uint32_t sk, uint32_t sv, const s16x8 (&qf)[D / 16],
+                                     State<D>& st, int lane, int limit, bool all_visible, bool hide,
+                                     uint32_t& found, float scale2, const F& keys_read, const G& values_here) {
+  const int hl = lane >> 5;
+  const KeyFragments<D> keys(sk, lane);
   f32x16 s[KT];
 #pragma unroll
-  for (int t = 0; t < KT; ++t) {
+  for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
+  // sums that do not wait for one another are taken in turn
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      const int row = t * 32 + ql;
-      const s16x8 kf = *reinterpret_cast<const s16x8*>(sk + row * D + swz<D>(row, ks * 2 + hl) * 8);
-      s[t] = E::mfma32(kf, qf[ks], s[t]);
-    }
-  }
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int t = 0; t < KT; ++t) s[t] = E::mfma32(keys.get(t, ks), qf[ks], s[t]);
+  keys_read();
   if (!all_visible) {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
@@ -155,12 +194,12 @@ __device__ __forceinline__ void tile(const short* sk, const short* sv, const s16
       for (int e = 0; e < 16; ++e)
         s[t][e] = t * 32 + (e >> 2) * 8 + hl * 4 + (e & 3) < limit ? s[t][e] : -INFINITY;
   }
-  float top = s[0][0];
+  float tops[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
   for (int t = 0; t < KT; ++t)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
-  top = half_max(top) * scale2;
+    for (int e = 0; e < 16; ++e) tops[e & 3] = fmaxf(tops[e & 3], s[t][e]);
+  const float top = half_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))) * scale2;
   if (__any(top > st.m + E::kLag)) {
     const float m_new = top > st.m + E::kLag ? top : st.m;
     // a query that has seen no finite score yet keeps m = -inf (and sums of 0)
@@ -173,53 +212,34 @@ __device__ __forceinline__ void tile(const short* sk, const short* sv, const s16
       for (int e = 0; e < 16; ++e) st.acc[dt][e] *= corr;
   }
   const float shift = E::kShift - (st.m == -INFINITY ? 0.0f : st.m);
-  float sum = 0.0f;
+  float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   s16x8 pf[2 * KT];
 #pragma unroll
   for (int t = 0; t < KT; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float w = hw_exp2(fmaf(s[t][e], scale2, shift));
-      sum += w;
+      sums[e & 3] += w;
       // 16-bit weights (relative error 2^-9 bf16, 2^-12 fp16, each with its own sign): what the
       // matrix instruction takes; the sum keeps the unrounded ones
       pf[t * 2 + (e >> 3)][e & 7] = E::from_f32(w);
     }
-  st.l += sum;
-  if (!all_visible && __any(not_finite<E, D, KT>(sv, lane))) {
-    // 0 * inf and 0 * NaN: a value that is not finite is taken out of the product, and the queries that
-    // see its key get +-big * big = +-inf instead (both for a NaN), in bf16, which spans fp32's range
-    constexpr short kBig = 0x7F00;  // 2^127
+  st.l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  values_here();
+  const ValueFragments<D> values(sv, lane);
+  if (hide) {
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) {
+    for (int k = 0; k < 2 * KT; ++k)
 #pragma unroll
-      for (int k = 0; k < 2 * KT; ++k) {
-        // one at a time, nothing of it computed ahead: this must not cost the usual path registers
-        int lane_here = lane, limit_here = limit;
-        asm volatile("" : "+v"(lane_here), "+v"(limit_here));
-        s16x8 vf = v_fragment<D>(sv, lane_here, k, dt), up = {}, down = {}, seen;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const short v = vf[e];
-          const bool bad = (v & E::kInf) == E::kInf, nan = bad && (v & 0x7fff) != E::kInf;
-          vf[e] = bad ? (short)0 : v;
-          up[e] = nan || (bad && v > 0) ? kBig : (short)0;
-          down[e] = nan || (bad && v < 0) ? (short)(kBig | 0x8000) : (short)0;
-          seen[e] = k * 16 + (e >> 2) * 8 + (lane_here >> 5) * 4 + (e & 3) < limit_here ? kBig : (short)0;
-        }
-        st.acc[dt] = E::mfma32(vf, pf[k], st.acc[dt]);
-        st.acc[dt] = Bf16::mfma32(up, seen, st.acc[dt]);
-        st.acc[dt] = Bf16::mfma32(down, seen, st.acc[dt]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
+      for (int dt = 0; dt < D / 32; ++dt)
+        st.acc[dt] = E::mfma32(finite_only<E>(values.get(k, dt), found), pf[k], st.acc[dt]);
     return;
   }
 #pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt)
+  for (int k = 0; k < 2 * KT; ++k)
 #pragma unroll
-    for (int k = 0; k < 2 * KT; ++k)
-      st.acc[dt] = E::mfma32(v_fragment<D>(sv, lane, k, dt), pf[k], st.acc[dt]);
+    for (int dt = 0; dt < D / 32; ++dt)
+      st.acc[dt] = E::mfma32(values.get(k, dt), pf[k], st.acc[dt]);
 }
 
 // The queries of a row tile: rows first .. first + count - 1 of the (token, head of the group) pairs of
@@ -240,39 +260,30 @@ __device__ __forceinline__ void load_q(const FcvLmAttention& p, const Rows& rows
     qf[ks] = *reinterpret_cast<const s16x8*>(q + ks * 16 + hl * 8);
 }
 
-// Copies of one wave: N times 64 / (D / 8) rows, from row `row0` on, of tiles of keys (or values) with a
-// row stride in elements.  The lanes' offsets are worked out once; rows past the range's last one are
-// read as that one (and get no weight).
+// Copies of one wave: N times 64 / (D / 8) rows, from row `row0` (a multiple of 16) on, of a tile of
+// `tile_rows` keys (or values) with a row stride in bytes.  left: rows of the range from the tile's first
+// on; rows past it are read as its last one (and get no weight).
 template <int D, int N>
-struct Copies {
-  static constexpr int kRows = 64 / (D / 8);
-  uint32_t off[N];
-  static __device__ __forceinline__ uint32_t chunk(int r, int lane) {
-    return swz<D>(r, lane % (D / 8)) * 16;
-  }
-  __device__ __forceinline__ void init(uint32_t row_bytes, int row0, int lane) {
+__device__ __forceinline__ void copy_rows(const short* tile, uint32_t row_bytes, int tile_rows, int left,
+                                          int row0, int lane, uint32_t lds) {
+  constexpr int kChunks = D / 8, kRows = 64 / kChunks;
+  const int r0 = lane / kChunks;
+  const uint32_t chunk = swz<D>(r0, lane % kChunks) * 16;
+  if (left >= tile_rows) {
+    const char* base = reinterpret_cast<const char*>(scalar(tile)) + (int64_t)row0 * row_bytes;
+    const uint32_t row = r0 * row_bytes;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = row0 + i * kRows + lane / (D / 8);
-      off[i] = r * row_bytes + chunk(r, lane);
-    }
-  }
-  // left: rows of the range from the tile's first on
-  __device__ __forceinline__ void issue(const short* tile, uint32_t row_bytes, int tile_rows, int left,
-                                        int row0, int lane, uint32_t lds) const {
-    const short* base = scalar(tile);
-    if (left >= tile_rows) {
+    for (int i = 0; i < N; ++i)  // kRows further on, the position's bits 2 and up count i
+      lds_dma16(base + (int64_t)(i * kRows) * row_bytes, row + (chunk ^ (uint32_t)swz<D>(i * kRows, 0) * 16),
+                lds + i * 1024);
+  } else {
+    const char* base = reinterpret_cast<const char*>(scalar(tile));
 #pragma unroll
-      for (int i = 0; i < N; ++i) lds_dma16(base, off[i], lds + i * 1024);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int r = row0 + i * kRows + lane / (D / 8);
-        lds_dma16(base, min(r, left - 1) * row_bytes + chunk(r, lane), lds + i * 1024);
-      }
-    }
+    for (int i = 0; i < N; ++i)
+      lds_dma16(base, min(row0 + i * kRows + r0, left - 1) * row_bytes +
+                          (chunk ^ (uint32_t)swz<D>(i * kRows, 0) * 16), lds + i * 1024);
   }
-};
+}
 
 // A row tile of up to 32 queries against keys [k0, k1) of a segment; the four waves take the range's
 // tiles in turn, each through LDS buffers of its own (no barrier), and are joined at the end.
@@ -280,7 +291,7 @@ struct Copies {
 template <class E, int D>
 __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Segment& seg, int k0, int k1,
                          bool own, int first_pos, int part) {
-  constexpr int kCopies = kFewKeys / Copies<D, 1>::kRows;
+  constexpr int kCopies = kFewKeys / (512 / D);
   constexpr int kTileElems = kFewKeys * D;
   const FcvLmAttention& p = a.p;
   const int lane = threadIdx.x & 63, ql = lane & 31, hl = lane >> 5;
@@ -294,35 +305,41 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) low = min(low, __shfl_xor(low, off, kWave));
 
-  short* ring = smem + wave * 4 * kTileElems;
-  const uint32_t ring_lds =
-      scalar((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)ring);
+  // a wave's two buffers hold a tile's keys and its values; each is filled again as soon as it was read
+  const uint32_t sk = lds_base(smem) + wave * 2 * kTileElems * 2, sv = sk + kTileElems * 2;
   const uint32_t k_bytes = (uint32_t)seg.k_row * 2, v_bytes = (uint32_t)seg.v_row * 2;
-  Copies<D, kCopies> kc, vc;
-  kc.init(k_bytes, 0, lane);
-  vc.init(v_bytes, 0, lane);
-  auto fetch = [&](int kt, int stage) {
-    const uint32_t at = ring_lds + stage * 2 * kTileElems * 2;
-    kc.issue(seg.k + (int64_t)kt * seg.k_row, k_bytes, kFewKeys, k1 - kt, 0, lane, at);
-    vc.issue(seg.v + (int64_t)kt * seg.v_row, v_bytes, kFewKeys, k1 - kt, 0, lane, at + kTileElems * 2);
+  auto fetch_k = [&](int kt) {
+    copy_rows<D, kCopies>(seg.k + (int64_t)kt * seg.k_row, k_bytes, kFewKeys, k1 - kt, 0, lane, sk);
+  };
+  auto fetch_v = [&](int kt) {
+    copy_rows<D, kCopies>(seg.v + (int64_t)kt * seg.v_row, v_bytes, kFewKeys, k1 - kt, 0, lane, sv);
   };
 
   State<D> st;
   st.reset();
-  int kt = k0 + wave * kFewKeys, stage = 0;
-  if (kt < k1) fetch(kt, 0);
-  for (; kt < k1; kt += kWaves * kFewKeys, stage ^= 1) {
+  uint32_t found = 0;
+  int kt = k0 + wave * kFewKeys;
+  if (kt < k1) {
+    fetch_k(kt);
+    fetch_v(kt);
+  }
+  for (; kt < k1; kt += kWaves * kFewKeys) {
     const int next = kt + kWaves * kFewKeys;
-    if (next < k1) {
-      fetch(next, stage ^ 1);
-      wait_vmem<2 * kCopies>();
-    } else {
-      wait_vmem<0>();
-    }
-    const short* sk = ring + stage * 2 * kTileElems;
-    tile<E, D, 1>(sk, sk + kTileElems, qf, st, lane, limit - kt, kt + kFewKeys <= low, a.scale2);
-    // the tile's reads have returned before its buffer is filled again
+    wait_vmem<kCopies>();  // the keys are here, the values may be on their way
+    tile<E, D, 1>(
+        sk, sv, qf, st, lane, limit - kt, kt + kFewKeys <= low, own && kt + kFewKeys > low, found, a.scale2,
+        [&] {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads have returned
+          if (next < k1) fetch_k(next);
+        },
+        [&] {
+          if (next < k1)
+            wait_vmem<kCopies>();
+          else
+            wait_vmem<0>();
+        });
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next < k1) fetch_v(next);
   }
 
   // join the waves: O is [wave][dim][query], a lane's own column
@@ -330,6 +347,7 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
   __syncthreads();  // every wave is done with its buffers
   float* so = reinterpret_cast<float*>(smem);                          // [kWaves][D][kFewRows]
   float2* ss = reinterpret_cast<float2*>(so + kWaves * D * kFewRows);  // [kWaves][kFewRows]
+  const bool any_found = __syncthreads_or(found != 0);
   if (hl == 0) ss[wave * kFewRows + ql] = float2{st.m, l_wave};
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
@@ -354,6 +372,11 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
       l = fmaf(s.y, f, l);
       o = fmaf(so[(w * D + d) * kFewRows + r], f, o);
     }
+    if (any_found) {
+      const int from = max(k0, k0 + (low - k0) / kFewKeys * kFewKeys);  // the first tile with a mask
+      const int to = min(k1, first_pos + rows.token(r) - rows.token0 + 1);
+      o += not_finite4<E>(seg.v, seg.v_row, from, to, d & ~3)[d & 3];
+    }
     const int64_t at = part * rows_all + (int64_t)rows.token(r) * p.n_heads + rows.head(r);
     a.part_o[at * D + d] = o;
     if (d == 0) a.part_s[at] = float2{m, l};
@@ -366,7 +389,7 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
 template <class E, int D>
 __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Segment& prefix, int k0,
                           int k1, const Segment& own, int o0, int o1, int first_pos, int part) {
-  constexpr int kCopies = kManyKeys / Copies<D, 1>::kRows / kWaves;  // a wave's, of K and of V
+  constexpr int kCopies = kManyKeys / (512 / D) / kWaves;  // a wave's, of K and of V
   constexpr int kTileElems = kManyKeys * D;
   const FcvLmAttention& p = a.p;
   const int lane = threadIdx.x & 63, ql = lane & 31, hl = lane >> 5;
@@ -383,11 +406,11 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
     high = max(high, __shfl_xor(high, off, kWave));
   }
 
-  const int row0 = wave * kCopies * Copies<D, 1>::kRows;
-  const uint32_t lds = scalar(
-      (int)((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem + wave * kCopies * 1024));
+  const int row0 = wave * kCopies * (512 / D);
+  const uint32_t lds = lds_base(smem);
   State<D> st;
   st.reset();
+  uint32_t found = 0;
   int stage = 0;
 #pragma unroll 1
   for (int g = 0; g < 2; ++g) {
@@ -395,13 +418,11 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
     const int begin = g == 0 ? k0 : o0, end = g == 0 ? k1 : o1;
     if (begin >= end) continue;
     const uint32_t k_bytes = (uint32_t)seg.k_row * 2, v_bytes = (uint32_t)seg.v_row * 2;
-    Copies<D, kCopies> kc, vc;
-    kc.init(k_bytes, row0, lane);
-    vc.init(v_bytes, row0, lane);
     auto fetch = [&](int kt, int to) {
-      const uint32_t at = lds + to * 2 * kTileElems * 2;
-      kc.issue(seg.k + (int64_t)kt * seg.k_row, k_bytes, kManyKeys, end - kt, row0, lane, at);
-      vc.issue(seg.v + (int64_t)kt * seg.v_row, v_bytes, kManyKeys, end - kt, row0, lane, at + kTileElems * 2);
+      const uint32_t at = lds + to * 2 * kTileElems * 2 + wave * kCopies * 1024;
+      copy_rows<D, kCopies>(seg.k + (int64_t)kt * seg.k_row, k_bytes, kManyKeys, end - kt, row0, lane, at);
+      copy_rows<D, kCopies>(seg.v + (int64_t)kt * seg.v_row, v_bytes, kManyKeys, end - kt, row0, lane,
+                            at + kTileElems * 2);
     };
     fetch(begin, stage);
     for (int kt = begin; kt < end; kt += kManyKeys, stage ^= 1) {
@@ -410,12 +431,24 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
       __syncthreads();
       if (kt + kManyKeys < end) fetch(kt + kManyKeys, stage ^ 1);
       if (g == 1 && kt >= high) continue;  // none of the wave's queries sees the tile
-      const short* sk = smem + stage * 2 * kTileElems;
-      tile<E, D, kManyKeys / 32>(sk, sk + kTileElems, qf, st, lane, (g == 0 ? end : limit) - kt,
-                                 kt + kManyKeys <= (g == 0 ? end : low), a.scale2);
+      const uint32_t sk = lds + stage * 2 * kTileElems * 2;
+      tile<E, D, kManyKeys / 32>(sk, sk + kTileElems * 2, qf, st, lane, (g == 0 ? end : limit) - kt,
+                                 kt + kManyKeys <= (g == 0 ? end : low), g == 1 && kt + kManyKeys > low,
+                                 found, a.scale2, [] {}, [] {});
     }
   }
 
+  if (__any(found != 0)) {
+    const int from = max(o0, o0 + (low - o0) / kManyKeys * kManyKeys);  // the first tile with a mask
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = not_finite4<E>(own.v, own.v_row, from, limit, dt * 32 + g * 8 + hl * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.acc[dt][4 * g + e] += v[e];
+      }
+  }
   const float l = half_sum(st.l);
   const int r = wave * 32 + ql;
   if (r < rows.count) {
@@ -450,12 +483,13 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
 
 template <int D>
 constexpr int lds_elems() {
-  // few: [kWaves][2][K, V][32][D], and the join's sums behind as many bytes of O; many: [2][K, V][64][D]
-  return kWaves * 4 * kFewKeys * D + kWaves * kFewRows * 4;
+  // few: [kWaves][K, V][32][D], in the end as many bytes of O and the waves' m and l behind them;
+  // many: [2][K, V][64][D]
+  return kWaves * 2 * kFewKeys * D + kWaves * kFewRows * 4;
 }
 
 template <class E, int D, bool FEW>
-__global__ __launch_bounds__(256, FEW ? 1 : 2) void prefix_attention_kernel(const Args a) {
+__global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const Args a) {
   __shared__ __attribute__((aligned(1024))) short smem[FEW ? lds_elems<D>() : 4 * kManyKeys * D];
   const FcvLmAttention& p = a.p;
   const Shape& s = a.s;
