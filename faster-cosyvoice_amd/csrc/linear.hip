@@ -519,8 +519,17 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const Args a) {
   if (i >= (int64_t)p.m * quads) return;
   const int row = (int)(i / quads), col = (int)(i % quads) * 4;
   f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < a.splits; ++s)
-    v += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)s * p.m + row) * a.part_ld + col);
+  const float* part = a.part + (int64_t)row * a.part_ld + col;
+  const int64_t range = (int64_t)p.m * a.part_ld;
+  for (int s0 = 0; s0 < a.splits; s0 += 4) {  // four asked for at once
+    f32x4 u[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      u[s] = s0 + s < a.splits ? *reinterpret_cast<const f32x4*>(part + (s0 + s) * range)
+                               : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) v += u[s];
+  }
   const bool vec = a.vec && col + 3 < p.n;
   finish4<E>(p, vec, row, col, v, bias4<E>(p, vec, col), residual4<E>(p, vec, row, col));
 }

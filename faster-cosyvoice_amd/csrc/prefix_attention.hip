@@ -13,6 +13,7 @@
 // to 16 bits, are the B operand of O^T = V^T P^T as they stand.  V^T's fragments are read from the
 // row-major tile by ds_read_b64_tr_b16, which hands each of 16 lanes one column of a 4 x 16 block.
 #include <algorithm>
+#include <cmath>
 
 #include "lm.hpp"
 
@@ -25,6 +26,7 @@ constexpr int kFewRows = 32;    // queries of a row tile whose waves share the k
 constexpr int kFewKeys = 32;    // keys of a wave's tile there
 constexpr int kManyRows = 128;  // queries of a row tile whose waves share its queries out, 32 each
 constexpr int kManyKeys = 64;   // keys of a workgroup's tile there
+constexpr int kStackedFew = 256; // stacked rows that tiles of 32 take: one launch with the sequences'
 constexpr int kMaxParts = 64;   // lanes of the joining wave
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -291,6 +293,14 @@ __device__ __forceinline__ void copy_rows(const short* tile, uint32_t row_bytes,
 template <class E, int D>
 __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Segment& seg, int k0, int k1,
                          bool own, int first_pos, int part) {
+  if (k0 >= k1) {  // nothing to sum: no weight, and no output that the join would read
+    if (threadIdx.x < (unsigned)rows.count) {
+      const int64_t at = (int64_t)part * a.p.tokens * a.p.n_heads +
+                         (int64_t)rows.token(threadIdx.x) * a.p.n_heads + rows.head(threadIdx.x);
+      a.part_s[at] = float2{-INFINITY, 0.0f};
+    }
+    return;
+  }
   constexpr int kCopies = kFewKeys / (512 / D);
   constexpr int kTileElems = kFewKeys * D;
   const FcvLmAttention& p = a.p;
@@ -482,15 +492,16 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
 }
 
 template <int D>
-constexpr int lds_elems() {
-  // few: [kWaves][K, V][32][D], in the end as many bytes of O and the waves' m and l behind them;
-  // many: [2][K, V][64][D]
+constexpr int few_elems() {
+  // [kWaves][K, V][32][D], in the end as many bytes of O and the waves' m and l behind them
   return kWaves * 2 * kFewKeys * D + kWaves * kFewRows * 4;
 }
 
-template <class E, int D, bool FEW>
+// The blocks of the stacked rows first, then the sequences'; a launch has those of one kind of tile.
+// (Both kinds in one kernel need more registers than two workgroups a CU have.)
+template <class E, int D, bool MANY>
 __global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const Args a) {
-  __shared__ __attribute__((aligned(1024))) short smem[FEW ? lds_elems<D>() : 4 * kManyKeys * D];
+  __shared__ __attribute__((aligned(1024))) short smem[MANY ? 4 * kManyKeys * D : few_elems<D>()];
   const FcvLmAttention& p = a.p;
   const Shape& s = a.s;
   const int group = p.n_heads / p.n_kv_heads;
@@ -534,8 +545,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const Args a) 
   const int c0 = (int)min((int64_t)range * step, (int64_t)total);
   const int c1 = (int)min((int64_t)c0 + step, (int64_t)total);
   const int part = stacked ? range : s.np + range;
-  const bool many = !FEW || (stacked ? s.prefix_many : s.own_many);
-  const int tile_rows = many ? kManyRows : kFewRows;
+  constexpr int tile_rows = MANY ? kManyRows : kFewRows;
   const int n_rows = tokens * group, first_pos = length - tokens;
   const int tiles = (n_rows + tile_rows - 1) / tile_rows;
   const int stride = stacked ? s.prefix_tiles : s.own_tiles;
@@ -543,56 +553,91 @@ __global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const Args a) 
     const int index = tiles - 1 - i;  // the last tiles see the most keys and go first
     const int first = index * tile_rows;
     const Rows rows = {kvh, group, token0, first, min(tile_rows, n_rows - first)};
-    if (many) {
+    if constexpr (MANY) {
       // own keys past the tile's last query are not visited
       const int seen = stacked ? 0 : min(length, first_pos + (first + rows.count - 1) / group + 1);
       many_rows<E, D>(a, smem, rows, prefix, min(c0, prefix_len), min(c1, prefix_len), own,
                       max(c0 - prefix_len, 0), min(max(c1 - prefix_len, 0), seen), first_pos, part);
-    } else if constexpr (FEW) {
+    } else {
       const Segment seg = stacked ? prefix : own;
       few_rows<E, D>(a, smem, rows, seg, c0, c1, !stacked, first_pos, part);
     }
   }
 }
 
-// Joins the parts of each (token, head): one wave to a row, lane l holds dims 2 l, 2 l + 1.
-template <class E, int D>
+// Joins the parts of each (token, head): W waves to a row, each its share of the parts, eight at a time;
+// lane l holds dims 2 l, 2 l + 1 (of 128) or l.
+template <class E, int D, int W>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
+  __shared__ float sums[4][D];
+  static_assert(kMaxParts == kWave, "a lane to a part");
   const FcvLmAttention& p = a.p;
   const int live = p.cu_q ? min(max(p.cu_q[p.batch], 0), p.tokens) : p.tokens;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)live * p.n_heads) return;
-  const int lane = threadIdx.x & 63, parts = a.s.parts();
-  static_assert(kMaxParts == kWave, "a lane to a part");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = wave % W;
+  const int64_t row = (int64_t)blockIdx.x * (4 / W) + wave / W;
+  if (row >= (int64_t)live * p.n_heads) return;  // W = 4: the whole workgroup
+  const int parts = a.s.parts();
   const int64_t rows_all = (int64_t)p.tokens * p.n_heads;
-  float2 mine = {-INFINITY, 0.0f};
-  if (lane < parts) mine = a.part_s[lane * rows_all + row];
-  float top = mine.x;
+  float2 part = {-INFINITY, 0.0f};
+  if (lane < parts) part = a.part_s[lane * rows_all + row];
+  float top = part.x;
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
-  const float base = top == -INFINITY ? 0.0f : top;
-  const float f = hw_exp2(mine.x - base);
-  const float l = wave_sum(mine.y * f);
-  float o0 = 0.0f, o1 = 0.0f;
-  for (int i = 0; i < parts; ++i) {
-    const float w = __shfl(f, i, kWave);
-    const float* o = a.part_o + (i * rows_all + row) * D;
-    if (D == 128) {
-      const float2 v = reinterpret_cast<const float2*>(o)[lane];
-      o0 = fmaf(v.x, w, o0);
-      o1 = fmaf(v.y, w, o1);
-    } else {
-      o0 = fmaf(o[lane], w, o0);
+  const float f = hw_exp2(part.x - (top == -INFINITY ? 0.0f : top));
+  const float l = wave_sum(part.y * f);
+  float2 o = {0.0f, 0.0f};
+  // a part without weight (a range that a short sequence does not reach) was not written
+  const uint64_t live_parts = __ballot(f != 0.0f);
+  for (int i0 = mine; i0 < parts; i0 += 8 * W) {
+    float2 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * W;
+      v[u] = float2{0.0f, 0.0f};
+      if (i < parts && (live_parts >> i & 1)) {
+        const float* src = a.part_o + (i * rows_all + row) * D;
+        if (D == 128)
+          v[u] = reinterpret_cast<const float2*>(src)[lane];
+        else
+          v[u].x = src[lane];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * W;
+      if (i >= parts) break;
+      const float w = __shfl(f, i, kWave);
+      o.x = fmaf(v[u].x, w, o.x);
+      if (D == 128) o.y = fmaf(v[u].y, w, o.y);
+    }
+  }
+  if constexpr (W > 1) {
+    if (D == 128)
+      reinterpret_cast<float2*>(sums[wave])[lane] = o;
+    else
+      sums[wave][lane] = o.x;
+    __syncthreads();
+    if (wave != 0) return;
+    o = float2{0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (D == 128) {
+        const float2 v = reinterpret_cast<const float2*>(sums[w])[lane];
+        o.x += v.x;
+        o.y += v.y;
+      } else {
+        o.x += sums[w][lane];
+      }
     }
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
   const int token = (int)(row / p.n_heads), head = (int)(row % p.n_heads);
   short* out = static_cast<short*>(p.out) + token * p.out_row + head * p.out_head;
   if (D == 128) {
-    const uint32_t lo = (uint16_t)E::from_f32(o0 * inv), hi = (uint16_t)E::from_f32(o1 * inv);
+    const uint32_t lo = (uint16_t)E::from_f32(o.x * inv), hi = (uint16_t)E::from_f32(o.y * inv);
     reinterpret_cast<uint32_t*>(out)[lane] = lo | hi << 16;
   } else {
-    out[lane] = E::from_f32(o0 * inv);
+    out[lane] = E::from_f32(o.x * inv);
   }
   if (p.lse && lane == 0) p.lse[row] = (top - E::kShift + log2f(l)) * 0.6931471805599453f;
 }
@@ -607,9 +652,13 @@ Shape shape_of(const FcvLmAttention& p) {
   const int64_t seq_rows = std::min<int64_t>(p.max_q, std::max(p.tokens, 1)) * group;
   const int64_t all_rows = (int64_t)p.tokens * group;
   const int max_length = std::min(std::max(p.max_length, 1), p.capacity);
-  // Ranges of about equal work, so that the blocks fill the CUs twice.
-  auto cut = [](int keys, int64_t blocks, int least, int unit, int most) {
-    const int64_t want = std::min<int64_t>({(2 * kCus + blocks - 1) / blocks, ceil_div(keys, least), most});
+  // Keys of a range.  With r ranges a block's chain of tiles takes tile_us * tiles / r and the join about
+  // 0.1 us a part plus the part's bytes, written and read at 4 TB/s; the sum is least at the root of the
+  // quotient.  Beyond `full` blocks more ranges only wait for others.
+  const float part_us = 0.1f + (float)p.tokens * p.n_heads * p.head_dim * 8.0f / 4.0e6f;
+  auto cut = [&](int keys, int unit, float tile_us, int64_t blocks, int64_t full, int most) {
+    const float best = std::sqrt((float)ceil_div(keys, unit) * tile_us / part_us);
+    const int64_t want = std::min<int64_t>({(int64_t)best, std::max<int64_t>(full / blocks, 1), most});
     return ceil_div(ceil_div(keys, std::max<int64_t>(want, 1)), unit) * unit;
   };
   s.own_many = seq_rows > kFewRows;
@@ -617,16 +666,19 @@ Shape shape_of(const FcvLmAttention& p) {
   // stacking its rows with others'.
   s.fused = p.prefix_len == 0 || seq_rows >= kManyRows || (p.batch == 1 && s.own_many);
   if (!s.fused) {
-    s.prefix_many = all_rows > kFewRows;
+    s.prefix_many = all_rows > kStackedFew || s.own_many;
     s.prefix_tiles = ceil_div(all_rows, s.prefix_many ? kManyRows : kFewRows);
-    s.prefix_step = cut(p.prefix_len, (int64_t)s.prefix_tiles * p.n_kv_heads, 256, 128, 32);
+    s.prefix_step = cut(p.prefix_len, s.prefix_many ? kManyKeys : kWaves * kFewKeys, 0.6f,
+                        (int64_t)s.prefix_tiles * p.n_kv_heads, 2 * kCus, 32);
     s.np = ceil_div(p.prefix_len, s.prefix_step);
     s.prefix_blocks = (int64_t)s.prefix_tiles * p.n_kv_heads * s.np;
   }
   s.own_tiles = std::max(1, ceil_div(seq_rows, s.own_many ? kManyRows : kFewRows));
   const int keys = (s.fused ? p.prefix_len : 0) + max_length;
   const int64_t blocks = (int64_t)s.own_tiles * p.n_kv_heads * p.batch;
-  s.own_step = s.own_many ? cut(keys, blocks, 512, kManyKeys, 32) : cut(keys, blocks, 256, kWaves * kFewKeys, 32);
+  // sequences differ in length: their ranges are dealt out in several rounds where they are short
+  s.own_step = s.own_many ? cut(keys, kManyKeys, 0.6f, blocks, 2 * kCus, 32)
+                          : cut(keys, kWaves * kFewKeys, 1.2f, blocks, 8 * kCus, 32);
   s.no = ceil_div(keys, s.own_step);
   s.own_blocks = blocks * s.no;
   s.direct = s.own_many && s.parts() == 1;
@@ -679,15 +731,32 @@ int check(const FcvLmAttention* p) {
 }
 
 template <class E, int D>
-void launch(const Args& a, hipStream_t stream) {
-  const unsigned blocks = (unsigned)(a.s.prefix_blocks + a.s.own_blocks);
-  if (a.s.own_many && (a.s.np == 0 || a.s.prefix_many))
-    hipLaunchKernelGGL((prefix_attention_kernel<E, D, false>), dim3(blocks), dim3(256), 0, stream, a);
+void launch_tiles(bool many, const Args& a, int64_t blocks, hipStream_t stream) {
+  if (many)
+    hipLaunchKernelGGL((prefix_attention_kernel<E, D, true>), dim3((unsigned)blocks), dim3(256), 0,
+                       stream, a);
   else
-    hipLaunchKernelGGL((prefix_attention_kernel<E, D, true>), dim3(blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((prefix_attention_kernel<E, D, false>), dim3((unsigned)blocks), dim3(256), 0,
+                       stream, a);
+}
+
+template <class E, int D>
+void launch(const Args& a, hipStream_t stream) {
+  if (a.s.np == 0 || a.s.prefix_many == a.s.own_many) {
+    launch_tiles<E, D>(a.s.own_many, a, a.s.prefix_blocks + a.s.own_blocks, stream);
+  } else {
+    launch_tiles<E, D>(a.s.prefix_many, a, a.s.prefix_blocks, stream);
+    Args own = a;
+    own.s.prefix_blocks = 0;
+    launch_tiles<E, D>(a.s.own_many, own, a.s.own_blocks, stream);
+  }
   if (a.s.direct) return;
+  // a workgroup to a row where there are more parts than one wave asks for at once
   const int64_t rows = (int64_t)a.p.tokens * a.p.n_heads;
-  hipLaunchKernelGGL((join_kernel<E, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
+  if (a.s.parts() > 8)
+    hipLaunchKernelGGL((join_kernel<E, D, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((join_kernel<E, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
 }
 
 }  // namespace
