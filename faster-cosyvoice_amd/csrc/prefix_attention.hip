@@ -26,7 +26,7 @@ constexpr int kFewRows = 32;    // queries of a row tile whose waves share the k
 constexpr int kFewKeys = 32;    // keys of a wave's tile there
 constexpr int kManyRows = 128;  // queries of a row tile whose waves share its queries out, 32 each
 constexpr int kManyKeys = 64;   // keys of a workgroup's tile there
-constexpr int kStackedFew = 256; // stacked rows that tiles of 32 take: one launch with the sequences'
+constexpr int kStackedFew = 4096;  // rows of all key heads up to which stacked rows are taken 32 at a time
 constexpr int kMaxParts = 64;   // lanes of the joining wave
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -190,11 +190,13 @@ __device__ __forceinline__ void tile(uint32_t sk, uint32_t sv, const s16x8 (&qf)
     for (int t = 0; t < KT; ++t) s[t] = E::mfma32(keys.get(t, ks), qf[ks], s[t]);
   keys_read();
   if (!all_visible) {
+    int first = limit - hl * 4;
+    asm volatile("" : "+v"(first));  // a branch, not 32 selects in every tile
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        s[t][e] = t * 32 + (e >> 2) * 8 + hl * 4 + (e & 3) < limit ? s[t][e] : -INFINITY;
+        s[t][e] = t * 32 + (e >> 2) * 8 + (e & 3) < first ? s[t][e] : -INFINITY;
   }
   float tops[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
 #pragma unroll
@@ -287,6 +289,13 @@ __device__ __forceinline__ void copy_rows(const short* tile, uint32_t row_bytes,
   }
 }
 
+// LDS in elements: the tiles' keys and values ([kWaves][K, V][32][D], or [2][K, V][64][D]), and over them in
+// the end [kWaves][32] rows of O (16 bytes apart in their banks) with the waves' m and l behind them.
+template <int D>
+constexpr int pitch() { return D + 4; }
+template <int D>
+constexpr int lds_elems() { return kWaves * 32 * (pitch<D>() * 2 + 4); }
+
 // A row tile of up to 32 queries against keys [k0, k1) of a segment; the four waves take the range's
 // tiles in turn, each through LDS buffers of its own (no barrier), and are joined at the end.
 // first_pos: the position of the sequence's first new token; own is false for the prefix.
@@ -352,43 +361,44 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
     if (next < k1) fetch_v(next);
   }
 
-  // join the waves: O is [wave][dim][query], a lane's own column
+  // join the waves: O is [wave][query][dim], four dims of a query a thread
   const float l_wave = half_sum(st.l);
-  __syncthreads();  // every wave is done with its buffers
-  float* so = reinterpret_cast<float*>(smem);                          // [kWaves][D][kFewRows]
-  float2* ss = reinterpret_cast<float2*>(so + kWaves * D * kFewRows);  // [kWaves][kFewRows]
-  const bool any_found = __syncthreads_or(found != 0);
-  if (hl == 0) ss[wave * kFewRows + ql] = float2{st.m, l_wave};
+  const bool any_found = __syncthreads_or(found != 0);  // and every wave is done with its buffers
+  float* so = reinterpret_cast<float*>(smem);
+  float2* ss = reinterpret_cast<float2*>(so + kWaves * kFewRows * pitch<D>());  // [kWaves][kFewRows]
+  if (ql < rows.count) {
+    if (hl == 0) ss[wave * kFewRows + ql] = float2{st.m, l_wave};
 #pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt)
+    for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int d = dt * 32 + (e >> 2) * 8 + hl * 4 + (e & 3);
-      so[(wave * D + d) * kFewRows + ql] = st.acc[dt][e];
-    }
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(so + (wave * kFewRows + ql) * pitch<D>() + dt * 32 + g * 8 + hl * 4) =
+            f32x4{st.acc[dt][4 * g], st.acc[dt][4 * g + 1], st.acc[dt][4 * g + 2], st.acc[dt][4 * g + 3]};
+  }
   __syncthreads();
   const int64_t rows_all = (int64_t)p.tokens * p.n_heads;
-  for (int i = threadIdx.x; i < rows.count * D; i += 256) {
-    const int r = i / D, d = i % D;
+  for (int i = threadIdx.x; i < rows.count * (D / 4); i += 256) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ss[w * kFewRows + r].x);
     const float base = m == -INFINITY ? 0.0f : m;
-    float o = 0.0f, l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const float2 s = ss[w * kFewRows + r];
       const float f = hw_exp2(s.x - base);
       l = fmaf(s.y, f, l);
-      o = fmaf(so[(w * D + d) * kFewRows + r], f, o);
+      o += *reinterpret_cast<const f32x4*>(so + (w * kFewRows + r) * pitch<D>() + d) * f;
     }
     if (any_found) {
       const int from = max(k0, k0 + (low - k0) / kFewKeys * kFewKeys);  // the first tile with a mask
       const int to = min(k1, first_pos + rows.token(r) - rows.token0 + 1);
-      o += not_finite4<E>(seg.v, seg.v_row, from, to, d & ~3)[d & 3];
+      o += not_finite4<E>(seg.v, seg.v_row, from, to, d);
     }
     const int64_t at = part * rows_all + (int64_t)rows.token(r) * p.n_heads + rows.head(r);
-    a.part_o[at * D + d] = o;
+    *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = o;
     if (d == 0) a.part_s[at] = float2{m, l};
   }
   __syncthreads();  // the next row tile fills the buffers again
@@ -415,6 +425,8 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
     low = min(low, __shfl_xor(low, off, kWave));
     high = max(high, __shfl_xor(high, off, kWave));
   }
+  low = scalar(low);
+  high = scalar(high);
 
   const int row0 = wave * kCopies * (512 / D);
   const uint32_t lds = lds_base(smem);
@@ -459,49 +471,48 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
         for (int e = 0; e < 4; ++e) st.acc[dt][4 * g + e] += v[e];
       }
   }
+  // through LDS, 32 lanes (16 of 64 dims) to a row, so that stores cover whole rows
   const float l = half_sum(st.l);
-  const int r = wave * 32 + ql;
-  if (r < rows.count) {
+  __syncthreads();  // every wave is done with the last tile
+  float* so = reinterpret_cast<float*>(smem) + wave * 32 * pitch<D>();
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(so + ql * pitch<D>() + dt * 32 + g * 8 + hl * 4) =
+          f32x4{st.acc[dt][4 * g], st.acc[dt][4 * g + 1], st.acc[dt][4 * g + 2], st.acc[dt][4 * g + 3]};
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  const int d = lane % (D / 4) * 4, mine = wave * 32;
+#pragma unroll 4
+  for (int q0 = 0; q0 < 32; q0 += 256 / D) {
+    const int q = q0 + lane / (D / 4), r = mine + q;
+    const float lr = __shfl(l, q, kWave), mr = __shfl(st.m, q, kWave);
+    if (r >= rows.count) continue;
+    const f32x4 o = *reinterpret_cast<const f32x4*>(so + q * pitch<D>() + d);
     const int token = rows.token(r), head = rows.head(r);
     if (a.s.direct) {
-      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-      short* out = static_cast<short*>(p.out) + token * p.out_row + head * p.out_head;
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          s16x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = E::from_f32(st.acc[dt][4 * g + e] * inv);
-          *reinterpret_cast<s16x4*>(out + dt * 32 + g * 8 + hl * 4) = v;
-        }
-      if (p.lse && hl == 0)
-        p.lse[(int64_t)token * p.n_heads + head] = (st.m - E::kShift + log2f(l)) * 0.6931471805599453f;
+      const float inv = lr > 0.0f || lr != lr ? 1.0f / lr : 0.0f;
+      *reinterpret_cast<s16x4*>(static_cast<short*>(p.out) + token * p.out_row + head * p.out_head + d) =
+          s16x4{E::from_f32(o[0] * inv), E::from_f32(o[1] * inv), E::from_f32(o[2] * inv),
+                E::from_f32(o[3] * inv)};
+      if (p.lse && d == 0)
+        p.lse[(int64_t)token * p.n_heads + head] = (mr - E::kShift + log2f(lr)) * 0.6931471805599453f;
     } else {
-      const int64_t at = (int64_t)part * p.tokens * p.n_heads + (int64_t)token * p.n_heads + head;
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(a.part_o + at * D + dt * 32 + g * 8 + hl * 4) =
-              f32x4{st.acc[dt][4 * g], st.acc[dt][4 * g + 1], st.acc[dt][4 * g + 2], st.acc[dt][4 * g + 3]};
-      if (hl == 0) a.part_s[at] = float2{st.m, l};
+      const int64_t at = ((int64_t)part * p.tokens + token) * p.n_heads + head;
+      *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = o;
+      if (d == 0) a.part_s[at] = float2{mr, lr};
     }
   }
   __syncthreads();  // the next row tile fills the buffers again
-}
-
-template <int D>
-constexpr int few_elems() {
-  // [kWaves][K, V][32][D], in the end as many bytes of O and the waves' m and l behind them
-  return kWaves * 2 * kFewKeys * D + kWaves * kFewRows * 4;
 }
 
 // The blocks of the stacked rows first, then the sequences'; a launch has those of one kind of tile.
 // (Both kinds in one kernel need more registers than two workgroups a CU have.)
 template <class E, int D, bool MANY>
 __global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const Args a) {
-  __shared__ __attribute__((aligned(1024))) short smem[MANY ? 4 * kManyKeys * D : few_elems<D>()];
+  __shared__ __attribute__((aligned(1024))) short smem[lds_elems<D>()];
   const FcvLmAttention& p = a.p;
   const Shape& s = a.s;
   const int group = p.n_heads / p.n_kv_heads;
@@ -666,7 +677,7 @@ Shape shape_of(const FcvLmAttention& p) {
   // stacking its rows with others'.
   s.fused = p.prefix_len == 0 || seq_rows >= kManyRows || (p.batch == 1 && s.own_many);
   if (!s.fused) {
-    s.prefix_many = all_rows > kStackedFew || s.own_many;
+    s.prefix_many = s.own_many || (int64_t)p.tokens * p.n_heads > kStackedFew;
     s.prefix_tiles = ceil_div(all_rows, s.prefix_many ? kManyRows : kFewRows);
     s.prefix_step = cut(p.prefix_len, s.prefix_many ? kManyKeys : kWaves * kFewKeys, 0.6f,
                         (int64_t)s.prefix_tiles * p.n_kv_heads, 2 * kCus, 32);
