@@ -19,6 +19,8 @@ looked at on the host (include/fcv_lm.h says what the kernels make of each).
 
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import _lib
@@ -27,14 +29,33 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1}  # FCV_LM_F16, FCV_LM_BF16
 _F32 = 2                                         # FCV_LM_F32
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
+# The argument structs, packed here rather than through ctypes fields: these calls take a few
+# microseconds on the GPU, and a ctypes struct of 30 fields takes as long to fill.
+_LINEAR = struct.Struct("@5Q4q8i")
+_QK_NORM_ROPE = struct.Struct("@10Q8q11if")
+_ATTENTION = struct.Struct("@10Q14q11if")
+_FNS: dict[str, object] = {}
 
-def _launch(fn, device: torch.device, *args) -> None:
-    """Call a library entry on ``device``'s current stream, with ``device`` current."""
-    index = device.index
-    if index != torch.cuda.current_device():
+
+def _entry(name: str, n_tail: int):
+    """The library entry ``name`` taking a packed struct, then workspace, bytes and stream (or as
+    many of them as it has)."""
+    fn = _FNS.get(name)
+    if fn is None:
+        restype, argtypes = _lib.SIGNATURES[name]
+        proto = _lib.ctypes.CFUNCTYPE(restype, _lib.c_void_p, *argtypes[1:])
+        fn = _FNS[name] = proto((name, _lib.load()))
+        assert len(argtypes) == 1 + n_tail
+    return fn
+
+
+def _launch(fn, index: int, *args) -> None:
+    """Call a library entry on device ``index``'s current stream, with that device current."""
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            return _launch(fn, device, *args)
-    rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc)
 
@@ -67,21 +88,23 @@ def _indices(t: torch.Tensor, name: str, n: int, like: torch.Tensor) -> int:
 
 def _rows(t: torch.Tensor, name: str, width: int) -> tuple[int, int]:
     """Row count and stride of a tensor seen as rows of its last dimension."""
-    if t.shape[-1] != width:
-        raise ValueError(f"{name} must have {width} columns, got {tuple(t.shape)}")
     if t.dim() != 2:
+        if t.shape[-1] != width:
+            raise ValueError(f"{name} must have {width} columns, got {tuple(t.shape)}")
         try:
             t = t.view(-1, width)
         except RuntimeError as e:
             raise ValueError(f"{name}'s leading dimensions {tuple(t.shape[:-1])} do not lie at one "
                              "stride: make it contiguous") from e
-    n, ld = t.shape[0], t.stride(0)
-    if width > 1 and t.stride(1) != 1:
+    n, columns = t.shape
+    if columns != width:
+        raise ValueError(f"{name} must have {width} columns, got {tuple(t.shape)}")
+    ld, step = t.stride()
+    if step != 1 and width > 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
     return n, ld if n > 1 else max(ld, width)
 
 
-@torch.no_grad()
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                  activation: str | None = None, residual: torch.Tensor | None = None,
                  out: torch.Tensor | None = None,
@@ -95,73 +118,82 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     input.  ``activation``: ``"relu"``, ``"silu"``, ``"gelu"`` (erf), ``"gelu_tanh"`` or none.
     Rows may lie at any stride; rows that start on 16-byte boundaries are read faster."""
     code = _dtype(x, "x")
-    if weight.dtype != x.dtype or weight.device != x.device or weight.dim() != 2:
-        raise ValueError(f"weight must be a {x.dtype} matrix on {x.device}")
+    device = x.device
+    if weight.dtype != x.dtype or weight.device != device or weight.dim() != 2:
+        raise ValueError(f"weight must be a {x.dtype} matrix on {device}")
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
     n, k = weight.shape
     if n < 1 or k < 1:
-        raise ValueError(f"weight is empty: {tuple(weight.shape)}")
+        raise ValueError(f"weight is empty: {(n, k)}")
     m, ldx = _rows(x, "x", k)
     _, ldw = _rows(weight, "weight", k)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}")
-    shape = x.shape[:-1] + (n,)
+    shape = (m, n) if x.dim() == 2 else (*x.shape[:-1], n)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype if out_dtype is None else out_dtype,
-                          device=x.device)
-        if out_dtype is not None:
-            out_code = _side(out, "out", x, code)
-        else:
+        if out_dtype is None or out_dtype == x.dtype:
             out_code = code
+        elif out_dtype == torch.float32:
+            out_code = _F32
+        else:
+            raise ValueError(f"out must be {x.dtype} or float32, not {out_dtype}")
+        out = torch.empty(shape, dtype=x.dtype if out_dtype is None else out_dtype, device=device)
         ldy = n
     else:
         if out.shape != shape:
-            raise ValueError(f"out must have shape {tuple(shape)}, got {tuple(out.shape)}")
+            raise ValueError(f"out must have shape {shape}, got {tuple(out.shape)}")
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"out is {out.dtype}, not {out_dtype}")
         out_code = _side(out, "out", x, code)
         _, ldy = _rows(out, "out", n)
         if m > 1 and ldy < n:
             raise ValueError("out's rows overlap")
-    bias_ptr, bias_code = None, code
+    bias_ptr, bias_code = 0, code
     if bias is not None:
         bias_code = _side(bias, "bias", x, code)
         if bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
             raise ValueError(f"bias must be a contiguous vector of {n}")
         bias_ptr = bias.data_ptr()
-    res_ptr, res_code, ldr = None, code, 0
+    res_ptr, res_code, ldr = 0, code, 0
     if residual is not None:
         res_code = _side(residual, "residual", x, code)
         if residual.shape != shape:
-            raise ValueError(f"residual must have shape {tuple(shape)}, got "
+            raise ValueError(f"residual must have shape {shape}, got "
                              f"{tuple(residual.shape)}")
         _, ldr = _rows(residual, "residual", n)
         res_ptr = residual.data_ptr()
     if m == 0:
         return out
-    lib = _lib.load()
-    args = _lib.FcvLmLinear(x.data_ptr(), weight.data_ptr(), bias_ptr, res_ptr, out.data_ptr(),
-                            ldx, ldw, ldr, ldy, m, n, k, code, bias_code, res_code, out_code, act)
-    need = lib.fcv_lm_linear_workspace_bytes(args)
+    args = _LINEAR.pack(x.data_ptr(), weight.data_ptr(), bias_ptr, res_ptr, out.data_ptr(), ldx, ldw,
+                        ldr, ldy, m, n, k, code, bias_code, res_code, out_code, act)
+    need = _entry("fcv_lm_linear_workspace_bytes", 0)(args)
+    fn = _entry("fcv_lm_linear", 3)
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        _launch(lib.fcv_lm_linear, x.device, args, ws.data_ptr(), need)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        _launch(fn, device.index, args, ws.data_ptr(), need)
     else:
-        _launch(lib.fcv_lm_linear, x.device, args, None, 0)
+        _launch(fn, device.index, args, None, 0)
     return out
 
 
-def _cache(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
-    if t.dtype != like.dtype or t.device != like.device or t.dim() != 4 or t.numel() == 0:
-        raise ValueError(f"{name} must be a {like.dtype} tensor [sessions, capacity, kv heads, "
-                         f"head dim] on {like.device}")
-    if t.stride(3) != 1:
-        raise ValueError(f"{name}'s last dimension must be contiguous")
+def _caches(k: torch.Tensor, v: torch.Tensor, like: torch.Tensor):
+    """Shape of a pair of caches, and their strides."""
+    for t, name in ((k, "k_cache"), (v, "v_cache")):
+        if t.dtype != like.dtype or t.device != like.device or t.dim() != 4 or t.numel() == 0:
+            raise ValueError(f"{name} must be a {like.dtype} tensor [sessions, capacity, kv heads, "
+                             f"head dim] on {like.device}")
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if shape != v.shape:
+        raise ValueError(f"k_cache {tuple(shape)} and v_cache {tuple(v.shape)} differ")
+    if shape[3] not in (64, 128):
+        raise ValueError(f"head dim must be 64 or 128, got {shape[3]}")
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError("the caches' last dimension must be contiguous")
+    return shape, ks, vs
 
 
-@torch.no_grad()
 def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                  k_cache: torch.Tensor, v_cache: torch.Tensor, cache_rows: torch.Tensor, *,
                  n_heads: int, q_weight: torch.Tensor | None = None,
@@ -178,13 +210,7 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
     them heads are not normed.  Returns the queries ``[T, n_heads, head dim]``.  A prompt that a
     batch shares is written with one session's caches (``prefix[None]``)."""
     code = _dtype(qkv, "qkv")
-    _cache(k_cache, "k_cache", qkv)
-    _cache(v_cache, "v_cache", qkv)
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ")
-    sessions, capacity, n_kv, dim = k_cache.shape
-    if dim not in (64, 128):
-        raise ValueError(f"head dim must be 64 or 128, got {dim}")
+    (sessions, capacity, n_kv, dim), ks, vs = _caches(k_cache, v_cache, qkv)
     if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * dim or n_heads < 1:
         raise ValueError(f"qkv must be [tokens, {(n_heads + 2 * n_kv) * dim}], got "
                          f"{tuple(qkv.shape)}")
@@ -195,8 +221,9 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
         if t.dtype != torch.float32 or t.device != qkv.device or t.dim() != 2 \
                 or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float32 table on {qkv.device}")
-    if cos.shape != sin.shape or cos.shape[0] < 1:
-        raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be equal tables")
+    table = cos.shape
+    if table != sin.shape or table[0] < 1:
+        raise ValueError(f"cos {tuple(table)} and sin {tuple(sin.shape)} must be equal tables")
     w_code = code
     if q_weight is not None and k_weight is not None:
         w_code = _side(q_weight, "q_weight", qkv, code)
@@ -207,30 +234,28 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
                 raise ValueError(f"{name} must be a contiguous vector of {dim}")
     elif q_weight is not k_weight:
         raise ValueError("q_weight and k_weight come together")
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if any(t.shape[i] > 1 and t.stride(i) == 0 for i in range(3)):
-            raise ValueError(f"{name} is expanded: its rows share memory")
+    if 0 in ks and any(n > 1 and st == 0 for n, st in zip(k_cache.shape, ks)) \
+            or 0 in vs and any(n > 1 and st == 0 for n, st in zip(v_cache.shape, vs)):
+        raise ValueError("k_cache or v_cache is expanded: its rows share memory")
     if out is None:
-        out = torch.empty(tokens, n_heads, dim, dtype=qkv.dtype, device=qkv.device)
+        out = torch.empty((tokens, n_heads, dim), dtype=qkv.dtype, device=qkv.device)
     elif out.dtype != qkv.dtype or out.device != qkv.device or out.shape != (tokens, n_heads, dim) \
             or out.stride(2) != 1 or (n_heads > 1 and out.stride(1) != dim):
         raise ValueError(f"out must be a {qkv.dtype} tensor {(tokens, n_heads, dim)} on "
                          f"{qkv.device} whose heads are contiguous")
     if tokens == 0:
         return out
-    ks, vs = k_cache.stride(), v_cache.stride()
-    args = _lib.FcvLmQkNormRope(
+    args = _QK_NORM_ROPE.pack(
         qkv.data_ptr(), pos_ptr, row_ptr, cos.data_ptr(), sin.data_ptr(),
-        None if q_weight is None else q_weight.data_ptr(),
-        None if k_weight is None else k_weight.data_ptr(), out.data_ptr(), k_cache.data_ptr(),
-        v_cache.data_ptr(), qkv_row, out.stride(0) if tokens > 1 else n_heads * dim, ks[0], ks[1],
-        ks[2], vs[0], vs[1], vs[2], tokens, n_heads, n_kv, dim, 2 * cos.shape[1], cos.shape[0],
-        sessions, capacity, code, w_code, bool(interleaved), eps)
-    _launch(_lib.load().fcv_lm_qk_norm_rope, qkv.device, args)
+        0 if q_weight is None else q_weight.data_ptr(),
+        0 if k_weight is None else k_weight.data_ptr(), out.data_ptr(), k_cache.data_ptr(),
+        v_cache.data_ptr(), qkv_row, out.stride(0) if tokens > 1 else n_heads * dim, *ks[:3],
+        *vs[:3], tokens, n_heads, n_kv, dim, 2 * table[1], table[0], sessions, capacity, code,
+        w_code, bool(interleaved), eps)
+    _launch(_entry("fcv_lm_qk_norm_rope", 1), qkv.device.index, args)
     return out
 
 
-@torch.no_grad()
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                      lengths: torch.Tensor, *, prefix_k: torch.Tensor | None = None,
                      prefix_v: torch.Tensor | None = None, cu_q: torch.Tensor | None = None,
@@ -250,13 +275,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ``scale`` defaults to ``head dim ** -0.5``.  A query that sees no key gives zeros.  Returns
     the output, or with ``return_lse`` also the log sums of exponentials, fp32 ``[T, heads]``."""
     code = _dtype(q, "q")
-    _cache(k_cache, "k_cache", q)
-    _cache(v_cache, "v_cache", q)
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ")
-    sessions, capacity, n_kv, dim = k_cache.shape
-    if dim not in (64, 128):
-        raise ValueError(f"head dim must be 64 or 128, got {dim}")
+    (sessions, capacity, n_kv, dim), ks, vs = _caches(k_cache, v_cache, q)
     if q.dim() != 3 or q.shape[2] != dim or q.shape[1] % n_kv or q.shape[1] < 1:
         raise ValueError(f"q must be [tokens, heads, {dim}] with heads a multiple of {n_kv}, got "
                          f"{tuple(q.shape)}")
@@ -267,7 +286,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if batch < 1:
         raise ValueError("lengths is empty")
     len_ptr = _indices(lengths, "lengths", batch, q)
-    cu_ptr = None if cu_q is None else _indices(cu_q, "cu_q", batch + 1, q)
+    cu_ptr = 0 if cu_q is None else _indices(cu_q, "cu_q", batch + 1, q)
     if cu_q is None:
         if tokens % batch:
             raise ValueError(f"without cu_q the {tokens} rows of q must divide by the {batch} "
@@ -275,10 +294,10 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         max_q = max(tokens // batch, 1)
     elif max_q is None:
         max_q = max(tokens, 1)
-    slot_ptr = None if slots is None else _indices(slots, "slots", batch, q)
+    slot_ptr = 0 if slots is None else _indices(slots, "slots", batch, q)
     if slots is None and batch > sessions:
         raise ValueError(f"{batch} sequences need slots: the caches hold {sessions} sessions")
-    prefix_len, pk_ptr, pv_ptr, pk, pv = 0, None, None, (0, 0), (0, 0)
+    prefix_len, pk_ptr, pv_ptr, pk, pv = 0, 0, 0, (0, 0), (0, 0)
     if (prefix_k is None) != (prefix_v is None):
         raise ValueError("prefix_k and prefix_v come together")
     if prefix_k is not None:
@@ -294,7 +313,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
             pk_ptr, pv_ptr = prefix_k.data_ptr(), prefix_v.data_ptr()
             pk, pv = prefix_k.stride(), prefix_v.stride()
     if out is None:
-        out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=q.device)
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
     elif out.dtype != q.dtype or out.device != q.device or out.shape != q.shape \
             or out.stride(2) != 1:
         raise ValueError(f"out must be a {q.dtype} tensor {tuple(q.shape)} on {q.device}, its last "
@@ -306,19 +325,19 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device)
     if tokens == 0:
         return (out, lse) if return_lse else out
-    ks, vs = k_cache.stride(), v_cache.stride()
-    args = _lib.FcvLmAttention(
+    qs, os = q.stride(), out.stride()
+    args = _ATTENTION.pack(
         q.data_ptr(), pk_ptr, pv_ptr, k_cache.data_ptr(), v_cache.data_ptr(), cu_ptr, len_ptr,
-        slot_ptr, out.data_ptr(), None if lse is None else lse.data_ptr(), q.stride(0),
-        q.stride(1), out.stride(0), out.stride(1), pk[0], pk[1], pv[0], pv[1], ks[0], ks[1], ks[2],
-        vs[0], vs[1], vs[2], tokens, batch, heads, n_kv, dim, prefix_len, sessions, capacity,
-        max_q, capacity if max_length is None else max_length, code,
+        slot_ptr, out.data_ptr(), 0 if lse is None else lse.data_ptr(), qs[0], qs[1], os[0], os[1],
+        pk[0], pk[1], pv[0], pv[1], *ks[:3], *vs[:3], tokens, batch, heads, n_kv, dim, prefix_len,
+        sessions, capacity, max_q, capacity if max_length is None else max_length, code,
         dim ** -0.5 if scale is None else scale)
-    lib = _lib.load()
-    need = lib.fcv_lm_prefix_attention_workspace_bytes(args)
+    need = _entry("fcv_lm_prefix_attention_workspace_bytes", 0)(args)
+    fn = _entry("fcv_lm_prefix_attention", 3)
+    device = q.device
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _launch(lib.fcv_lm_prefix_attention, q.device, args, ws.data_ptr(), need)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        _launch(fn, device.index, args, ws.data_ptr(), need)
     else:
-        _launch(lib.fcv_lm_prefix_attention, q.device, args, None, 0)
+        _launch(fn, device.index, args, None, 0)
     return (out, lse) if return_lse else out
