@@ -19,20 +19,35 @@ namespace {
 constexpr int kThreads = 256;
 
 template <class E>
-__device__ __forceinline__ float weight_at(const void* w, bool f32, int i) {
-  return f32 ? static_cast<const float*>(w)[i] : E::to_f32(static_cast<const short*>(w)[i]);
+__device__ __forceinline__ void load8(const void* w, bool f32, int i, float (&out)[8]) {
+  if (f32) {
+    const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(w) + i);
+    const f32x4 lo = p[0], hi = p[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      out[e] = lo[e];
+      out[e + 4] = hi[e];
+    }
+  } else {
+    const s16x8 v = *reinterpret_cast<const s16x8*>(static_cast<const short*>(w) + i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = E::to_f32(v[e]);
+  }
 }
 
+// heads_inv: 2^32 / heads, rounded up.
 template <class E, int D>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const FcvLmQkNormRope p,
-                                                                uint32_t total) {
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const FcvLmQkNormRope p, uint32_t total,
+                                                                uint32_t heads_inv) {
   constexpr int L = D / 16;  // lanes of a head
-  const int heads = p.n_heads + 2 * p.n_kv_heads;
+  const uint32_t heads = p.n_heads + 2 * p.n_kv_heads;
   const uint32_t unit = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) / L;
   const int j = threadIdx.x % L;
   if (unit >= total) return;  // whole heads: lanes that sum together leave together
-  const uint32_t token = unit / (uint32_t)heads;
-  const int head = (int)(unit - token * (uint32_t)heads);
+  // unit / heads: the product is at most one too large
+  uint32_t token = __umulhi(unit, heads_inv);
+  if (token * heads > unit) --token;
+  const int head = (int)(unit - token * heads);
 
   const bool is_q = head < p.n_heads, is_v = head >= p.n_heads + p.n_kv_heads;
   const int half_chunks = p.rope_dim / 16;  // chunks of half the rotated part
@@ -52,13 +67,32 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const FcvLmQkNor
     const int32_t row = p.cache_rows[token];
     store = row >= 0 && (int64_t)row < (int64_t)p.sessions * p.capacity;
     const uint32_t r = store ? (uint32_t)row : 0;
-    const uint32_t session = r / (uint32_t)p.capacity, at = r - session * (uint32_t)p.capacity;
+    const uint32_t session = p.sessions == 1 ? 0 : r / (uint32_t)p.capacity;
+    const uint32_t at = r - session * (uint32_t)p.capacity;
     const int h = head - p.n_heads - (is_v ? p.n_kv_heads : 0);
     dst = is_v ? static_cast<short*>(p.v_cache) + session * p.v_session + at * p.v_row + h * p.v_head
                : static_cast<short*>(p.k_cache) + session * p.k_session + at * p.k_row + h * p.k_head;
   }
 
   if (!is_v) {
+    // the table's entries of both chunks: four pairs each of 2 i, 2 i + 1, or the same eight of i, i + R / 2
+    float cs[8], sn[8];
+    if (turned) {
+      const int pos = min(max(p.positions[token], 0), p.max_pos - 1);
+      const int64_t row = (int64_t)pos * (p.rope_dim / 2);
+      const int i0 = p.interleaved ? c0 * 4 : c0 * 8, i1 = p.interleaved ? c1 * 4 : c0 * 8 + 4;
+      const f32x4 ca = *reinterpret_cast<const f32x4*>(p.rope_cos + row + i0);
+      const f32x4 cb = *reinterpret_cast<const f32x4*>(p.rope_cos + row + i1);
+      const f32x4 sa = *reinterpret_cast<const f32x4*>(p.rope_sin + row + i0);
+      const f32x4 sb = *reinterpret_cast<const f32x4*>(p.rope_sin + row + i1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        cs[e] = ca[e];
+        cs[e + 4] = cb[e];
+        sn[e] = sa[e];
+        sn[e + 4] = sb[e];
+      }
+    }
     float a[8], b[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -75,33 +109,31 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const FcvLmQkNor
       if constexpr (L == 8) ss += dpp_f<0x141>(ss);  // the other four of eight
       const float inv = 1.0f / sqrtf(fmaf(ss, 1.0f / D, p.eps));
       const bool wf = p.weight_dtype == FCV_LM_F32;
+      float wa[8], wb[8];
+      load8<E>(w, wf, c0 * 8, wa);
+      load8<E>(w, wf, c1 * 8, wb);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        a[e] *= inv * weight_at<E>(w, wf, c0 * 8 + e);
-        b[e] *= inv * weight_at<E>(w, wf, c1 * 8 + e);
+        a[e] *= inv * wa[e];
+        b[e] *= inv * wb[e];
       }
     }
     if (turned) {
-      const int pos = min(max(p.positions[token], 0), p.max_pos - 1);
-      const int half = p.rope_dim / 2;
-      const float* cs = p.rope_cos + (int64_t)pos * half;
-      const float* sn = p.rope_sin + (int64_t)pos * half;
       if (p.interleaved) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const int i0 = c0 * 4 + e / 2, i1 = c1 * 4 + e / 2;
           const float u0 = a[e], u1 = a[e + 1], v0 = b[e], v1 = b[e + 1];
-          a[e] = fmaf(u0, cs[i0], -(u1 * sn[i0]));
-          a[e + 1] = fmaf(u1, cs[i0], u0 * sn[i0]);
-          b[e] = fmaf(v0, cs[i1], -(v1 * sn[i1]));
-          b[e + 1] = fmaf(v1, cs[i1], v0 * sn[i1]);
+          a[e] = fmaf(u0, cs[e / 2], -(u1 * sn[e / 2]));
+          a[e + 1] = fmaf(u1, cs[e / 2], u0 * sn[e / 2]);
+          b[e] = fmaf(v0, cs[4 + e / 2], -(v1 * sn[4 + e / 2]));
+          b[e + 1] = fmaf(v1, cs[4 + e / 2], v0 * sn[4 + e / 2]);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float u = a[e], v = b[e], c = cs[c0 * 8 + e], s = sn[c0 * 8 + e];
-          a[e] = fmaf(u, c, -(v * s));
-          b[e] = fmaf(v, c, u * s);
+          const float u = a[e], v = b[e];
+          a[e] = fmaf(u, cs[e], -(v * sn[e]));
+          b[e] = fmaf(v, cs[e], u * sn[e]);
         }
       }
     }
@@ -143,8 +175,10 @@ int check(const FcvLmQkNormRope* p) {
                 p->k_cache && p->v_cache,
             FCV_ERR_INVALID, "null argument");
   FCV_CHECK(aligned(p->qkv, 16) && aligned(p->q_out, 16) && aligned(p->k_cache, 16) &&
-                aligned(p->v_cache, 16),
-            FCV_ERR_INVALID, "qkv, q_out and the caches must start on 16-byte boundaries");
+                aligned(p->v_cache, 16) && aligned(p->rope_cos, 16) && aligned(p->rope_sin, 16) &&
+                aligned(p->q_weight, 16) && aligned(p->k_weight, 16),
+            FCV_ERR_INVALID,
+            "qkv, q_out, the caches, the tables and the weights must start on 16-byte boundaries");
   FCV_CHECK((p->qkv_row | p->q_row | p->k_session | p->k_row | p->k_head | p->v_session | p->v_row |
              p->v_head) % 8 == 0,
             FCV_ERR_INVALID, "strides must be multiples of 8 elements");
@@ -158,12 +192,16 @@ int check(const FcvLmQkNormRope* p) {
 template <class E>
 void launch(const FcvLmQkNormRope& p, hipStream_t stream) {
   const uint32_t total = (uint32_t)p.tokens * (uint32_t)(p.n_heads + 2 * p.n_kv_heads);
+  const uint32_t heads = p.n_heads + 2 * p.n_kv_heads;
+  const uint32_t heads_inv = (uint32_t)(((1ULL << 32) + heads - 1) / heads);
   const uint32_t per_block = kThreads * 16 / p.head_dim;
   const dim3 grid((total + per_block - 1) / per_block);
   if (p.head_dim == 64)
-    hipLaunchKernelGGL((qk_norm_rope_kernel<E, 64>), grid, dim3(kThreads), 0, stream, p, total);
+    hipLaunchKernelGGL((qk_norm_rope_kernel<E, 64>), grid, dim3(kThreads), 0, stream, p, total,
+                       heads_inv);
   else
-    hipLaunchKernelGGL((qk_norm_rope_kernel<E, 128>), grid, dim3(kThreads), 0, stream, p, total);
+    hipLaunchKernelGGL((qk_norm_rope_kernel<E, 128>), grid, dim3(kThreads), 0, stream, p, total,
+                       heads_inv);
 }
 
 }  // namespace
