@@ -1,9 +1,21 @@
 // y = act(x W^T + bias) + residual on the matrix cores, for any row count, width and stride.
 //
-// The product runs on v_mfma_f32_32x32x16 with W as the A operand and x as the B operand, so that a
-// lane's accumulator holds four consecutive columns of one row of y per register group.
+// x and W are read as they lie (K contiguous in both).  W is the A operand and x the B operand, so that a
+// lane's accumulator holds four consecutive columns of one row of y per register group; sums are fp32, the
+// epilogue is fp32, and y is rounded once.
+//
+// Three kernels (plan_of chooses by an estimate):
+//   linear_tile_kernel  tiles of y from operand slices that are copied straight into LDS (a ring of two to
+//                       four slices of 64 of K), K cut over several workgroups where the tiles are few;
+//   linear_few_kernel   up to 16 rows, W read once into registers;
+//   linear_any_kernel   rows off 16-byte boundaries or K no multiple of 8: operands through registers.
+//
+// Bound and rate: large products by the matrix pipes, 8192 x 4096 x 8192 bf16 with bias and SiLU 450 us
+// (1.22 PFLOP/s; 61 % of the cycles at the clock the card holds under it, and the same within 10 % with
+// three to five slices of 32, with the copies asked for at once, and with four waves of 128 x 128); 9184 x
+// 1024 x 2048 with tanh-GELU 55 us, half of it rounds that are not full and stores that all CUs send at
+// once.  Small products by what a CU takes in (about 55 B/ns of copies): 32 x 4096 x 4096 12 us.
 #include <algorithm>
-#include <cstdlib>
 #include <type_traits>
 
 #include "lm.hpp"
@@ -76,6 +88,19 @@ __device__ __forceinline__ void store4(void* p, bool f32, int64_t i, const f32x4
         s16x4{E::from_f32(v[0]), E::from_f32(v[1]), E::from_f32(v[2]), E::from_f32(v[3])};
 }
 
+// Column n of row m from its sum.
+template <class E>
+__device__ __forceinline__ void finish1(const FcvLmLinear& p, int m, int n, float z) {
+  if (p.bias) z += element<E>(p.bias, p.bias_dtype == FCV_LM_F32, n);
+  with_act(p.activation, [&](auto k) { z = act<decltype(k)::value>(z); });
+  if (p.residual) z += element<E>(p.residual, p.residual_dtype == FCV_LM_F32, (int64_t)m * p.ldr + n);
+  const int64_t at = (int64_t)m * p.ldy + n;
+  if (p.y_dtype == FCV_LM_F32)
+    static_cast<float*>(p.y)[at] = z;
+  else
+    static_cast<short*>(p.y)[at] = E::from_f32(z);
+}
+
 // Four columns n .. n + 3 of row m from their sums: those below N one at a time, or all of them
 // where they are one aligned access (`vec`).
 template <class E>
@@ -87,23 +112,10 @@ __device__ __forceinline__ void finish4(const FcvLmLinear& p, bool vec, int m, i
     return;
   }
   const int count = min(4, p.n - n);
-  if (p.bias) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < count) v[e] += element<E>(p.bias, p.bias_dtype == FCV_LM_F32, n + e);
-  }
-  v = act4(v, p.activation);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (e >= count) break;
-    float z = v[e];
-    if (p.residual)
-      z += element<E>(p.residual, p.residual_dtype == FCV_LM_F32, (int64_t)m * p.ldr + n + e);
-    const int64_t at = (int64_t)m * p.ldy + n + e;
-    if (p.y_dtype == FCV_LM_F32)
-      static_cast<float*>(p.y)[at] = z;
-    else
-      static_cast<short*>(p.y)[at] = E::from_f32(z);
+#pragma unroll 1
+  for (int e = 0; e < count; ++e) {
+    finish1<E>(p, m, n + e, v[0]);
+    v = f32x4{v[1], v[2], v[3], 0.0f};
   }
 }
 
@@ -495,16 +507,15 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
     });
     return;
   }
-  const f32x4 bias = bias4<E>(p, vec, col);
+  // rows off their boundaries, or a tile past N: a column a lane, neighbouring lanes along a row
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     park(i);
-#pragma unroll 1
-    for (int q = 0; q < kPasses; ++q) {
-      const int row = m0 + wm0 + i * 32 + rr + q * kPassRows;
-      if (row < p.m && col < p.n)
-        finish4<E>(p, vec, row, col, *reinterpret_cast<const f32x4*>(mine + q * kPassRows * kPitch),
-                   bias, residual4<E>(p, vec, row, col));
+#pragma unroll 4
+    for (int q = 0; q < kCols / 2; ++q) {
+      const int r = (q * 64 + lane) / kCols, c = (q * 64 + lane) % kCols;
+      const int row = m0 + wm0 + i * 32 + r, n = n0 + wn0 + c;
+      if (row < p.m && n < p.n) finish1<E>(p, row, n, stg[r * kPitch + c]);
     }
     wave_fence();
   }
@@ -608,6 +619,7 @@ int check(const FcvLmLinear* p) {
   FCV_CHECK(p->activation >= FCV_LM_ACT_NONE && p->activation <= FCV_LM_ACT_GELU_TANH,
             FCV_ERR_INVALID, "unknown activation");
   FCV_CHECK(p->m >= 0 && p->n >= 1 && p->k >= 1, FCV_ERR_INVALID, "need m >= 0, n >= 1 and k >= 1");
+  FCV_CHECK(p->k <= (1 << 28), FCV_ERR_INVALID, "k is limited to 2^28");
   FCV_CHECK(p->m <= (1 << 22) && p->n <= (1 << 22) && (int64_t)p->m * p->n <= (1LL << 34),
             FCV_ERR_INVALID, "m and n are limited to 2^22 each and their product to 2^34");
   FCV_CHECK(p->ldx >= 0 && p->ldw >= 0 && p->ldr >= 0, FCV_ERR_INVALID, "negative row stride");
@@ -759,7 +771,6 @@ extern "C" int fcv_lm_linear(const FcvLmLinear* args, void* workspace, size_t wo
             "workspace too small: need " + std::to_string(need) + " bytes");
   FCV_CHECK(need == 0 || fcv::lm::aligned(workspace, 256), FCV_ERR_INVALID,
             "workspace must be 256-byte aligned");
-  if (getenv("FCV_LM_SAY")) fprintf(stderr, "form %d splits %d slices %d\n", (int)plan.form, plan.splits, plan.slices);
   if (args->dtype == FCV_LM_F16)
     fcv::lm::launch<fcv::lm::Half>(*args, plan, workspace, stream);
   else

@@ -43,7 +43,8 @@ struct Bf16 {
   typedef __bf16 T;
   static constexpr short kOne = 0x3F80;
   static constexpr short kInf = 0x7F80;
-  static constexpr float kShift = 0.0f, kLag = 8.0f;  // bf16 has fp32's range
+  // bf16 has fp32's range: sums of 2^16 of its largest values do not pass fp32's
+  static constexpr float kShift = -24.0f, kLag = 8.0f;
   static __device__ __forceinline__ float to_f32(short b) {
     return __uint_as_float((uint32_t)(uint16_t)b << 16);
   }

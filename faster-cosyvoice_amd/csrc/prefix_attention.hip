@@ -27,6 +27,7 @@ constexpr int kFewKeys = 32;    // keys of a wave's tile there
 constexpr int kManyRows = 128;  // queries of a row tile whose waves share its queries out, 32 each
 constexpr int kManyKeys = 64;   // keys of a workgroup's tile there
 constexpr int kStackedFew = 4096;  // rows of all key heads up to which stacked rows are taken 32 at a time
+constexpr int kShortKeys = 768;    // prefix and own keys up to which tiles of 32 queries take them all at once
 constexpr int kMaxParts = 64;   // lanes of the joining wave
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -109,6 +110,8 @@ struct State {
 // LDS addresses of a tile's fragments, for the tile whose keys (or values) start at byte `base`, a
 // multiple of 256.  In swz, a row's bits and a chunk's are joined by exclusive or, so that a lane's
 // addresses differ from its first by constants in the low byte and in the instruction's offset.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"  // of the host's pass
 typedef __attribute__((address_space(3))) const s16x8* lds16;
 typedef __attribute__((address_space(3))) s16x4* lds8;
 
@@ -141,6 +144,8 @@ struct ValueFragments {
   }
 };
 
+#pragma clang diagnostic pop
+
 // v with zeros in the place of infinities and NaN, whose presence is noted in `found`.
 template <class E>
 __device__ __forceinline__ s16x8 finite_only(const s16x8& v, uint32_t& found) {
@@ -168,17 +173,13 @@ __device__ __forceinline__ f32x4 not_finite4(const short* v, int64_t v_row, int 
   return sum;
 }
 
-// One tile of 32 KT keys from LDS.  `limit` (per lane) is the first key of the tile that the lane's
-// query does not see; all_visible says that no lane has one.  With hide, values that are not finite are
-// left out and noted in `found`.
-// keys_read() is called once the keys have been read, values_here() before the first value is.
-template <class E, int D, int KT, class F, class G>
-__device__ __forceinline__ void tile(uint32_t sk, uint32_t sv, const s16x8 (&qf)[D / 16],
-                                     State<D>& st, int lane, int limit, bool all_visible, bool hide,
-                                     uint32_t& found, float scale2, const F& keys_read, const G& values_here) {
-  const int hl = lane >> 5;
+// The steps of a tile of 32 KT keys.
+
+// s = K Q^T of the keys at LDS byte sk.
+template <class E, int D, int KT>
+__device__ __forceinline__ void tile_scores(uint32_t sk, const s16x8 (&qf)[D / 16], int lane,
+                                            f32x16 (&s)[KT]) {
   const KeyFragments<D> keys(sk, lane);
-  f32x16 s[KT];
 #pragma unroll
   for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -188,9 +189,15 @@ __device__ __forceinline__ void tile(uint32_t sk, uint32_t sv, const s16x8 (&qf)
   for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
     for (int t = 0; t < KT; ++t) s[t] = E::mfma32(keys.get(t, ks), qf[ks], s[t]);
-  keys_read();
+}
+
+// Hides the scores of keys from `limit` (the lane's, from the tile's first key on) and takes the running
+// maximum along.
+template <class E, int D, int KT>
+__device__ __forceinline__ void tile_maximum(f32x16 (&s)[KT], State<D>& st, int lane, int limit,
+                                             bool all_visible, float scale2) {
   if (!all_visible) {
-    int first = limit - hl * 4;
+    int first = limit - (lane >> 5) * 4;
     asm volatile("" : "+v"(first));  // a branch, not 32 selects in every tile
 #pragma unroll
     for (int t = 0; t < KT; ++t)
@@ -215,9 +222,14 @@ __device__ __forceinline__ void tile(uint32_t sk, uint32_t sv, const s16x8 (&qf)
 #pragma unroll
       for (int e = 0; e < 16; ++e) st.acc[dt][e] *= corr;
   }
+}
+
+// The weights of the scores, and their sum.
+template <class E, int D, int KT>
+__device__ __forceinline__ void tile_weights(const f32x16 (&s)[KT], State<D>& st, float scale2,
+                                             s16x8 (&pf)[2 * KT]) {
   const float shift = E::kShift - (st.m == -INFINITY ? 0.0f : st.m);
   float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  s16x8 pf[2 * KT];
 #pragma unroll
   for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -229,7 +241,13 @@ __device__ __forceinline__ void tile(uint32_t sk, uint32_t sv, const s16x8 (&qf)
       pf[t * 2 + (e >> 3)][e & 7] = E::from_f32(w);
     }
   st.l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  values_here();
+}
+
+// O^T += V^T P^T of the values at LDS byte sv.  With hide, values that are not finite are left out and
+// noted in `found`.
+template <class E, int D, int KT>
+__device__ __forceinline__ void tile_values(uint32_t sv, const s16x8 (&pf)[2 * KT], State<D>& st, int lane,
+                                            bool hide, uint32_t& found) {
   const ValueFragments<D> values(sv, lane);
   if (hide) {
 #pragma unroll
@@ -242,8 +260,7 @@ __device__ __forceinline__ void tile(uint32_t sk, uint32_t sv, const s16x8 (&qf)
 #pragma unroll
   for (int k = 0; k < 2 * KT; ++k)
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-      st.acc[dt] = E::mfma32(values.get(k, dt), pf[k], st.acc[dt]);
+    for (int dt = 0; dt < D / 32; ++dt) st.acc[dt] = E::mfma32(values.get(k, dt), pf[k], st.acc[dt]);
 }
 
 // The queries of a row tile: rows first .. first + count - 1 of the (token, head of the group) pairs of
@@ -296,69 +313,75 @@ constexpr int pitch() { return D + 4; }
 template <int D>
 constexpr int lds_elems() { return kWaves * 32 * (pitch<D>() * 2 + 4); }
 
-// A row tile of up to 32 queries against keys [k0, k1) of a segment; the four waves take the range's
-// tiles in turn, each through LDS buffers of its own (no barrier), and are joined at the end.
-// first_pos: the position of the sequence's first new token; own is false for the prefix.
+// A row tile of up to 32 queries against keys [k0, k1) of the prefix and [o0, o1) of the sequence's own; the
+// four waves take a range's tiles in turn, each through LDS buffers of its own (no barrier), and are joined
+// at the end.  first_pos: the position of the sequence's first new token.
 template <class E, int D>
-__device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Segment& seg, int k0, int k1,
-                         bool own, int first_pos, int part) {
-  if (k0 >= k1) {  // nothing to sum: no weight, and no output that the join would read
+__device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Segment& prefix, int k0,
+                         int k1, const Segment& own, int o0, int o1, int first_pos, int part) {
+  const FcvLmAttention& p = a.p;
+  if (k0 >= k1 && o0 >= o1 && !a.s.direct) {  // nothing to sum: no weight, no output that the join would read
     if (threadIdx.x < (unsigned)rows.count) {
-      const int64_t at = (int64_t)part * a.p.tokens * a.p.n_heads +
-                         (int64_t)rows.token(threadIdx.x) * a.p.n_heads + rows.head(threadIdx.x);
+      const int64_t at = (int64_t)part * p.tokens * p.n_heads +
+                         (int64_t)rows.token(threadIdx.x) * p.n_heads + rows.head(threadIdx.x);
       a.part_s[at] = float2{-INFINITY, 0.0f};
     }
     return;
   }
   constexpr int kCopies = kFewKeys / (512 / D);
   constexpr int kTileElems = kFewKeys * D;
-  const FcvLmAttention& p = a.p;
   const int lane = threadIdx.x & 63, ql = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   s16x8 qf[D / 16];
   load_q<D>(p, rows, ql, hl, qf);
-  // first key past the query's view; the wave's smallest decides which tiles need the mask
-  const int limit = own ? min(k1, first_pos + rows.token(min(ql, rows.count - 1)) - rows.token0 + 1) : k1;
+  // first own key past the query's view; the wave's smallest decides which tiles need the mask
+  const int limit = min(o1, first_pos + rows.token(min(ql, rows.count - 1)) - rows.token0 + 1);
   int low = limit;
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) low = min(low, __shfl_xor(low, off, kWave));
+  low = scalar(low);
 
   // a wave's two buffers hold a tile's keys and its values; each is filled again as soon as it was read
   const uint32_t sk = lds_base(smem) + wave * 2 * kTileElems * 2, sv = sk + kTileElems * 2;
-  const uint32_t k_bytes = (uint32_t)seg.k_row * 2, v_bytes = (uint32_t)seg.v_row * 2;
-  auto fetch_k = [&](int kt) {
-    copy_rows<D, kCopies>(seg.k + (int64_t)kt * seg.k_row, k_bytes, kFewKeys, k1 - kt, 0, lane, sk);
-  };
-  auto fetch_v = [&](int kt) {
-    copy_rows<D, kCopies>(seg.v + (int64_t)kt * seg.v_row, v_bytes, kFewKeys, k1 - kt, 0, lane, sv);
-  };
-
   State<D> st;
   st.reset();
   uint32_t found = 0;
-  int kt = k0 + wave * kFewKeys;
-  if (kt < k1) {
-    fetch_k(kt);
-    fetch_v(kt);
-  }
-  for (; kt < k1; kt += kWaves * kFewKeys) {
-    const int next = kt + kWaves * kFewKeys;
-    wait_vmem<kCopies>();  // the keys are here, the values may be on their way
-    tile<E, D, 1>(
-        sk, sv, qf, st, lane, limit - kt, kt + kFewKeys <= low, own && kt + kFewKeys > low, found, a.scale2,
-        [&] {
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads have returned
-          if (next < k1) fetch_k(next);
-        },
-        [&] {
-          if (next < k1)
-            wait_vmem<kCopies>();
-          else
-            wait_vmem<0>();
-        });
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (next < k1) fetch_v(next);
+#pragma unroll 1
+  for (int g = 0; g < 2; ++g) {
+    const Segment seg = g == 0 ? prefix : own;
+    const int begin = g == 0 ? k0 : o0, end = g == 0 ? k1 : o1;
+    const uint32_t k_bytes = (uint32_t)seg.k_row * 2, v_bytes = (uint32_t)seg.v_row * 2;
+    auto fetch_k = [&](int kt) {
+      copy_rows<D, kCopies>(seg.k + (int64_t)kt * seg.k_row, k_bytes, kFewKeys, end - kt, 0, lane, sk);
+    };
+    auto fetch_v = [&](int kt) {
+      copy_rows<D, kCopies>(seg.v + (int64_t)kt * seg.v_row, v_bytes, kFewKeys, end - kt, 0, lane, sv);
+    };
+    int kt = begin + wave * kFewKeys;
+    if (kt < end) {
+      fetch_k(kt);
+      fetch_v(kt);
+    }
+    for (; kt < end; kt += kWaves * kFewKeys) {
+      const int next = kt + kWaves * kFewKeys;
+      const bool all_visible = kt + kFewKeys <= (g == 0 ? end : low);
+      wait_vmem<kCopies>();  // the keys are here, the values may be on their way
+      f32x16 scores[1];
+      tile_scores<E, D, 1>(sk, qf, lane, scores);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads have returned
+      if (next < end) fetch_k(next);
+      tile_maximum<E, D, 1>(scores, st, lane, (g == 0 ? end : limit) - kt, all_visible, a.scale2);
+      s16x8 pf[2];
+      tile_weights<E, D, 1>(scores, st, a.scale2, pf);
+      if (next < end)
+        wait_vmem<kCopies>();
+      else
+        wait_vmem<0>();
+      tile_values<E, D, 1>(sv, pf, st, lane, g == 1 && !all_visible, found);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (next < end) fetch_v(next);
+    }
   }
 
   // join the waves: O is [wave][query][dim], four dims of a query a thread
@@ -393,9 +416,20 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
       o += *reinterpret_cast<const f32x4*>(so + (w * kFewRows + r) * pitch<D>() + d) * f;
     }
     if (any_found) {
-      const int from = max(k0, k0 + (low - k0) / kFewKeys * kFewKeys);  // the first tile with a mask
-      const int to = min(k1, first_pos + rows.token(r) - rows.token0 + 1);
-      o += not_finite4<E>(seg.v, seg.v_row, from, to, d);
+      const int from = max(o0, o0 + (low - o0) / kFewKeys * kFewKeys);  // the first tile with a mask
+      const int to = min(o1, first_pos + rows.token(r) - rows.token0 + 1);
+      o += not_finite4<E>(own.v, own.v_row, from, to, d);
+    }
+    if (a.s.direct) {
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      *reinterpret_cast<s16x4*>(static_cast<short*>(p.out) + rows.token(r) * p.out_row +
+                                rows.head(r) * p.out_head + d) =
+          s16x4{E::from_f32(o[0] * inv), E::from_f32(o[1] * inv), E::from_f32(o[2] * inv),
+                E::from_f32(o[3] * inv)};
+      if (p.lse && d == 0)
+        p.lse[(int64_t)rows.token(r) * p.n_heads + rows.head(r)] =
+            (m - E::kShift + log2f(l)) * 0.6931471805599453f;
+      continue;
     }
     const int64_t at = part * rows_all + (int64_t)rows.token(r) * p.n_heads + rows.head(r);
     *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = o;
@@ -454,9 +488,13 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
       if (kt + kManyKeys < end) fetch(kt + kManyKeys, stage ^ 1);
       if (g == 1 && kt >= high) continue;  // none of the wave's queries sees the tile
       const uint32_t sk = lds + stage * 2 * kTileElems * 2;
-      tile<E, D, kManyKeys / 32>(sk, sk + kTileElems * 2, qf, st, lane, (g == 0 ? end : limit) - kt,
-                                 kt + kManyKeys <= (g == 0 ? end : low), g == 1 && kt + kManyKeys > low,
-                                 found, a.scale2, [] {}, [] {});
+      const bool all_visible = kt + kManyKeys <= (g == 0 ? end : low);
+      f32x16 scores[2];
+      tile_scores<E, D, 2>(sk, qf, lane, scores);
+      tile_maximum<E, D, 2>(scores, st, lane, (g == 0 ? end : limit) - kt, all_visible, a.scale2);
+      s16x8 pf[4];
+      tile_weights<E, D, 2>(scores, st, a.scale2, pf);
+      tile_values<E, D, 2>(sk + kTileElems * 2, pf, st, lane, g == 1 && !all_visible, found);
     }
   }
 
@@ -564,15 +602,14 @@ __global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const Args a) 
     const int index = tiles - 1 - i;  // the last tiles see the most keys and go first
     const int first = index * tile_rows;
     const Rows rows = {kvh, group, token0, first, min(tile_rows, n_rows - first)};
-    if constexpr (MANY) {
-      // own keys past the tile's last query are not visited
-      const int seen = stacked ? 0 : min(length, first_pos + (first + rows.count - 1) / group + 1);
-      many_rows<E, D>(a, smem, rows, prefix, min(c0, prefix_len), min(c1, prefix_len), own,
-                      max(c0 - prefix_len, 0), min(max(c1 - prefix_len, 0), seen), first_pos, part);
-    } else {
-      const Segment seg = stacked ? prefix : own;
-      few_rows<E, D>(a, smem, rows, seg, c0, c1, !stacked, first_pos, part);
-    }
+    // own keys past the tile's last query are not visited
+    const int seen = stacked ? 0 : min(length, first_pos + (first + rows.count - 1) / group + 1);
+    const int p0 = min(c0, prefix_len), p1 = min(c1, prefix_len);
+    const int o0 = max(c0 - prefix_len, 0), o1 = min(max(c1 - prefix_len, 0), seen);
+    if constexpr (MANY)
+      many_rows<E, D>(a, smem, rows, prefix, p0, p1, own, o0, o1, first_pos, part);
+    else
+      few_rows<E, D>(a, smem, rows, prefix, p0, p1, own, o0, o1, first_pos, part);
   }
 }
 
@@ -675,7 +712,10 @@ Shape shape_of(const FcvLmAttention& p) {
   s.own_many = seq_rows > kFewRows;
   // A sequence with at least a tile of rows of its own reads the prefix with them: nothing is gained by
   // stacking its rows with others'.
-  s.fused = p.prefix_len == 0 || seq_rows >= kManyRows || (p.batch == 1 && s.own_many);
+  // Nor where all keys are few: one launch and no join (a token behind 512 + 100 keys 17 -> 13 us with
+  // the host's share; on the GPU alone even at about that many keys).
+  const bool short_keys = !s.own_many && p.prefix_len + (int64_t)max_length <= kShortKeys;
+  s.fused = p.prefix_len == 0 || seq_rows >= kManyRows || (p.batch == 1 && s.own_many) || short_keys;
   if (!s.fused) {
     s.prefix_many = s.own_many || (int64_t)p.tokens * p.n_heads > kStackedFew;
     s.prefix_tiles = ceil_div(all_rows, s.prefix_many ? kManyRows : kFewRows);
@@ -690,9 +730,10 @@ Shape shape_of(const FcvLmAttention& p) {
   // sequences differ in length: their ranges are dealt out in several rounds where they are short
   s.own_step = s.own_many ? cut(keys, kManyKeys, 0.6f, blocks, 2 * kCus, 32)
                           : cut(keys, kWaves * kFewKeys, 1.2f, blocks, 8 * kCus, 32);
+  if (short_keys) s.own_step = keys;
   s.no = ceil_div(keys, s.own_step);
   s.own_blocks = blocks * s.no;
-  s.direct = s.own_many && s.parts() == 1;
+  s.direct = s.parts() == 1;
   return s;
 }
 
@@ -735,6 +776,8 @@ int check(const FcvLmAttention* p) {
   FCV_CHECK(aligned(p->q, 16) && aligned(p->out, 16) && aligned(p->k_cache, 16) &&
                 aligned(p->v_cache, 16) && aligned(p->prefix_k, 16) && aligned(p->prefix_v, 16),
             FCV_ERR_INVALID, "q, out, the prefix and the caches must start on 16-byte boundaries");
+  FCV_CHECK((p->n_heads == 1 || p->out_head >= p->head_dim) && (p->tokens == 1 || p->out_row >= p->head_dim),
+            FCV_ERR_INVALID, "rows of out overlap");
   const Shape s = shape_of(*p);
   FCV_CHECK(s.prefix_blocks + s.own_blocks <= (1 << 23), FCV_ERR_INVALID,
             "the batch is too large for one call: split it");

@@ -156,6 +156,17 @@ def test_large_scores_and_scale(fcv):
         check(fcv, a, "scale", scale=0.9, max_q=9)
 
 
+def test_values_near_the_types_largest(fcv):
+    """Sums of values near the type's largest stay finite: only their mean has to fit the type."""
+    for dtype in (torch.bfloat16, torch.float16):
+        a = make([1, 60, 2], [300, 77, 2], 400, 4, 2, 64, dtype)
+        for n in ("v_cache", "prefix_v"):
+            a[n][:] = a[n].sign() * torch.finfo(dtype).max / 2
+        a["v_cache"].nan_to_num_(0)
+        a["prefix_v"][:, :, :32] = a["prefix_v"][:, :, :32].abs()
+        check(fcv, a, "large", max_q=60)
+
+
 def test_small_weights_carry_a_long_row(fcv):
     """One key far above thousands of equal ones, whose weights (2^-14 and less of the largest) sum to
     as much as it."""

@@ -52,6 +52,20 @@ def test_sizes(fcv, m, k, n, dtype):
           "bias, silu, residual")
 
 
+# one size for each tile shape and ring that the estimate picks, K ending inside a slice, rows and
+# columns inside a tile, with and without four aligned columns a store
+TILES = [(77, 904, 601), (600, 1000, 4096), (2000, 4104, 2000), (19000, 200, 381), (2048, 1032, 4096),
+         (4600, 1000, 2000), (4096, 1000, 4090), (4090, 1000, 4100), (8, 4104, 130), (300, 4104, 70)]
+
+
+@pytest.mark.parametrize("m,k,n", TILES)
+def test_every_tile_shape(fcv, m, k, n):
+    say(f"[linear] tiles {m} x {k} x {n}")
+    dtype = torch.bfloat16
+    x, w, b, r = make(m, k, n, dtype, bias=torch.float32, residual=dtype)
+    check(fcv.fused_linear(x, w, b, activation="gelu", residual=r), x, w, b, "gelu", r, dtype, "tiles")
+
+
 @pytest.mark.parametrize("act", [None, "none", "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("m,k,n", [(1, 512, 64), (40, 256, 72), (300, 128, 260)])
 def test_activations_and_fp32_sides(fcv, m, k, n, act):

@@ -47,7 +47,7 @@ def _linear(fcv, **kw):
     (dict(k=0), "k >= 1"), (dict(ldx=-64), "negative"), (dict(ldw=-64), "negative"),
     (dict(ldy=31), "shorter"), (dict(ldr=-8), "negative"), (dict(x=None), "null"),
     (dict(w=BIG + 1), "boundary"), (dict(y=BIG + 2, y_dtype=2), "boundary"),
-    (dict(m=1 << 23), "limited"), (dict(m=1 << 20, n=1 << 20, ldy=1 << 20), "limited"),
+    (dict(m=1 << 23), "limited"), (dict(k=1 << 29), "2\\^28"), (dict(m=1 << 20, n=1 << 20, ldy=1 << 20), "limited"),
 ])
 def test_linear_refuses(fcv, bad, match):
     _refuse(fcv, _linear(fcv, **bad), match)
@@ -100,7 +100,7 @@ def _attention(fcv, ws=BIG, ws_bytes=1 << 40, **kw):
     (dict(max_length=-1), "max_length"), (dict(scale=0.0), "scale"),
     (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(q_head=60), "multiples of 8"), (dict(pv_row=-8), "multiples of 8"),
-    (dict(k_row=1 << 24), "2\\^24"), (dict(lengths=None), "null"), (dict(prefix_v=None), "prefix"),
+    (dict(k_row=1 << 24), "2\\^24"), (dict(out_head=0), "overlap"), (dict(out_row=0), "overlap"), (dict(lengths=None), "null"), (dict(prefix_v=None), "prefix"),
     (dict(out=BIG + 8), "16-byte"), (dict(prefix_k=BIG + 4), "16-byte"),
     (dict(tokens=1 << 26), "2\\^26"), (dict(ws=None), "null workspace"),
     (dict(ws_bytes=16), "too small"), (dict(ws=BIG + 16), "256-byte"),
