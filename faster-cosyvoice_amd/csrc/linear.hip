@@ -508,17 +508,40 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
     return;
   }
   // rows off their boundaries, or a tile past N: a column a lane, neighbouring lanes along a row
+  static_assert(64 % kCols == 0, "a lane keeps its column");
+  const int n = n0 + wn0 + lane % kCols;
+  const float bias1 = p.bias && n < p.n ? element<E>(p.bias, p.bias_dtype == FCV_LM_F32, n) : 0.0f;
+  with_act(p.activation, [&](auto kind) {
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    park(i);
-#pragma unroll 4
-    for (int q = 0; q < kCols / 2; ++q) {
-      const int r = (q * 64 + lane) / kCols, c = (q * 64 + lane) % kCols;
-      const int row = m0 + wm0 + i * 32 + r, n = n0 + wn0 + c;
-      if (row < p.m && n < p.n) finish1<E>(p, row, n, stg[r * kPitch + c]);
+    for (int i = 0; i < TM; ++i) {
+      park(i);
+      const int row0 = m0 + wm0 + i * 32 + lane / kCols;
+#pragma unroll 1
+      for (int q0 = 0; q0 < kCols / 2; q0 += 8) {  // 8 of the block's passes of 64 / kCols rows
+        float r[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int row = row0 + (q0 + q) * (64 / kCols);
+          r[q] = p.residual && row < p.m && n < p.n
+                     ? element<E>(p.residual, p.residual_dtype == FCV_LM_F32, (int64_t)row * p.ldr + n)
+                     : 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int row = row0 + (q0 + q) * (64 / kCols);
+          const float v = stg[(row - m0 - wm0 - i * 32) * kPitch + lane % kCols];
+          const float z = act<decltype(kind)::value>(v + bias1) + r[q];
+          if (row >= p.m || n >= p.n) continue;
+          const int64_t at = (int64_t)row * p.ldy + n;
+          if (p.y_dtype == FCV_LM_F32)
+            static_cast<float*>(p.y)[at] = z;
+          else
+            static_cast<short*>(p.y)[at] = E::from_f32(z);
+        }
+      }
+      wave_fence();
     }
-    wave_fence();
-  }
+  });
 }
 
 // Sums of the ranges in their order, then the epilogue; a thread has four columns of a row.
