@@ -452,7 +452,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
   float* stg = reinterpret_cast<float*>(smem) + wave * 32 * kPitch;
   const int rr = lane / kLanes, rc = (lane % kLanes) * 4;
   const int col = n0 + wn0 + rc;
-  const bool vec = a.vec && col + 3 < p.n;
+  const bool inside = col < p.n;
   auto park = [&](int i) {
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -480,9 +480,9 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
     }
     return;
   }
-  if (__all(vec)) {
+  if (__all(a.vec && (!inside || col + 3 < p.n))) {
     with_act(p.activation, [&](auto kind) {
-      const f32x4 bias = bias4<E>(p, true, col);
+      const f32x4 bias = bias4<E>(p, inside, col);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const int row0 = m0 + wm0 + i * 32 + rr;
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
         // a block's residuals are asked for together, before its stores
 #pragma unroll
         for (int q = 0; q < kPasses; ++q)
-          r[q] = residual4<E>(p, true, min(row0 + q * kPassRows, p.m - 1), col);
+          r[q] = residual4<E>(p, inside, min(row0 + q * kPassRows, p.m - 1), col);
         park(i);
         f32x4 v[kPasses];
 #pragma unroll
@@ -501,13 +501,13 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
         for (int q = 0; q < kPasses; ++q) {
           const f32x4 z = act4<decltype(kind)::value>(v[q] + bias) + r[q];
           const int row = row0 + q * kPassRows;
-          if (row < p.m) store4<E>(p.y, p.y_dtype == FCV_LM_F32, (int64_t)row * p.ldy + col, z);
+          if (row < p.m && inside) store4<E>(p.y, p.y_dtype == FCV_LM_F32, (int64_t)row * p.ldy + col, z);
         }
       }
     });
     return;
   }
-  // rows off their boundaries, or a tile past N: a column a lane, neighbouring lanes along a row
+  // rows off their boundaries, or N no multiple of four: a column a lane, neighbouring lanes along a row
   static_assert(64 % kCols == 0, "a lane keeps its column");
   const int n = n0 + wn0 + lane % kCols;
   const float bias1 = p.bias && n < p.n ? element<E>(p.bias, p.bias_dtype == FCV_LM_F32, n) : 0.0f;
