@@ -8,7 +8,7 @@
 //   linear_tile_kernel  tiles of y from operand slices that are copied straight into LDS (a ring of two to
 //                       four slices of 64 of K), K cut over several workgroups where the tiles are few;
 //   linear_few_kernel   up to 16 rows, W read once into registers;
-//   linear_any_kernel   rows off 16-byte boundaries or K no multiple of 8: operands through registers.
+//   linear_any_kernel   more rows off 16-byte boundaries, or K no multiple of 8: through registers.
 //
 // Bound and rate: large products by the matrix pipes, 8192 x 4096 x 8192 bf16 with bias and SiLU 450 us
 // (1.22 PFLOP/s; 61 % of the cycles at the clock the card holds under it, and the same within 10 % with
@@ -26,7 +26,6 @@ namespace {
 
 struct Args {
   FcvLmLinear p;
-  bool x_chunks, w_chunks;  // rows start on 16-byte boundaries
   bool vec;                 // four columns of y, the residual and the bias are one aligned access
   int splits, slices;       // ranges of K, and the 64-wide slices of one
   float* part;              // [splits][m][part_ld] sums of the ranges
@@ -132,10 +131,16 @@ __device__ __forceinline__ f32x4 residual4(const FcvLmLinear& p, bool vec, int m
 
 // ---- any alignment: operands through registers --------------------------------------------------
 
+// 8 elements from any element's boundary (the same load instruction as an aligned one).
+__device__ __forceinline__ s16x8 load8_any(const short* p) {
+  typedef s16x8 any __attribute__((aligned(2)));
+  return *reinterpret_cast<const any*>(p);
+}
+
 // Elements k .. k + 7 of a row of `len`, zeros past its end.
-__device__ __forceinline__ s16x8 row_chunk(const short* row, int k, int len, bool chunks) {
+__device__ __forceinline__ s16x8 row_chunk(const short* row, int k, int len) {
+  if (k + 8 <= len) return load8_any(row + k);
   s16x8 v = {};
-  if (chunks && k + 8 <= len) return *reinterpret_cast<const s16x8*>(row + k);
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     if (k + e < len) v[e] = row[k + e];
@@ -144,6 +149,9 @@ __device__ __forceinline__ s16x8 row_chunk(const short* row, int k, int len, boo
 
 constexpr int kTile = 64, kDepth = 64, kPitch = kDepth + 8;
 
+// Tiles of 64 x 64, the next slice's elements in registers while this one's products run.  Bound by the
+// loads, whose chunks cross lines, and by the one step of lookahead: 4000 x 3001 x 4000 336 us (0.29
+// PFLOP/s), 1 x 1001 x 2000 (linear_few_kernel) 6 us.
 template <class E>
 __global__ __launch_bounds__(256) void linear_any_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) short sx[kTile][kPitch];
@@ -155,17 +163,23 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const Args a) {
   const int fr = lane & 31, fh = lane >> 5;
   const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
   const int lr = threadIdx.x >> 3, lc = (threadIdx.x & 7) * 8;
+  const int first = blockIdx.y * a.slices * kDepth, end = min(first + a.slices * kDepth, p.k);
+  const short *x[2], *w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    x[i] = static_cast<const short*>(p.x) + (int64_t)min(m0 + lr + 32 * i, p.m - 1) * p.ldx;
+    w[i] = static_cast<const short*>(p.w) + (int64_t)min(n0 + lr + 32 * i, p.n - 1) * p.ldw;
+  }
   f32x16 acc;
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
-  for (int k0 = 0; k0 < p.k; k0 += kDepth) {
-    s16x8 rx[2], rw[2];
+  s16x8 rx[2], rw[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int m = min(m0 + lr + 32 * i, p.m - 1), n = min(n0 + lr + 32 * i, p.n - 1);
-      rx[i] = row_chunk(static_cast<const short*>(p.x) + (int64_t)m * p.ldx, k0 + lc, p.k, a.x_chunks);
-      rw[i] = row_chunk(static_cast<const short*>(p.w) + (int64_t)n * p.ldw, k0 + lc, p.k, a.w_chunks);
-    }
+  for (int i = 0; i < 2; ++i) {
+    rx[i] = row_chunk(x[i], first + lc, end);
+    rw[i] = row_chunk(w[i], first + lc, end);
+  }
+  for (int k0 = first; k0 < end; k0 += kDepth) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -173,6 +187,13 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const Args a) {
       *reinterpret_cast<s16x8*>(&sw[lr + 32 * i][lc]) = rw[i];
     }
     __syncthreads();
+    if (k0 + kDepth < end) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        rx[i] = row_chunk(x[i], k0 + kDepth + lc, end);
+        rw[i] = row_chunk(w[i], k0 + kDepth + lc, end);
+      }
+    }
 #pragma unroll
     for (int ks = 0; ks < kDepth / 16; ++ks) {
       const s16x8 fx = *reinterpret_cast<const s16x8*>(&sx[wm + fr][ks * 16 + fh * 8]);
@@ -186,9 +207,13 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const Args a) {
   for (int g = 0; g < 4; ++g) {
     const int n = n0 + wn + g * 8 + fh * 4;
     if (n >= p.n) break;
+    const f32x4 v = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+    if (a.splits > 1) {
+      *reinterpret_cast<f32x4*>(a.part + ((int64_t)blockIdx.y * p.m + m) * a.part_ld + n) = v;
+      continue;
+    }
     const bool vec = a.vec && n + 3 < p.n;
-    finish4<E>(p, vec, m, n, f32x4{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]},
-               bias4<E>(p, vec, n), residual4<E>(p, vec, m, n));
+    finish4<E>(p, vec, m, n, v, bias4<E>(p, vec, n), residual4<E>(p, vec, m, n));
   }
 }
 
@@ -596,16 +621,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(const Args a
     if (k + kFewSteps * 32 <= k1) {
 #pragma unroll
       for (int u = 0; u < kFewSteps; ++u) {
-        fw[u] = *reinterpret_cast<const s16x8*>(w + k + u * 32);
-        fx[u] = *reinterpret_cast<const s16x8*>(x + k + u * 32);
+        fw[u] = load8_any(w + k + u * 32);
+        fx[u] = load8_any(x + k + u * 32);
       }
     } else {
-      // chunks at or past the end (a multiple of 8) are zeros
 #pragma unroll
       for (int u = 0; u < kFewSteps; ++u) {
-        const bool in = k + u * 32 + fk < k1;
-        fw[u] = in ? *reinterpret_cast<const s16x8*>(w + k + u * 32) : s16x8{};
-        fx[u] = in ? *reinterpret_cast<const s16x8*>(x + k + u * 32) : s16x8{};
+        fw[u] = row_chunk(w, k + u * 32, k1 - fk);  // w and x begin at the lane's element fk
+        fx[u] = row_chunk(x, k + u * 32, k1 - fk);
       }
     }
 #pragma unroll
@@ -670,6 +693,7 @@ struct Shape {
   float alone_us, slice_us, tile_us;
 };
 constexpr Shape kShapes[] = {
+    {kAny, 64, 64, 4, 0.85f, 1.75f, 2.0f},
     {kTile64, 64, 64, 2, 0.29f, 0.45f, 1.3f},       {kTile64x128, 64, 128, 2, 0.44f, 0.67f, 2.5f},
     {kTile128, 128, 128, 2, 0.62f, 1.10f, 5.0f},    {kTile128x256, 128, 256, 1, 0.96f, 0.96f, 5.6f},
     {kTile192x256, 192, 256, 1, 1.40f, 1.40f, 7.5f}, {kTile256, 256, 256, 1, 1.65f, 1.65f, 9.4f}};
@@ -695,7 +719,6 @@ Plan plan_of(const FcvLmLinear& p) {
                       p.ldw < (1 << 22);  // a tile's rows lie within 32-bit byte offsets
   const int slices = (p.k + kSlice - 1) / kSlice;
   Plan best{kAny, 1, slices};
-  if (!chunks) return best;
   float best_us = 3.0e38f;
   auto consider = [&](Form form, int splits, float us) {
     us += join_us(p, splits);
@@ -713,6 +736,7 @@ Plan plan_of(const FcvLmLinear& p) {
       consider(kFew, splits, 3.4f + (float)((blocks + kCus - 1) / kCus) * bytes / 40.0e3f);
     }
     for (const Shape& s : kShapes) {
+      if (chunks == (s.form == kAny)) continue;
       const int64_t blocks = tiles_of(p, s.bm, s.bn) * splits;
       const bool alone = blocks <= kCus;
       const int64_t round = alone ? kCus : (int64_t)kCus * s.per_cu;
@@ -740,15 +764,14 @@ void launch(const FcvLmLinear& p, const Plan& plan, void* workspace, hipStream_t
   auto quad = [](const void* t, int dtype, int64_t ld) {
     return t == nullptr || (aligned(t, dtype == FCV_LM_F32 ? 16 : 8) && ld % 4 == 0);
   };
-  const Args a{p, aligned(p.x, 16) && (p.ldx % 8 == 0 || p.m == 1),
-               aligned(p.w, 16) && (p.ldw % 8 == 0 || p.n == 1),
-               quad(p.y, p.y_dtype, p.ldy) && quad(p.residual, p.residual_dtype, p.ldr) &&
-                   quad(p.bias, p.bias_dtype, 0),
+  const Args a{p, quad(p.y, p.y_dtype, p.ldy) && quad(p.residual, p.residual_dtype, p.ldr) &&
+                      quad(p.bias, p.bias_dtype, 0),
                plan.splits, plan.slices, static_cast<float*>(workspace), part_ld(p)};
   switch (plan.form) {
     case kAny:
-      hipLaunchKernelGGL((linear_any_kernel<E>), dim3((unsigned)tiles_of(p, kTile, kTile)), dim3(256),
-                         0, stream, a);
+      hipLaunchKernelGGL((linear_any_kernel<E>),
+                         dim3((unsigned)tiles_of(p, kTile, kTile), (unsigned)a.splits), dim3(256), 0,
+                         stream, a);
       break;
     case kFew:
       hipLaunchKernelGGL((linear_few_kernel<E>),

@@ -116,7 +116,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     ``residual`` ``[..., N]`` are of that type or fp32; the result is of ``out_dtype`` (``x``'s by
     default, or fp32) or goes to ``out``, which may be ``residual`` itself and overlaps no other
     input.  ``activation``: ``"relu"``, ``"silu"``, ``"gelu"`` (erf), ``"gelu_tanh"`` or none.
-    Rows may lie at any stride; rows that start on 16-byte boundaries are read faster."""
+    Rows may lie at any stride; many rows go faster where they start on 16-byte
+    boundaries."""
     code = _dtype(x, "x")
     device = x.device
     if weight.dtype != x.dtype or weight.device != device or weight.dim() != 2:

@@ -44,8 +44,9 @@ extern "C" {
 #define FCV_LM_ACT_GELU_TANH 4
 
 /* y[i][j] = act(sum_k x[i][k] w[j][k] + bias[j]) + residual[i][j], rounded once; m and n
- * up to 2^22, their product up to 2^34, k up to 2^28.  Where all rows of x and w start on 16-byte boundaries they are read 16 bytes at a
- * time, others element by element.  y may be the residual itself (same type and stride); it
+ * up to 2^22, their product up to 2^34, k up to 2^28.  Rows may start on any
+ * element's boundary; where all rows of x and w start on 16-byte ones and k is a multiple of 8, many
+ * rows go faster.  y may be the residual itself (same type and stride); it
  * overlaps nothing else. */
 typedef struct FcvLmLinear {
   const void* x;        /* [m][k], row stride ldx */
