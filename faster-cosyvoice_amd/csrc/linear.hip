@@ -281,7 +281,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
   const int tiles_m = (p.m + BM - 1) / BM, tiles_n = (p.n + BN - 1) / BN;
   // blocks are dealt round-robin over the XCDs: each takes a contiguous range of the tiles, visited
   // in groups of kGroupM row tiles x all column tiles
-  int split, m0, n0;
+  int split, n0, m0;
   {
     const int total = tiles_m * tiles_n * a.splits;
     const int xcd = blockIdx.x % kXcds, idx = blockIdx.x / kXcds;

@@ -102,11 +102,33 @@ def _attention(fcv, ws=BIG, ws_bytes=1 << 40, **kw):
     (dict(q_head=60), "multiples of 8"), (dict(pv_row=-8), "multiples of 8"),
     (dict(k_row=1 << 24), "2\\^24"), (dict(out_head=0), "overlap"), (dict(out_row=0), "overlap"), (dict(lengths=None), "null"), (dict(prefix_v=None), "prefix"),
     (dict(out=BIG + 8), "16-byte"), (dict(prefix_k=BIG + 4), "16-byte"),
-    (dict(tokens=1 << 26), "2\\^26"), (dict(ws=None), "null workspace"),
-    (dict(ws_bytes=16), "too small"), (dict(ws=BIG + 16), "256-byte"),
+    (dict(tokens=1 << 26), "2\\^26"), (dict(ws=None, prefix_len=4000), "null workspace"),
+    (dict(ws_bytes=16, prefix_len=4000), "too small"),
+    (dict(ws=BIG + 16, prefix_len=4000), "256-byte"),
 ])
 def test_attention_refuses(fcv, bad, match):
     _refuse(fcv, _attention(fcv, **bad), match)
+
+
+def test_workspace_sizes(fcv):
+    """None where one launch does it all; it grows with the rows and holds a part a range."""
+    lib = fcv._lib.load()
+
+    def need(**kw):
+        base = dict(q=BIG, prefix_k=BIG, prefix_v=BIG, k_cache=BIG, v_cache=BIG, lengths=BIG,
+                    out=BIG, q_row=256, q_head=64, out_row=256, out_head=64, pk_row=128, pk_head=64,
+                    pv_row=128, pv_head=64, k_session=1 << 20, k_row=128, k_head=64,
+                    v_session=1 << 20, v_row=128, v_head=64, tokens=4, batch=4, n_heads=4,
+                    n_kv_heads=2, head_dim=64, prefix_len=7, sessions=64, capacity=5000, max_q=1,
+                    max_length=10, dtype=1, scale=0.125)
+        base.update(kw)
+        return lib.fcv_lm_prefix_attention_workspace_bytes(fcv._lib.FcvLmAttention(**base))
+
+    assert need() == 0 and need(tokens=0, q=None, out=None) == 0
+    few = need(prefix_len=5000)
+    assert few >= 2 * 4 * 4 * 64 * 4
+    assert need(prefix_len=5000, tokens=8, batch=8) > few
+    assert need(head_dim=65) == 0  # what the call refuses needs none
 
 
 def test_cpu_tensors_are_refused(fcv):
