@@ -1,17 +1,32 @@
 // Attention of a batch whose sequences share one prefix in front of caches of their own.
 //
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(t_j - max t + shift),  t_j = scale log2(e) q.k_j
-// over the prefix's keys and the sequence's own up to the query's.  The keys are split into parts;
-// each leaves its maximum m, its sum l and its unnormalised output, and a second launch joins a
-// query's parts in a fixed order:  M = max m,  out = sum 2^(m - M) o / sum 2^(m - M) l.
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(t_j - m + shift),  t_j = scale log2(e) q.k_j
+// over the prefix's keys and the sequence's own up to the query's, with m the running maximum of t (or
+// somewhat below it, see kLag).  The keys are split into parts; each leaves its m, its sum l of p and its
+// sum o of p v, and a second launch joins a query's parts in a fixed order:
+//   M = max m,  out = sum 2^(m - M) o / sum 2^(m - M) l.
 //
 // The prefix is read once for the batch: the queries of all sequences that read one key head are the
-// rows of one product against it.  A sequence's own keys meet its own queries only.
+// rows of one product against it.  A sequence's own keys meet its own queries only.  A sequence that
+// appends 128 rows (tokens x heads of a key head) or more reads prefix and own keys in one pass, and so
+// does a call of few keys; these need no join.
 //
 // Matrix form (v_mfma_f32_32x32x16): S^T = K Q^T puts query l % 32 into lane l with 16 of a tile's
 // 32 keys, so that the softmax is per lane (one exchange with lane l ^ 32) and the weights, rounded
 // to 16 bits, are the B operand of O^T = V^T P^T as they stand.  V^T's fragments are read from the
 // row-major tile by ds_read_b64_tr_b16, which hands each of 16 lanes one column of a 4 x 16 block.
+// Keys and values are copied straight into LDS.
+//
+// Bound and rate, 32 / 8 heads x 128 in bf16:
+//   64 queries behind a prompt of 8192 and 200 to 2000 own keys each: 95 to 105 us, 3.3 TB/s of the bytes
+//     that have to be read (the own keys alone 79 us, 3.75 TB/s; the prompt's product runs beside them);
+//   4 texts of 300 to 1024 tokens behind 4096 keys: 306 us, 0.71 PFLOP/s.  The vector pipe (32 exponentials
+//     and about 120 other instructions a wave and tile of 64 keys) and the matrix pipe (32 products) take
+//     their turns rather than overlap, and 77 % of the CU time is in blocks.  A tile's scores taken ahead
+//     beside the weights of the one before was slower (358 us: more registers, or half the tile), and so
+//     were fewer keys a barrier.  What cost most on the way were reloads of spilled registers: each waits
+//     for the copies in flight (522 to 308 us without).
+//   A token behind 512 + 100 keys: 9 us on the GPU.
 #include <algorithm>
 #include <cmath>
 
@@ -28,7 +43,8 @@ constexpr int kManyRows = 128;  // queries of a row tile whose waves share its q
 constexpr int kManyKeys = 64;   // keys of a workgroup's tile there
 constexpr int kStackedFew = 4096;  // rows of all key heads up to which stacked rows are taken 32 at a time
 constexpr int kShortKeys = 768;    // prefix and own keys up to which tiles of 32 queries take them all at once
-constexpr int kMaxParts = 64;   // lanes of the joining wave
+constexpr int kMaxKeys = 1 << 29;  // of the prefix and of a session: their sum and a tile more fit 31 bits
+constexpr int kMaxParts = 64;      // lanes of the joining wave
 constexpr float kLog2e = 1.4426950408889634f;
 
 // How a call is split.  Parts 0 .. np - 1 are ranges of the prefix for the rows of all sequences
@@ -589,7 +605,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const Args a) 
                        p.k_row, p.v_row};
   // keys [c0, c1) of the prefix (if it is read here) and the sequence's own behind it
   const int prefix_len = stacked || s.fused ? p.prefix_len : 0;
-  const int total = prefix_len + length;  // below 2^31: both are at most 2^30
+  const int total = prefix_len + length;  // at most 2 kMaxKeys
   const int step = stacked ? s.prefix_step : max(s.own_step, (total + s.no - 1) / s.no);
   const int c0 = (int)min((int64_t)range * step, (int64_t)total);
   const int c1 = (int)min((int64_t)c0 + step, (int64_t)total);
@@ -754,10 +770,10 @@ int check(const FcvLmAttention* p) {
             FCV_ERR_INVALID, "need batch >= 1 and tokens * n_heads in [0, 2^26)");
   FCV_CHECK(p->cu_q || p->tokens % p->batch == 0, FCV_ERR_INVALID,
             "without cu_q every sequence has tokens / batch queries: not a whole number");
-  FCV_CHECK(p->prefix_len >= 0 && p->prefix_len <= (1 << 30), FCV_ERR_INVALID,
-            "prefix_len must be in [0, 2^30]");
-  FCV_CHECK(p->sessions >= 1 && p->capacity >= 1 && p->capacity <= (1 << 30), FCV_ERR_INVALID,
-            "the caches need at least one session and a capacity in [1, 2^30]");
+  FCV_CHECK(p->prefix_len >= 0 && p->prefix_len <= kMaxKeys, FCV_ERR_INVALID,
+            "prefix_len must be in [0, 2^29]");
+  FCV_CHECK(p->sessions >= 1 && p->capacity >= 1 && p->capacity <= kMaxKeys, FCV_ERR_INVALID,
+            "the caches need at least one session and a capacity in [1, 2^29]");
   FCV_CHECK(p->slots || p->batch <= p->sessions, FCV_ERR_INVALID,
             "without slots the batch must not pass the sessions");
   FCV_CHECK(p->max_q >= 1 && p->max_length >= 0, FCV_ERR_INVALID, "need max_q >= 1 and max_length >= 0");

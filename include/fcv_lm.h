@@ -119,7 +119,8 @@ typedef struct FcvLmQkNormRope {
 
 int fcv_lm_qk_norm_rope(const FcvLmQkNormRope* args, hipStream_t stream);
 
-/* Rows cu_q[b] .. cu_q[b + 1] - 1 of q are the last queries of sequence b, n of them: query i sees
+/* Rows cu_q[b] .. cu_q[b + 1] - 1 of q (cu_q[0] = 0, non-decreasing) are the last queries of sequence b,
+ * n of them: query i sees
  * every key of the prefix (prefix_len of them, may be 0) and the keys of row slots[b] of the caches
  * up to its own, 0 .. lengths[b] - n + i (the new tokens' keys are in the cache already).  With
  * s = scale q.k over the visible keys
@@ -131,8 +132,9 @@ int fcv_lm_qk_norm_rope(const FcvLmQkNormRope* args, hipStream_t stream);
  * lengths are clipped to [0, capacity], and a slot outside [0, sessions) has no keys.
  * max_q and max_length bound the new tokens and the keys of a sequence: they shape the launch, and
  * a batch that passes them is computed all the same, more slowly.
- * head_dim is 64 or 128; strides are multiples of 8 and tensors start on 16-byte boundaries; a
- * key's or value's row stride is below 2^24. */
+ * prefix_len and capacity are at most 2^29, tokens * n_heads is below 2^26; head_dim is 64 or 128;
+ * strides are multiples of 8 and tensors start on 16-byte boundaries; a key's or value's row stride is
+ * below 2^24. */
 typedef struct FcvLmAttention {
   const void* q;          /* [tokens][n_heads][head_dim], strides q_row, q_head */
   const void* prefix_k;   /* [prefix_len][n_kv_heads][head_dim] */

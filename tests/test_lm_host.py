@@ -96,6 +96,7 @@ def _attention(fcv, ws=BIG, ws_bytes=1 << 40, **kw):
     (dict(dtype=2), "dtype"), (dict(head_dim=80), "head_dim"), (dict(n_heads=5), "multiple"),
     (dict(n_kv_heads=0), "multiple"), (dict(batch=0), "batch"), (dict(tokens=-4), "batch"),
     (dict(tokens=5), "whole number"), (dict(prefix_len=-1), "prefix_len"),
+    (dict(prefix_len=(1 << 29) + 1), "prefix_len"), (dict(capacity=1 << 30), "capacity"),
     (dict(sessions=0), "session"), (dict(sessions=3), "slots"), (dict(max_q=0), "max_q"),
     (dict(max_length=-1), "max_length"), (dict(scale=0.0), "scale"),
     (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
