@@ -829,16 +829,18 @@ void launch(const Args& a, hipStream_t stream) {
     hipLaunchKernelGGL((join_kernel<E, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
 }
 
+size_t workspace_bytes(const FcvLmAttention& p, const Shape& s) {
+  if (s.direct) return 0;
+  return (size_t)(sums_bytes(p, s) + (int64_t)s.parts() * p.tokens * p.n_heads * p.head_dim * 4);
+}
+
 }  // namespace
 }  // namespace lm
 }  // namespace fcv
 
 extern "C" size_t fcv_lm_prefix_attention_workspace_bytes(const FcvLmAttention* args) {
   if (fcv::lm::check(args) || args->tokens == 0) return 0;
-  const fcv::lm::Shape s = fcv::lm::shape_of(*args);
-  if (s.direct) return 0;
-  return (size_t)(fcv::lm::sums_bytes(*args, s) +
-                  (int64_t)s.parts() * args->tokens * args->n_heads * args->head_dim * 4);
+  return fcv::lm::workspace_bytes(*args, fcv::lm::shape_of(*args));
 }
 
 extern "C" int fcv_lm_prefix_attention(const FcvLmAttention* args, void* workspace,
@@ -846,15 +848,17 @@ extern "C" int fcv_lm_prefix_attention(const FcvLmAttention* args, void* workspa
   using namespace fcv::lm;
   if (int rc = check(args)) return rc;
   if (args->tokens == 0) return FCV_OK;
-  const size_t need = fcv_lm_prefix_attention_workspace_bytes(args);
+  Args a{*args, shape_of(*args), nullptr, nullptr, args->scale * kLog2e};
+  const size_t need = fcv::lm::workspace_bytes(*args, a.s);
   FCV_CHECK(need == 0 || workspace, FCV_ERR_INVALID, "null workspace");
   FCV_CHECK(workspace_bytes >= need, FCV_ERR_INVALID,
             "workspace too small: need " + std::to_string(need) + " bytes");
   FCV_CHECK(need == 0 || aligned(workspace, 256), FCV_ERR_INVALID,
             "workspace must be 256-byte aligned");
-  Args a{*args, shape_of(*args), nullptr, nullptr, args->scale * kLog2e};
-  a.part_s = static_cast<float2*>(workspace);
-  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_bytes(*args, a.s));
+  if (need) {
+    a.part_s = static_cast<float2*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_bytes(*args, a.s));
+  }
   const bool half = args->dtype == FCV_LM_F16;
   if (args->head_dim == 64)
     half ? launch<Half, 64>(a, stream) : launch<Bf16, 64>(a, stream);

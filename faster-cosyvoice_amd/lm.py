@@ -140,7 +140,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
             out_code = _F32
         else:
             raise ValueError(f"out must be {x.dtype} or float32, not {out_dtype}")
-        out = torch.empty(shape, dtype=x.dtype if out_dtype is None else out_dtype, device=device)
+        out = x.new_empty(shape) if out_code == code else x.new_empty(shape, dtype=out_dtype)
         ldy = n
     else:
         if out.shape != shape:
@@ -172,7 +172,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     need = _entry("fcv_lm_linear_workspace_bytes", 0)(args)
     fn = _entry("fcv_lm_linear", 3)
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws = x.new_empty(need, dtype=torch.uint8)
         _launch(fn, device.index, args, ws.data_ptr(), need)
     else:
         _launch(fn, device.index, args, None, 0)
@@ -239,7 +239,7 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
             or 0 in vs and any(n > 1 and st == 0 for n, st in zip(v_cache.shape, vs)):
         raise ValueError("k_cache or v_cache is expanded: its rows share memory")
     if out is None:
-        out = torch.empty((tokens, n_heads, dim), dtype=qkv.dtype, device=qkv.device)
+        out = qkv.new_empty((tokens, n_heads, dim))
     elif out.dtype != qkv.dtype or out.device != qkv.device or out.shape != (tokens, n_heads, dim) \
             or out.stride(2) != 1 or (n_heads > 1 and out.stride(1) != dim):
         raise ValueError(f"out must be a {qkv.dtype} tensor {(tokens, n_heads, dim)} on "
@@ -314,7 +314,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
             pk_ptr, pv_ptr = prefix_k.data_ptr(), prefix_v.data_ptr()
             pk, pv = prefix_k.stride(), prefix_v.stride()
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.device != q.device or out.shape != q.shape \
             or out.stride(2) != 1:
         raise ValueError(f"out must be a {q.dtype} tensor {tuple(q.shape)} on {q.device}, its last "
@@ -323,7 +323,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError("out is expanded: its rows share memory")
     lse = None
     if return_lse:
-        lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device)
+        lse = q.new_empty((tokens, heads), dtype=torch.float32)
     if tokens == 0:
         return (out, lse) if return_lse else out
     qs, os = q.stride(), out.stride()
@@ -335,10 +335,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         dim ** -0.5 if scale is None else scale)
     need = _entry("fcv_lm_prefix_attention_workspace_bytes", 0)(args)
     fn = _entry("fcv_lm_prefix_attention", 3)
-    device = q.device
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        _launch(fn, device.index, args, ws.data_ptr(), need)
+        ws = q.new_empty(need, dtype=torch.uint8)
+        _launch(fn, q.device.index, args, ws.data_ptr(), need)
     else:
-        _launch(fn, device.index, args, None, 0)
+        _launch(fn, q.device.index, args, None, 0)
     return (out, lse) if return_lse else out
