@@ -10,10 +10,10 @@
 //   linear_few_kernel   up to 16 rows, W read once into registers;
 //   linear_any_kernel   more rows off 16-byte boundaries, or K no multiple of 8: through registers.
 //
-// Bound and rate: large products by the matrix pipes, 8192 x 4096 x 8192 bf16 with bias and SiLU 450 us
-// (1.22 PFLOP/s; 61 % of the cycles at the clock the card holds under it, and the same within 10 % with
+// Bound and rate: large products by the matrix pipes, 8192 x 4096 x 8192 bf16 with bias and SiLU 460 us
+// (1.20 PFLOP/s; 61 % of the cycles at the clock the card holds under it, and the same within 10 % with
 // three to five slices of 32, with the copies asked for at once, and with four waves of 128 x 128); 9184 x
-// 1024 x 2048 with tanh-GELU 55 us, half of it rounds that are not full and stores that all CUs send at
+// 1024 x 2048 with tanh-GELU 58 us, half of it rounds that are not full and stores that all CUs send at
 // once.  Small products by what a CU takes in (about 55 B/ns of copies): 32 x 4096 x 4096 12 us.
 #include <algorithm>
 #include <type_traits>
@@ -236,7 +236,8 @@ struct Tile {
   static constexpr int kLds = STAGES * kStage * 2;
   static constexpr int kGroupM = 1024 / BM > 0 ? 1024 / BM : 1;
   static constexpr int kPerCu = 160 * 1024 / kLds;
-  static constexpr int kWavesPerSimd = kPerCu * kWaves >= 8 ? (kPerCu * kWaves >= 12 && TM * TN <= 2 ? 3 : 2) : 1;
+  // waves a SIMD that the registers have to leave room for
+  static constexpr int kWavesPerSimd = kPerCu * kWaves >= 8 ? 2 : 1;
   // small tiles: a whole slice's fragments are read at once, under the products of the slice before
   static constexpr bool kWhole = TM * TN == 1;
   static_assert(BM % (kCopyRows * kWaves) == 0 && BN % (kCopyRows * kWaves) == 0, "copy split");
@@ -304,8 +305,10 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
   const bool ragged = p.k % BK != 0 && slice0 + KT == all;  // the last slice passes K
 
   // byte offset of each copy's source from the tile's first row; rows past the matrix read its last
-  const char* xb = reinterpret_cast<const char*>(static_cast<const short*>(p.x) + (int64_t)m0 * p.ldx) + (int64_t)slice0 * BK * 2;
-  const char* wb = reinterpret_cast<const char*>(static_cast<const short*>(p.w) + (int64_t)n0 * p.ldw) + (int64_t)slice0 * BK * 2;
+  const char* xb = reinterpret_cast<const char*>(static_cast<const short*>(p.x) + (int64_t)m0 * p.ldx +
+                                                 (int64_t)slice0 * BK);
+  const char* wb = reinterpret_cast<const char*>(static_cast<const short*>(p.w) + (int64_t)n0 * p.ldw +
+                                                 (int64_t)slice0 * BK);
   const int crow = lane / C::kChunks, cpos = lane % C::kChunks;
   uint32_t x_off[C::kXCopies], w_off[C::kWCopies];
 #pragma unroll
