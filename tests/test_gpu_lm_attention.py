@@ -99,6 +99,41 @@ def test_ragged_appends(fcv, news, lengths, hq, hk, dim, dtype):
             check(fcv, a, "max_q too small", max_q=2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hk,dim", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("prefix", [0, 901, 2304])
+def test_key_ranges_are_joined(fcv, prefix, hq, hk, dim, dtype):
+    """Enough keys for several ranges of the prompt and of the caches; ranges that a short sequence does
+    not reach; bounds above and below the lengths."""
+    say(f"[attn] ranges, prefix {prefix}, {hq}/{hk} x {dim} {dtype}")
+    a = make([1, 2, 1, 3, 1], [1100, 2, 333, 64, 1], prefix, hq, hk, dim, dtype, capacity=1500)
+    check(fcv, a, "bounds", max_q=3, max_length=1100)
+    check(fcv, a, "capacity", max_q=3)
+    check(fcv, a, "too small", max_q=1, max_length=900)
+    slot = int(a["slots"][3])
+    for value in (float("inf"), -float("inf"), float("nan")):  # the last of three new tokens
+        a["v_cache"][slot, 63, 0, 5] = value
+        got, _ = check(fcv, a, "hidden", max_q=3, max_length=1100)
+        assert got[4:6].isfinite().all() and not got[6, 0, 5].isfinite()
+
+
+def test_many_stacked_rows_behind_a_prompt(fcv):
+    """More queries than tiles of 32 take against the prompt, few of each sequence."""
+    for dim, hq, hk in ((64, 64, 2), (128, 64, 8)):
+        say(f"[attn] 66 x {hq} stacked rows x {dim}")
+        lengths = [1 + 13 * i % 70 for i in range(66)]
+        a = make([1] * 66, lengths, 900, hq, hk, dim, torch.bfloat16)
+        check(fcv, a, "stacked", max_q=1, max_length=max(lengths))
+
+
+def test_uniform_rows_without_cu_q(fcv):
+    for n in (3, 40):
+        a = make([n] * 4, [n, 50, 64, 100], 77, 6, 2, 64, torch.float16)
+        want = fcv.prefix_attention(**a, max_q=n)
+        got, _ = check(fcv, dict(a, cu_q=None), "uniform")
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_rows_that_see_nothing(fcv, dim):
     """No prefix: an empty cache, more queries than keys, a slot outside the caches, a negative

@@ -83,6 +83,18 @@ def test_padding_rows_and_positions_past_the_tables(fcv):
     check(fcv, zero, pos, cos, sin, k, v, rows, 4, qw, kw, True, "zeros")
 
 
+def test_the_same_row_twice_holds_one_of_its_tokens(fcv):
+    qkv, pos, cos, sin, k, v, rows, qw, kw = make(fcv, 2, 4, 2, 64, 64, torch.bfloat16)
+    apart = [t.clone() for t in (k, v)]
+    fcv.qk_norm_rope(qkv, pos, cos, sin, *apart, rows, n_heads=4, q_weight=qw, k_weight=kw)
+    rows2 = rows[:1].repeat(2)
+    fcv.qk_norm_rope(qkv, pos, cos, sin, k, v, rows2, n_heads=4, q_weight=qw, k_weight=kw)
+    for got, both in zip((k, v), apart):
+        flat, other = got.view(-1, 2, 64), both.view(-1, 2, 64)
+        here = flat[int(rows[0])]
+        assert ((here == other[int(rows[0])]) | (here == other[int(rows[1])])).all()
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_strides(fcv, dim):
     """qkv and out inside wider buffers, caches with heads before positions, a prompt's own buffer."""
