@@ -37,6 +37,11 @@ _ATTENTION = struct.Struct("@10Q14q11if")
 _FNS: dict[str, object] = {}
 
 
+def _out_of_range(e: struct.error) -> ValueError:
+    """What a pack raises (floats past fp32 pack as infinities, which the library refuses)."""
+    return ValueError(f"a size is out of its argument's range: {e}")
+
+
 def _entry(name: str, n_tail: int):
     """The library entry ``name`` taking a packed struct, then workspace, bytes and stream (or as
     many of them as it has)."""
@@ -167,8 +172,12 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         res_ptr = residual.data_ptr()
     if m == 0:
         return out
-    args = _LINEAR.pack(x.data_ptr(), weight.data_ptr(), bias_ptr, res_ptr, out.data_ptr(), ldx, ldw,
-                        ldr, ldy, m, n, k, code, bias_code, res_code, out_code, act)
+    try:
+        args = _LINEAR.pack(
+            x.data_ptr(), weight.data_ptr(), bias_ptr, res_ptr, out.data_ptr(), ldx, ldw, ldr, ldy,
+            m, n, k, code, bias_code, res_code, out_code, act)
+    except struct.error as e:
+        raise _out_of_range(e) from e
     need = _entry("fcv_lm_linear_workspace_bytes", 0)(args)
     fn = _entry("fcv_lm_linear", 3)
     if need:
@@ -246,13 +255,16 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
                          f"{qkv.device} whose heads are contiguous")
     if tokens == 0:
         return out
-    args = _QK_NORM_ROPE.pack(
-        qkv.data_ptr(), pos_ptr, row_ptr, cos.data_ptr(), sin.data_ptr(),
-        0 if q_weight is None else q_weight.data_ptr(),
-        0 if k_weight is None else k_weight.data_ptr(), out.data_ptr(), k_cache.data_ptr(),
-        v_cache.data_ptr(), qkv_row, out.stride(0) if tokens > 1 else n_heads * dim, *ks[:3],
-        *vs[:3], tokens, n_heads, n_kv, dim, 2 * table[1], table[0], sessions, capacity, code,
-        w_code, bool(interleaved), eps)
+    try:
+        args = _QK_NORM_ROPE.pack(
+            qkv.data_ptr(), pos_ptr, row_ptr, cos.data_ptr(), sin.data_ptr(),
+            0 if q_weight is None else q_weight.data_ptr(),
+            0 if k_weight is None else k_weight.data_ptr(), out.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), qkv_row, out.stride(0) if tokens > 1 else n_heads * dim, *ks[:3],
+            *vs[:3], tokens, n_heads, n_kv, dim, 2 * table[1], table[0], sessions, capacity, code,
+            w_code, bool(interleaved), eps)
+    except struct.error as e:
+        raise _out_of_range(e) from e
     _launch(_entry("fcv_lm_qk_norm_rope", 1), qkv.device.index, args)
     return out
 
@@ -271,8 +283,9 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     sequence ``b`` reads session ``slots[b]`` (``b`` without ``slots``), its ``lengths[b]`` keys
     include those of its new tokens.  Its queries are rows ``cu_q[b] .. cu_q[b + 1] - 1``; without
     ``cu_q`` every sequence has ``T / len(lengths)``.  Rows past ``cu_q[-1]`` are not read, and
-    their rows of ``out`` stay as they are (whatever the memory held, without ``out``).  ``max_q`` and ``max_length`` bound the queries and keys of a sequence and shape the
-    launch (they default to ``T`` and the capacity); batches that pass them are still computed.
+    their rows of ``out`` stay as they are (whatever the memory held, without ``out``).  ``max_q`` and
+    ``max_length`` bound the queries and keys of a sequence and shape the launch (they default to
+    ``T`` and the capacity); batches that pass them are still computed.
     ``scale`` defaults to ``head dim ** -0.5``.  A query that sees no key gives zeros.  Returns
     the output, or with ``return_lse`` also the log sums of exponentials, fp32 ``[T, heads]``."""
     code = _dtype(q, "q")
@@ -327,12 +340,15 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if tokens == 0:
         return (out, lse) if return_lse else out
     qs, os = q.stride(), out.stride()
-    args = _ATTENTION.pack(
-        q.data_ptr(), pk_ptr, pv_ptr, k_cache.data_ptr(), v_cache.data_ptr(), cu_ptr, len_ptr,
-        slot_ptr, out.data_ptr(), 0 if lse is None else lse.data_ptr(), qs[0], qs[1], os[0], os[1],
-        pk[0], pk[1], pv[0], pv[1], *ks[:3], *vs[:3], tokens, batch, heads, n_kv, dim, prefix_len,
-        sessions, capacity, max_q, capacity if max_length is None else max_length, code,
-        dim ** -0.5 if scale is None else scale)
+    try:
+        args = _ATTENTION.pack(
+            q.data_ptr(), pk_ptr, pv_ptr, k_cache.data_ptr(), v_cache.data_ptr(), cu_ptr, len_ptr,
+            slot_ptr, out.data_ptr(), 0 if lse is None else lse.data_ptr(), qs[0], qs[1], os[0], os[1],
+            pk[0], pk[1], pv[0], pv[1], *ks[:3], *vs[:3], tokens, batch, heads, n_kv, dim, prefix_len,
+            sessions, capacity, max_q, capacity if max_length is None else max_length, code,
+            dim ** -0.5 if scale is None else scale)
+    except struct.error as e:
+        raise _out_of_range(e) from e
     need = _entry("fcv_lm_prefix_attention_workspace_bytes", 0)(args)
     fn = _entry("fcv_lm_prefix_attention", 3)
     if need:

@@ -279,6 +279,14 @@ def test_long_cache_offsets_pass_32_bits(fcv):
     assert ((got[0].double() - want).abs() <= 2 ** -6 * want.abs() + 1e-9).all()
 
 
+def test_bounds_past_32_bits_are_refused(fcv):
+    a = make([1, 1], [4, 5], 6, 4, 2, 64, torch.bfloat16)
+    for args, match in ((dict(max_q=1 << 31), "range"), (dict(max_length=1 << 31), "range"),
+                        (dict(scale=1e300), "scale")):
+        with pytest.raises(ValueError, match=match):
+            fcv.prefix_attention(**{**a, **args})
+
+
 def test_refusals(fcv):
     a = make([1, 1], [4, 5], 6, 4, 2, 64, torch.bfloat16)
 
