@@ -13,7 +13,7 @@
 //
 // Matrix form (v_mfma_f32_32x32x16): S^T = K Q^T puts query l % 32 into lane l with 16 of a tile's
 // 32 keys, so that the softmax is per lane (one exchange with lane l ^ 32) and the weights, rounded
-// to 16 bits, are the B operand of O^T = V^T P^T as they stand.  V^T's fragments are read from the
+// to 16 bits (bf16 of few queries: in two parts), are the B operand of O^T = V^T P^T as they stand.  V^T's fragments are read from the
 // row-major tile by ds_read_b64_tr_b16, which hands each of 16 lanes one column of a 4 x 16 block.
 // Keys and values are copied straight into LDS.
 //
@@ -240,10 +240,12 @@ __device__ __forceinline__ void tile_maximum(f32x16 (&s)[KT], State<D>& st, int 
   }
 }
 
-// The weights of the scores, and their sum.
-template <class E, int D, int KT>
+// The weights of the scores, and their sum.  The matrix instruction takes weights of 16 bits (relative
+// error 2^-9 bf16, 2^-12 fp16, each with its own sign; the sum keeps the unrounded ones).  With N = 2 a
+// weight goes in as two of them, rounded and rest.
+template <class E, int D, int KT, int N>
 __device__ __forceinline__ void tile_weights(const f32x16 (&s)[KT], State<D>& st, float scale2,
-                                             s16x8 (&pf)[2 * KT]) {
+                                             s16x8 (&pf)[N][2 * KT]) {
   const float shift = E::kShift - (st.m == -INFINITY ? 0.0f : st.m);
   float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -252,31 +254,38 @@ __device__ __forceinline__ void tile_weights(const f32x16 (&s)[KT], State<D>& st
     for (int e = 0; e < 16; ++e) {
       const float w = hw_exp2(fmaf(s[t][e], scale2, shift));
       sums[e & 3] += w;
-      // 16-bit weights (relative error 2^-9 bf16, 2^-12 fp16, each with its own sign): what the
-      // matrix instruction takes; the sum keeps the unrounded ones
-      pf[t * 2 + (e >> 3)][e & 7] = E::from_f32(w);
+      const short rounded = E::from_f32(w);
+      pf[0][t * 2 + (e >> 3)][e & 7] = rounded;
+      if constexpr (N == 2) pf[1][t * 2 + (e >> 3)][e & 7] = E::from_f32(w - E::to_f32(rounded));
     }
   st.l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 
 // O^T += V^T P^T of the values at LDS byte sv.  With hide, values that are not finite are left out and
 // noted in `found`.
-template <class E, int D, int KT>
-__device__ __forceinline__ void tile_values(uint32_t sv, const s16x8 (&pf)[2 * KT], State<D>& st, int lane,
-                                            bool hide, uint32_t& found) {
+template <class E, int D, int KT, int N>
+__device__ __forceinline__ void tile_values(uint32_t sv, const s16x8 (&pf)[N][2 * KT], State<D>& st,
+                                            int lane, bool hide, uint32_t& found) {
   const ValueFragments<D> values(sv, lane);
   if (hide) {
 #pragma unroll
     for (int k = 0; k < 2 * KT; ++k)
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-        st.acc[dt] = E::mfma32(finite_only<E>(values.get(k, dt), found), pf[k], st.acc[dt]);
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const s16x8 v = finite_only<E>(values.get(k, dt), found);
+#pragma unroll
+        for (int n = 0; n < N; ++n) st.acc[dt] = E::mfma32(v, pf[n][k], st.acc[dt]);
+      }
     return;
   }
 #pragma unroll
   for (int k = 0; k < 2 * KT; ++k)
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) st.acc[dt] = E::mfma32(values.get(k, dt), pf[k], st.acc[dt]);
+    for (int dt = 0; dt < D / 32; ++dt) {
+      const s16x8 v = values.get(k, dt);
+#pragma unroll
+      for (int n = 0; n < N; ++n) st.acc[dt] = E::mfma32(v, pf[n][k], st.acc[dt]);
+    }
 }
 
 // The queries of a row tile: rows first .. first + count - 1 of the (token, head of the group) pairs of
@@ -388,7 +397,7 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads have returned
       if (next < end) fetch_k(next);
       tile_maximum<E, D, 1>(scores, st, lane, (g == 0 ? end : limit) - kt, all_visible, a.scale2);
-      s16x8 pf[2];
+      s16x8 pf[E::kFewParts][2];
       tile_weights<E, D, 1>(scores, st, a.scale2, pf);
       if (next < end)
         wait_vmem<kCopies>();
@@ -508,7 +517,7 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
       f32x16 scores[2];
       tile_scores<E, D, 2>(sk, qf, lane, scores);
       tile_maximum<E, D, 2>(scores, st, lane, (g == 0 ? end : limit) - kt, all_visible, a.scale2);
-      s16x8 pf[4];
+      s16x8 pf[1][4];
       tile_weights<E, D, 2>(scores, st, a.scale2, pf);
       tile_values<E, D, 2>(sk + kTileElems * 2, pf, st, lane, g == 1 && !all_visible, found);
     }

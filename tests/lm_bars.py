@@ -43,14 +43,14 @@ def norm_rope(y, size, dim, normed, dtype):
     return (err + rounding(y.abs() + err, dtype)) * (1 + 2 ** -10)
 
 
-def attention(out, mass, score, keys, dim, dtype, v_max):
+def attention(out, mass, score, keys, dim, dtype, v_max, parts=1):
     """Scores are off by (dim + 4) U score; twice that relative in a weight (numerator and
-    denominator).  A weight is rounded to T: eps(T) / 2 relative.  fp16 weights are held at 2^11
-    times their size, so one below fp16's normal numbers (2^-14) is below 2^-25 of the row's
-    largest and off by at most that, read as zero or not.  Sums of `keys` weights and of the parts:
+    denominator).  A weight is rounded to T: eps(T) / 2 relative, and with `parts` 2 its rest
+    is rounded again.  fp16 weights are held at 2^11 times their size, so one below fp16's normal
+    numbers (2^-14) is below 2^-25 of the row's largest and off by at most that, read as zero or not.  Sums of `keys` weights and of the parts:
     (keys + 64) U."""
     score, keys = score[..., None], keys[..., None]
-    eps = torch.finfo(dtype).eps / 2
+    eps = (torch.finfo(dtype).eps / 2) ** parts
     rel = eps + 2 * ((dim + 4) * score + 8 + keys + 64) * U
     err = rel * mass
     if dtype == torch.float16:

@@ -51,7 +51,7 @@ def make(news, lengths, prefix, hq, hk, dim, dtype, seed=0, capacity=None, sessi
                 prefix_k=pk.to(DEV), prefix_v=pv.to(DEV), cu_q=ints(cu), slots=ints(slots))
 
 
-def check(fcv, a, what, scale=None, **kw):
+def check(fcv, a, what, scale=None, parts=1, **kw):
     got, lse = fcv.prefix_attention(**a, scale=scale, return_lse=True, **kw)
     q = a["q"]
     cpu = {n: None if t is None else t.cpu() for n, t in a.items() if n != "out"}
@@ -60,7 +60,7 @@ def check(fcv, a, what, scale=None, **kw):
     dim = q.shape[2]
     v_max = max([float(t.nan_to_num(0, 0, 0).abs().max()) for t in
                  (a["v_cache"], a.get("prefix_v")) if t is not None and t.numel()])
-    tol = bars.attention(out, mass, score, keys, dim, q.dtype, v_max)
+    tol = bars.attention(out, mass, score, keys, dim, q.dtype, v_max, parts)
     bars.assert_within(got[:live], out[:live], tol[:live], what)
     bars.assert_within(lse[:live], want_lse[:live], bars.lse(score, keys, dim, want_lse)[:live],
                        what + " lse")
@@ -115,6 +115,15 @@ def test_key_ranges_are_joined(fcv, prefix, hq, hk, dim, dtype):
         a["v_cache"][slot, 63, 0, 5] = value
         got, _ = check(fcv, a, "hidden", max_q=3, max_length=1100)
         assert got[4:6].isfinite().all() and not got[6, 0, 5].isfinite()
+
+
+@pytest.mark.parametrize("hq,hk,dim", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("prefix", [0, 512, 2304])
+def test_bf16_decode_rounds_the_result_alone(fcv, prefix, hq, hk, dim):
+    for sharp in (0.5, 2.0, 8.0):
+        say(f"[attn] weights in two parts, prefix {prefix}, {hq}/{hk} x {dim}, sharp {sharp}")
+        a = make([1] * 4, [100, 1, 333, 40], prefix, hq, hk, dim, torch.bfloat16, sharp=sharp)
+        check(fcv, a, "two parts", parts=2, max_q=1, max_length=333)
 
 
 def test_many_stacked_rows_behind_a_prompt(fcv):
