@@ -28,6 +28,7 @@
 //     for the copies in flight (522 to 308 us without).
 //   A token behind 512 + 100 keys: 9 us on the GPU.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "lm.hpp"
@@ -175,18 +176,8 @@ __device__ __forceinline__ s16x8 finite_only(const s16x8& v, uint32_t& found) {
   return __builtin_bit_cast(s16x8, __builtin_bit_cast(u16x8, v) & keep);
 }
 
-// What the finite_only of a row's visible keys [from, to) took from value dims d .. d + 3: the row gets
-// it back once its sums are done (a 0 weight on a hidden infinity would be NaN).  Seldom runs.
-template <class E>
-__device__ __forceinline__ f32x4 not_finite4(const short* v, int64_t v_row, int from, int to, int d) {
-  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int key = from; key < to; ++key) {
-    const s16x4 x = *reinterpret_cast<const s16x4*>(v + key * v_row + d);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if ((x[e] & E::kInf) == E::kInf) sum[e] += E::to_f32(x[e]);
-  }
-  return sum;
+__device__ __forceinline__ bool finite4(const f32x4& o) {
+  return fmaf(o[0], 0.0f, o[1] * 0.0f) + fmaf(o[2], 0.0f, o[3] * 0.0f) == 0.0f;
 }
 
 // The steps of a tile of 32 KT keys.
@@ -332,17 +323,40 @@ __device__ __forceinline__ void copy_rows(const short* tile, uint32_t row_bytes,
 }
 
 // LDS in elements: the tiles' keys and values ([kWaves][K, V][32][D], or [2][K, V][64][D]), and over them in
-// the end [kWaves][32] rows of O (16 bytes apart in their banks) with the waves' m and l behind them.
+// the end [kWaves][32] rows of O (16 bytes apart in their banks) with their m and l behind them, and the
+// first keys that mend_tile finds and any_bad's words.
 template <int D>
 constexpr int pitch() { return D + 4; }
 template <int D>
-constexpr int lds_elems() { return kWaves * 32 * (pitch<D>() * 2 + 4); }
+constexpr int lds_elems() { return kWaves * 32 * (pitch<D>() * 2 + 4) + 4 * D + 8; }
+template <int D>
+__device__ __forceinline__ float2* lds_sums(short* smem) {
+  return reinterpret_cast<float2*>(smem + kWaves * 32 * pitch<D>() * 2);
+}
+template <int D>
+__device__ __forceinline__ int* lds_first(short* smem) {
+  return reinterpret_cast<int*>(lds_sums<D>(smem) + kWaves * 32);
+}
+
+// Whether `bad` holds in any lane of the workgroup, through a word of each wave's in LDS (the library's
+// vote costs 64 long requests 5 us); ends in a barrier, and a barrier stands before the next call's words.
+template <int D>
+__device__ __forceinline__ bool any_bad(short* smem, bool bad) {
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
+  int* words = lds_first<D>(smem) + 2 * D;
+  const bool wave_bad = __any(bad);
+  if ((threadIdx.x & 63) == 0) words[threadIdx.x >> 6] = wave_bad;
+  __syncthreads();
+  const i32x4 v = *reinterpret_cast<const i32x4*>(words);
+  return ((v[0] | v[1]) | (v[2] | v[3])) != 0;
+}
 
 // A row tile of up to 32 queries against keys [k0, k1) of the prefix and [o0, o1) of the sequence's own; the
 // four waves take a range's tiles in turn, each through LDS buffers of its own (no barrier), and are joined
-// at the end.  first_pos: the position of the sequence's first new token.
+// at the end.  first_pos: the position of the sequence's first new token.  Whether the results need
+// mend_tile.
 template <class E, int D>
-__device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Segment& prefix, int k0,
+__device__ bool few_rows(const Args& a, short* smem, const Rows& rows, const Segment& prefix, int k0,
                          int k1, const Segment& own, int o0, int o1, int first_pos, int part) {
   const FcvLmAttention& p = a.p;
   if (k0 >= k1 && o0 >= o1 && !a.s.direct) {  // nothing to sum: no weight, no output that the join would read
@@ -351,7 +365,7 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
                          (int64_t)rows.token(threadIdx.x) * p.n_heads + rows.head(threadIdx.x);
       a.part_s[at] = float2{-INFINITY, 0.0f};
     }
-    return;
+    return false;
   }
   constexpr int kCopies = kFewKeys / (512 / D);
   constexpr int kTileElems = kFewKeys * D;
@@ -411,9 +425,9 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
 
   // join the waves: O is [wave][query][dim], four dims of a query a thread
   const float l_wave = half_sum(st.l);
-  const bool any_found = __syncthreads_or(found != 0);  // and every wave is done with its buffers
+  __syncthreads();  // every wave is done with its buffers
   float* so = reinterpret_cast<float*>(smem);
-  float2* ss = reinterpret_cast<float2*>(so + kWaves * kFewRows * pitch<D>());  // [kWaves][kFewRows]
+  float2* ss = lds_sums<D>(smem);  // [kWaves][kFewRows]
   if (ql < rows.count) {
     if (hl == 0) ss[wave * kFewRows + ql] = float2{st.m, l_wave};
 #pragma unroll
@@ -425,6 +439,7 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
   }
   __syncthreads();
   const int64_t rows_all = (int64_t)p.tokens * p.n_heads;
+  bool bad = found != 0;
   for (int i = threadIdx.x; i < rows.count * (D / 4); i += 256) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
     float m = -INFINITY;
@@ -440,11 +455,7 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
       l = fmaf(s.y, f, l);
       o += *reinterpret_cast<const f32x4*>(so + (w * kFewRows + r) * pitch<D>() + d) * f;
     }
-    if (any_found) {
-      const int from = max(o0, o0 + (low - o0) / kFewKeys * kFewKeys);  // the first tile with a mask
-      const int to = min(o1, first_pos + rows.token(r) - rows.token0 + 1);
-      o += not_finite4<E>(own.v, own.v_row, from, to, d);
-    }
+    bad |= !finite4(o);
     if (a.s.direct) {
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       *reinterpret_cast<s16x4*>(static_cast<short*>(p.out) + rows.token(r) * p.out_row +
@@ -460,13 +471,13 @@ __device__ void few_rows(const Args& a, short* smem, const Rows& rows, const Seg
     *reinterpret_cast<f32x4*>(a.part_o + at * D + d) = o;
     if (d == 0) a.part_s[at] = float2{m, l};
   }
-  __syncthreads();  // the next row tile fills the buffers again
+  return any_bad<D>(smem, bad);  // the next row tile fills the buffers again
 }
 
 // A row tile of up to 128 queries, 32 a wave, against keys [k0, k1) of the prefix and [o0, o1) of the
 // sequence's own; all waves share a tile of 64 keys in LDS, the next one on its way.
 template <class E, int D>
-__device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Segment& prefix, int k0,
+__device__ bool many_rows(const Args& a, short* smem, const Rows& rows, const Segment& prefix, int k0,
                           int k1, const Segment& own, int o0, int o1, int first_pos, int part) {
   constexpr int kCopies = kManyKeys / (512 / D) / kWaves;  // a wave's, of K and of V
   constexpr int kTileElems = kManyKeys * D;
@@ -523,17 +534,6 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
     }
   }
 
-  if (__any(found != 0)) {
-    const int from = max(o0, o0 + (low - o0) / kManyKeys * kManyKeys);  // the first tile with a mask
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 v = not_finite4<E>(own.v, own.v_row, from, limit, dt * 32 + g * 8 + hl * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) st.acc[dt][4 * g + e] += v[e];
-      }
-  }
   // through LDS, 32 lanes (16 of 64 dims) to a row, so that stores cover whole rows
   const float l = half_sum(st.l);
   __syncthreads();  // every wave is done with the last tile
@@ -548,6 +548,7 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   const int d = lane % (D / 4) * 4, mine = wave * 32;
+  bool bad = found != 0;
 #pragma unroll 4
   for (int q0 = 0; q0 < 32; q0 += 256 / D) {
     const int q = q0 + lane / (D / 4), r = mine + q;
@@ -555,6 +556,7 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
     if (r >= rows.count) continue;
     const f32x4 o = *reinterpret_cast<const f32x4*>(so + q * pitch<D>() + d);
     const int token = rows.token(r), head = rows.head(r);
+    bad |= !finite4(o);
     if (a.s.direct) {
       const float inv = lr > 0.0f || lr != lr ? 1.0f / lr : 0.0f;
       *reinterpret_cast<s16x4*>(static_cast<short*>(p.out) + token * p.out_row + head * p.out_head + d) =
@@ -568,74 +570,196 @@ __device__ void many_rows(const Args& a, short* smem, const Rows& rows, const Se
       if (d == 0) a.part_s[at] = float2{mr, lr};
     }
   }
+  if (hl == 0) lds_sums<D>(smem)[wave * 32 + ql] = float2{st.m, l};  // for mend_tile
+  return any_bad<D>(smem, bad);  // the next row tile fills the buffers again
+}
+
+// What a workgroup does: a key head's rows of all sequences or of one, against a range of its keys.
+struct Work {
+  int kvh, group, part, token0, tokens, length, prefix_len;
+  int c0, c1;  // the range: keys of the prefix (if it is read here) and the sequence's own behind it
+  int first_tile, tiles, stride, tile_rows;
+  bool stacked;
+  Segment prefix, own;
+};
+
+template <bool MANY>
+__device__ __forceinline__ Work work_of(const Args& a, uint32_t b) {
+  const FcvLmAttention& p = a.p;
+  const Shape& s = a.s;
+  Work w;
+  w.group = p.n_heads / p.n_kv_heads;
+  w.stacked = b < (uint32_t)s.prefix_blocks;
+  if (!w.stacked) b -= (uint32_t)s.prefix_blocks;
+  // key head fastest: the row tiles of one head and range are dealt to one XCD and share its L2
+  w.kvh = scalar((int)(b % (uint32_t)p.n_kv_heads));
+  b /= (uint32_t)p.n_kv_heads;
+  const uint32_t ranges = w.stacked ? s.np : s.no;
+  const int range = scalar((int)(b % ranges));
+  b /= ranges;
+
+  int slot = 0;
+  w.token0 = w.length = 0;
+  w.first_tile = (int)b;
+  if (w.stacked) {
+    w.tokens = p.cu_q ? min(max(p.cu_q[p.batch], 0), p.tokens) : p.tokens;
+  } else {
+    const int seq = scalar((int)(b % (uint32_t)p.batch));
+    w.first_tile = (int)(b / (uint32_t)p.batch);
+    if (p.cu_q) {
+      w.token0 = min(max(p.cu_q[seq], 0), p.tokens);
+      w.tokens = min(max(p.cu_q[seq + 1], w.token0), p.tokens) - w.token0;
+    } else {
+      w.tokens = p.tokens / p.batch;
+      w.token0 = seq * w.tokens;
+    }
+    slot = p.slots ? p.slots[seq] : seq;
+    w.length = min(max(p.lengths[seq], 0), p.capacity);
+    if (slot < 0 || slot >= p.sessions) slot = w.length = 0;
+  }
+  w.prefix = {static_cast<const short*>(p.prefix_k) + w.kvh * p.pk_head,
+              static_cast<const short*>(p.prefix_v) + w.kvh * p.pv_head, p.pk_row, p.pv_row};
+  w.own = {static_cast<const short*>(p.k_cache) + slot * p.k_session + w.kvh * p.k_head,
+           static_cast<const short*>(p.v_cache) + slot * p.v_session + w.kvh * p.v_head, p.k_row, p.v_row};
+  w.prefix_len = w.stacked || s.fused ? p.prefix_len : 0;
+  const int total = w.prefix_len + w.length;  // at most 2 kMaxKeys
+  const int step = w.stacked ? s.prefix_step : max(s.own_step, (total + s.no - 1) / s.no);
+  w.c0 = (int)min((int64_t)range * step, (int64_t)total);
+  w.c1 = (int)min((int64_t)w.c0 + step, (int64_t)total);
+  w.part = w.stacked ? range : s.np + range;
+  w.tile_rows = MANY ? kManyRows : kFewRows;
+  w.tiles = (w.tokens * w.group + w.tile_rows - 1) / w.tile_rows;
+  w.stride = w.stacked ? s.prefix_tiles : s.own_tiles;
+  return w;
+}
+
+// The rows of one of its tiles, and their keys: [k0, k1) of the prefix, [o0, o1) of the sequence's own.
+struct TileWork {
+  Rows rows;
+  int k0, k1, o0, o1, first_pos;
+};
+
+__device__ __forceinline__ TileWork tile_of(const Work& w, int index) {
+  TileWork t;
+  const int first = index * w.tile_rows;
+  t.rows = {w.kvh, w.group, w.token0, first, min(w.tile_rows, w.tokens * w.group - first)};
+  t.first_pos = w.length - w.tokens;
+  // own keys past the tile's last query are not visited
+  const int seen =
+      w.stacked ? 0 : min(w.length, t.first_pos + (first + t.rows.count - 1) / w.group + 1);
+  t.k0 = min(w.c0, w.prefix_len);
+  t.k1 = min(w.c1, w.prefix_len);
+  t.o0 = max(w.c0 - w.prefix_len, 0);
+  t.o1 = min(max(w.c1 - w.prefix_len, 0), seen);
+  return t;
+}
+
+// Values that are not finite and that a query sees.  Every visible key has a weight above zero, so an
+// infinity among the values is what the row gets, and NaN for NaN or for both infinities.  The products
+// do not keep to that: a weight that rounds to zero or whose second part is negative makes NaN of an
+// infinity, a row read again behind a range's end has a weight of zero, and masked tiles leave such values
+// out.  All of these leave a sum that is not finite, or a note in `found`; the tile's values are then
+// looked through, and what each row sees is written over its results (a row whose sum of weights is NaN
+// has NaN already).  Seldom runs, takes about as long as the tile itself, and derives all it needs again
+// from opaque copies of the kernel's arguments: with what it needs kept from the key loops on, every call
+// pays (a token 10.2 to 11.1 us, 64 long requests 108 to 118 us; so 10.1 and 112), and as a function of
+// its own it costs small calls 0.6 us.
+typedef const __attribute__((address_space(4))) Args* ArgsAt;
+
+template <class E, int D, bool MANY>
+__device__ __forceinline__ void mend_tile(ArgsAt at, __attribute__((address_space(3))) short* lds,
+                                          uint32_t block, int index) {
+  const Args& a = *(const Args*)at;
+  const FcvLmAttention& p = a.p;
+  short* smem = (short*)lds;
+  const Work w = work_of<MANY>(a, block);
+  const TileWork t = tile_of(w, index);
+  __threadfence();  // the results stand before they are written over
+  // first[0][d], first[1][d]: the first own key whose value in dim d is inf or NaN, -inf or NaN; a key of
+  // the prefix, which every query sees, stands before all of them
+  int* first = lds_first<D>(smem);
+  for (int i = threadIdx.x; i < 2 * D; i += 64 * kWaves) first[i] = INT_MAX;
+  __syncthreads();
+  constexpr int kKeys = 64 * kWaves / (D / 8);  // a step's; 8 dims a thread
+  const int d = threadIdx.x % (D / 8) * 8, key0 = threadIdx.x / (D / 8);
+  int up[8], down[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) up[e] = down[e] = INT_MAX;
+#pragma unroll 1
+  for (int g = 0; g < 2; ++g) {
+    const short* v = (g == 0 ? w.prefix.v : w.own.v) + d;
+    const int64_t v_row = g == 0 ? w.prefix.v_row : w.own.v_row;
+    const int end = g == 0 ? t.k1 : t.o1;
+#pragma unroll 1
+    for (int key = (g == 0 ? t.k0 : t.o0) + key0; key < end; key += 4 * kKeys) {
+      s16x8 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)  // four asked for at once; keys past the end are the last one again
+        x[u] = *reinterpret_cast<const s16x8*>(v + (int64_t)min(key + u * kKeys, end - 1) * v_row);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = E::to_f32(x[u][e]);
+          const int here = g == 0 ? INT_MIN : min(key + u * kKeys, end - 1);
+          if (!(f < INFINITY)) up[e] = min(up[e], here);
+          if (!(f > -INFINITY)) down[e] = min(down[e], here);
+        }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (up[e] != INT_MAX) atomicMin(first + d + e, up[e]);
+    if (down[e] != INT_MAX) atomicMin(first + D + d + e, down[e]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.rows.count * D; i += 64 * kWaves) {
+    const int r = i / D, dim = i % D, token = t.rows.token(r), head = t.rows.head(r);
+    const int limit = min(t.o1, t.first_pos + token - w.token0 + 1);  // the first own key past its view
+    const bool has_up = first[dim] < limit, has_down = first[D + dim] < limit;
+    if (!has_up && !has_down) continue;
+    float o = has_up && has_down ? NAN : has_up ? INFINITY : -INFINITY;
+    if (a.s.direct) {
+      const float2* ss = lds_sums<D>(smem) + r;  // of the row, or of each wave's share of its keys
+#pragma unroll
+      for (int k = 0; k < (MANY ? 1 : kWaves); ++k)
+        if (ss[k * kFewRows].y != ss[k * kFewRows].y) o = NAN;
+      static_cast<short*>(p.out)[token * p.out_row + head * p.out_head + dim] = E::from_f32(o);
+    } else {
+      a.part_o[(((int64_t)w.part * p.tokens + token) * p.n_heads + head) * D + dim] = o;
+    }
+  }
   __syncthreads();  // the next row tile fills the buffers again
 }
 
 // The blocks of the stacked rows first, then the sequences'; a launch has those of one kind of tile.
-// (Both kinds in one kernel need more registers than two workgroups a CU have.)
+// (Both kinds in one kernel need more registers than two workgroups a CU have; few queries of 64 dims leave
+// room for three.)
 template <class E, int D, bool MANY>
-__global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const Args a) {
+__global__ __launch_bounds__(256, D == 64 && !MANY ? 3 : 2) void prefix_attention_kernel(const Args a) {
   __shared__ __attribute__((aligned(1024))) short smem[lds_elems<D>()];
-  const FcvLmAttention& p = a.p;
-  const Shape& s = a.s;
-  const int group = p.n_heads / p.n_kv_heads;
-  int64_t b = blockIdx.x;
-  const bool stacked = b < s.prefix_blocks;
-  if (!stacked) b -= s.prefix_blocks;
-  // key head fastest: the row tiles of one head and range are dealt to one XCD and share its L2
-  const int kvh = scalar((int)(b % p.n_kv_heads));
-  b /= p.n_kv_heads;
-  const int ranges = stacked ? s.np : s.no;
-  const int range = scalar((int)(b % ranges));
-  b /= ranges;
-
-  // the rows token0 .. of all sequences or of one, and its keys
-  int token0 = 0, tokens, slot = 0, length = 0, first_tile = (int)b;
-  if (stacked) {
-    tokens = p.cu_q ? min(max(p.cu_q[p.batch], 0), p.tokens) : p.tokens;
-  } else {
-    const int seq = scalar((int)(b % p.batch));
-    first_tile = (int)(b / p.batch);
-    if (p.cu_q) {
-      token0 = min(max(p.cu_q[seq], 0), p.tokens);
-      tokens = min(max(p.cu_q[seq + 1], token0), p.tokens) - token0;
-    } else {
-      tokens = p.tokens / p.batch;
-      token0 = seq * tokens;
-    }
-    slot = p.slots ? p.slots[seq] : seq;
-    length = min(max(p.lengths[seq], 0), p.capacity);
-    if (slot < 0 || slot >= p.sessions) slot = length = 0;
-  }
-  const Segment prefix = {static_cast<const short*>(p.prefix_k) + kvh * p.pk_head,
-                          static_cast<const short*>(p.prefix_v) + kvh * p.pv_head, p.pk_row, p.pv_row};
-  const Segment own = {static_cast<const short*>(p.k_cache) + slot * p.k_session + kvh * p.k_head,
-                       static_cast<const short*>(p.v_cache) + slot * p.v_session + kvh * p.v_head,
-                       p.k_row, p.v_row};
-  // keys [c0, c1) of the prefix (if it is read here) and the sequence's own behind it
-  const int prefix_len = stacked || s.fused ? p.prefix_len : 0;
-  const int total = prefix_len + length;  // at most 2 kMaxKeys
-  const int step = stacked ? s.prefix_step : max(s.own_step, (total + s.no - 1) / s.no);
-  const int c0 = (int)min((int64_t)range * step, (int64_t)total);
-  const int c1 = (int)min((int64_t)c0 + step, (int64_t)total);
-  const int part = stacked ? range : s.np + range;
-  constexpr int tile_rows = MANY ? kManyRows : kFewRows;
-  const int n_rows = tokens * group, first_pos = length - tokens;
-  const int tiles = (n_rows + tile_rows - 1) / tile_rows;
-  const int stride = stacked ? s.prefix_tiles : s.own_tiles;
-  for (int i = scalar(first_tile); i < tiles; i += stride) {
-    const int index = tiles - 1 - i;  // the last tiles see the most keys and go first
-    const int first = index * tile_rows;
-    const Rows rows = {kvh, group, token0, first, min(tile_rows, n_rows - first)};
-    // own keys past the tile's last query are not visited
-    const int seen = stacked ? 0 : min(length, first_pos + (first + rows.count - 1) / group + 1);
-    const int p0 = min(c0, prefix_len), p1 = min(c1, prefix_len);
-    const int o0 = max(c0 - prefix_len, 0), o1 = min(max(c1 - prefix_len, 0), seen);
+  const Work w = work_of<MANY>(a, blockIdx.x);
+  for (int i = scalar(w.first_tile); i < w.tiles; i += w.stride) {
+    const int index = w.tiles - 1 - i;  // the last tiles see the most keys and go first
+    const TileWork t = tile_of(w, index);
+    bool bad;
     if constexpr (MANY)
-      many_rows<E, D>(a, smem, rows, prefix, p0, p1, own, o0, o1, first_pos, part);
+      bad = many_rows<E, D>(a, smem, t.rows, w.prefix, t.k0, t.k1, w.own, t.o0, t.o1, t.first_pos, w.part);
     else
-      few_rows<E, D>(a, smem, rows, prefix, p0, p1, own, o0, o1, first_pos, part);
+      bad = few_rows<E, D>(a, smem, t.rows, w.prefix, t.k0, t.k1, w.own, t.o0, t.o1, t.first_pos, w.part);
+    if (bad) {
+      // opaque, so that nothing of what it derives is shared with the code above and kept until here
+      ArgsAt args = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
+      uint32_t block = blockIdx.x;
+      asm volatile("" : "+s"(args), "+s"(block));
+      mend_tile<E, D, MANY>(args, (__attribute__((address_space(3))) short*)smem, block, index);
+    }
   }
+}
+
+// o + v w; what a row saw that is not finite stays, however small the part's weight.
+__device__ __forceinline__ float add_part(float v, float w, float o) {
+  return fabsf(v) < INFINITY ? fmaf(v, w, o) : o + v;
 }
 
 // Joins the parts of each (token, head): W waves to a row, each its share of the parts, eight at a time;
@@ -659,8 +783,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   const float f = hw_exp2(part.x - (top == -INFINITY ? 0.0f : top));
   const float l = wave_sum(part.y * f);
   float2 o = {0.0f, 0.0f};
-  // a part without weight (a range that a short sequence does not reach) was not written
-  const uint64_t live_parts = __ballot(f != 0.0f);
+  // a part without keys (a range that a short sequence does not reach) was not written
+  const uint64_t live_parts = __ballot(part.x != -INFINITY);
   for (int i0 = mine; i0 < parts; i0 += 8 * W) {
     float2 v[8];
 #pragma unroll
@@ -680,8 +804,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
       const int i = i0 + u * W;
       if (i >= parts) break;
       const float w = __shfl(f, i, kWave);
-      o.x = fmaf(v[u].x, w, o.x);
-      if (D == 128) o.y = fmaf(v[u].y, w, o.y);
+      o.x = add_part(v[u].x, w, o.x);
+      if (D == 128) o.y = add_part(v[u].y, w, o.y);
     }
   }
   if constexpr (W > 1) {

@@ -126,7 +126,8 @@ int fcv_lm_qk_norm_rope(const FcvLmQkNormRope* args, hipStream_t stream);
  * s = scale q.k over the visible keys
  *   out = sum exp(s) v / sum exp(s),   lse = log sum exp(s).
  * A query that sees no key gives out = 0 and lse = -inf; keys and values that a query does not see
- * do not touch its result, whatever they hold.  Query head h reads key head h / (n_heads /
+ * do not touch its result, whatever they hold.  Of the values that it sees an infinity is what it
+ * gets, however small the weight, and NaN for NaN or both infinities.  Query head h reads key head h / (n_heads /
  * n_kv_heads).  Rows of q past cu_q[batch] are not read, and their rows of out and lse stay as they
  * were.  cu_q NULL: tokens / batch rows for every sequence; slots NULL: sequence b has session b.
  * lengths are clipped to [0, capacity], and a slot outside [0, sessions) has no keys.
