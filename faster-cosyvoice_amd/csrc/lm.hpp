@@ -17,7 +17,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // Element types: bits <-> fp32 (to the nearest, ties to even) and D = A B + C on fragments.
 struct Half {
-  typedef f16 T;
+  typedef f16x2 T2;
   static constexpr short kOne = 0x3C00;        // 1.0
   static constexpr short kInf = 0x7C00;        // +inf, and the exponent's mask
   // Softmax: a row's running maximum follows the true one when that is kLag (in powers of two) above
@@ -25,7 +25,6 @@ struct Half {
   // no weight passes 2^15, and one is in the normal range down to 2^-25 of the row's largest (many
   // small weights can carry most of a long row's sum).
   static constexpr float kShift = 11.0f, kLag = 4.0f;
-  static constexpr int kFewParts = 1;  // 16-bit parts of a weight in tiles of few queries
   static __device__ __forceinline__ float to_f32(short b) { return (float)__builtin_bit_cast(f16, b); }
   static __device__ __forceinline__ short from_f32(float v) {
     return __builtin_bit_cast(short, f2h(v));
@@ -41,16 +40,11 @@ struct Half {
 };
 
 struct Bf16 {
-  typedef __bf16 T;
+  typedef __bf16 T2 __attribute__((ext_vector_type(2)));
   static constexpr short kOne = 0x3F80;
   static constexpr short kInf = 0x7F80;
   // bf16 has fp32's range: sums of 2^16 of its largest values do not pass fp32's
   static constexpr float kShift = -24.0f, kLag = 8.0f;
-  // Two parts: with one, the weights' rounding is as large as the result's (a token behind 612 keys is
-  // off by 2.4e-3 relative L2, 1.6e-3 with two, which is the result's rounding alone) and a tile of 32
-  // keys has 8 products of 128 dims less; the calls are bound by latency or the cache's bytes and take
-  // the same time (12.8 us, and 64 long requests 100 to 104 us).
-  static constexpr int kFewParts = 2;
   static __device__ __forceinline__ float to_f32(short b) {
     return __uint_as_float((uint32_t)(uint16_t)b << 16);
   }

@@ -12,9 +12,9 @@
 // does a call of few keys; these need no join.
 //
 // Matrix form (v_mfma_f32_32x32x16): S^T = K Q^T puts query l % 32 into lane l with 16 of a tile's
-// 32 keys, so that the softmax is per lane (one exchange with lane l ^ 32) and the weights, rounded
-// to 16 bits (bf16 of few queries: in two parts), are the B operand of O^T = V^T P^T as they stand.  V^T's fragments are read from the
-// row-major tile by ds_read_b64_tr_b16, which hands each of 16 lanes one column of a 4 x 16 block.
+// 32 keys, so that the softmax is per lane (one exchange with lane l ^ 32) and the weights, in two 16-bit
+// parts, are the B operand of O^T = V^T P^T as they stand.  V^T's fragments are read from the row-major
+// tile by ds_read_b64_tr_b16, which hands each of 16 lanes one column of a 4 x 16 block.
 // Keys and values are copied straight into LDS.
 //
 // Bound and rate, 32 / 8 heads x 128 in bf16:
@@ -231,51 +231,109 @@ __device__ __forceinline__ void tile_maximum(f32x16 (&s)[KT], State<D>& st, int 
   }
 }
 
-// The weights of the scores, and their sum.  The matrix instruction takes weights of 16 bits (relative
-// error 2^-9 bf16, 2^-12 fp16, each with its own sign; the sum keeps the unrounded ones).  With N = 2 a
-// weight goes in as two of them, rounded and rest.
-template <class E, int D, int KT, int N>
-__device__ __forceinline__ void tile_weights(const f32x16 (&s)[KT], State<D>& st, float scale2,
-                                             s16x8 (&pf)[N][2 * KT]) {
+// The weights of a lane's scores 8 h .. + 7, and their sums.  The matrix instruction takes 16-bit operands,
+// so that a weight goes in as two of them, rounded and rest: together they are off by 2^-16 (bf16) or 2^-22
+// (fp16) of it, and a result's error is that of its own rounding.  With the rounded one alone it is 1.4
+// times that (2.33e-3 against 1.66e-3 relative L2 for texts in bf16), at 16 products of 48 less a wave and
+// tile of 64 keys: texts behind 4096 keys 307 against 393 us, tokens the same time (fp16 up to 6 % more).
+template <class E>
+__device__ __forceinline__ void weights8(const f32x16& s, int h, float scale2, float shift,
+                                         float (&sums)[4], s16x8 (&pf)[2]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  typedef typename E::T2 T2;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const f32x2 w = {hw_exp2(fmaf(s[8 * h + e], scale2, shift)),
+                     hw_exp2(fmaf(s[8 * h + e + 1], scale2, shift))};
+    sums[e & 3] += w[0];
+    sums[(e & 3) + 1] += w[1];
+    const T2 r = __builtin_convertvector(w, T2);
+    const f32x2 rest = {w[0] - (float)r[0], w[1] - (float)r[1]};
+    const s16x2 p0 = __builtin_bit_cast(s16x2, r);
+    const s16x2 p1 = __builtin_bit_cast(s16x2, __builtin_convertvector(rest, T2));
+    pf[0][e] = p0[0];
+    pf[0][e + 1] = p0[1];
+    pf[1][e] = p1[0];
+    pf[1][e + 1] = p1[1];
+  }
+}
+
+// O^T += V^T P^T of 16 keys, step k of a tile.  With HIDE, values that are not finite are left out and
+// noted in `found`.
+template <class E, int D, bool HIDE>
+__device__ __forceinline__ void values16(const ValueFragments<D>& values, int k, const s16x8 (&pf)[2],
+                                         State<D>& st, uint32_t& found) {
+  s16x8 v[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) {
+    v[dt] = values.get(k, dt);
+    if (HIDE) v[dt] = finite_only<E>(v[dt], found);
+  }
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) st.acc[dt] = E::mfma32(v[dt], pf[n], st.acc[dt]);
+}
+
+// Weights and values of a tile of 32 KT keys with the values at LDS byte sv, 16 keys after another: two
+// parts of all weights of 64 keys at once are more registers than two workgroups a CU have (456 us for the
+// 393 above).
+template <class E, int D, int KT, bool HIDE>
+__device__ __forceinline__ void tile_steps(const f32x16 (&s)[KT], uint32_t sv, State<D>& st, float scale2,
+                                           int lane, uint32_t& found) {
+  const ValueFragments<D> values(sv, lane);
   const float shift = E::kShift - (st.m == -INFINITY ? 0.0f : st.m);
   float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float w = hw_exp2(fmaf(s[t][e], scale2, shift));
-      sums[e & 3] += w;
-      const short rounded = E::from_f32(w);
-      pf[0][t * 2 + (e >> 3)][e & 7] = rounded;
-      if constexpr (N == 2) pf[1][t * 2 + (e >> 3)][e & 7] = E::from_f32(w - E::to_f32(rounded));
-    }
+  for (int k = 0; k < 2 * KT; ++k) {
+    s16x8 pf[2];
+    weights8<E>(s[k / 2], k % 2, scale2, shift, sums, pf);
+    values16<E, D, HIDE>(values, k, pf, st, found);
+  }
   st.l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
+template <class E, int D, int KT>
+__device__ __forceinline__ void tile_steps(const f32x16 (&s)[KT], uint32_t sv, State<D>& st, float scale2,
+                                           int lane, bool hide, uint32_t& found) {
+  if (hide)
+    tile_steps<E, D, KT, true>(s, sv, st, scale2, lane, found);
+  else
+    tile_steps<E, D, KT, false>(s, sv, st, scale2, lane, found);
+}
 
-// O^T += V^T P^T of the values at LDS byte sv.  With hide, values that are not finite are left out and
-// noted in `found`.
-template <class E, int D, int KT, int N>
-__device__ __forceinline__ void tile_values(uint32_t sv, const s16x8 (&pf)[N][2 * KT], State<D>& st,
-                                            int lane, bool hide, uint32_t& found) {
+// The same of 32 keys, apart, so that the weights do not wait for the values.
+template <class E, int D>
+__device__ __forceinline__ void tile_weights(const f32x16& s, State<D>& st, float scale2,
+                                             s16x8 (&pf)[2][2]) {
+  const float shift = E::kShift - (st.m == -INFINITY ? 0.0f : st.m);
+  float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  weights8<E>(s, 0, scale2, shift, sums, pf[0]);
+  weights8<E>(s, 1, scale2, shift, sums, pf[1]);
+  st.l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+}
+template <class E, int D>
+__device__ __forceinline__ void tile_values(uint32_t sv, const s16x8 (&pf)[2][2], State<D>& st, int lane,
+                                            bool hide, uint32_t& found) {
   const ValueFragments<D> values(sv, lane);
   if (hide) {
 #pragma unroll
-    for (int k = 0; k < 2 * KT; ++k)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt) {
         const s16x8 v = finite_only<E>(values.get(k, dt), found);
 #pragma unroll
-        for (int n = 0; n < N; ++n) st.acc[dt] = E::mfma32(v, pf[n][k], st.acc[dt]);
+        for (int n = 0; n < 2; ++n) st.acc[dt] = E::mfma32(v, pf[k][n], st.acc[dt]);
       }
     return;
   }
 #pragma unroll
-  for (int k = 0; k < 2 * KT; ++k)
+  for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
       const s16x8 v = values.get(k, dt);
 #pragma unroll
-      for (int n = 0; n < N; ++n) st.acc[dt] = E::mfma32(v, pf[n][k], st.acc[dt]);
+      for (int n = 0; n < 2; ++n) st.acc[dt] = E::mfma32(v, pf[k][n], st.acc[dt]);
     }
 }
 
@@ -411,13 +469,13 @@ __device__ bool few_rows(const Args& a, short* smem, const Rows& rows, const Seg
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads have returned
       if (next < end) fetch_k(next);
       tile_maximum<E, D, 1>(scores, st, lane, (g == 0 ? end : limit) - kt, all_visible, a.scale2);
-      s16x8 pf[E::kFewParts][2];
-      tile_weights<E, D, 1>(scores, st, a.scale2, pf);
+      s16x8 pf[2][2];
+      tile_weights<E, D>(scores[0], st, a.scale2, pf);
       if (next < end)
         wait_vmem<kCopies>();
       else
         wait_vmem<0>();
-      tile_values<E, D, 1>(sv, pf, st, lane, g == 1 && !all_visible, found);
+      tile_values<E, D>(sv, pf, st, lane, g == 1 && !all_visible, found);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (next < end) fetch_v(next);
     }
@@ -528,9 +586,7 @@ __device__ bool many_rows(const Args& a, short* smem, const Rows& rows, const Se
       f32x16 scores[2];
       tile_scores<E, D, 2>(sk, qf, lane, scores);
       tile_maximum<E, D, 2>(scores, st, lane, (g == 0 ? end : limit) - kt, all_visible, a.scale2);
-      s16x8 pf[1][4];
-      tile_weights<E, D, 2>(scores, st, a.scale2, pf);
-      tile_values<E, D, 2>(sk + kTileElems * 2, pf, st, lane, g == 1 && !all_visible, found);
+      tile_steps<E, D, 2>(scores, sk + kTileElems * 2, st, a.scale2, lane, g == 1 && !all_visible, found);
     }
   }
 
