@@ -7,9 +7,9 @@
 //   M = max m,  out = sum 2^(m - M) o / sum 2^(m - M) l.
 //
 // The prefix is read once for the batch: the queries of all sequences that read one key head are the
-// rows of one product against it.  A sequence's own keys meet its own queries only.  A sequence that
-// appends 128 rows (tokens x heads of a key head) or more reads prefix and own keys in one pass, and so
-// does a call of few keys; these need no join.
+// rows of one product against it.  A sequence's own keys meet its own queries only.  A batch whose sequences
+// append about 128 rows (tokens x heads of a key head) or more each reads prefix and own keys in one pass,
+// and so does a call of few keys; these need no join.
 //
 // Matrix form (v_mfma_f32_32x32x16): S^T = K Q^T puts query l % 32 into lane l with 16 of a tile's
 // 32 keys, so that the softmax is per lane (one exchange with lane l ^ 32) and the weights, in two 16-bit
@@ -915,12 +915,25 @@ Shape shape_of(const FcvLmAttention& p) {
     return ceil_div(ceil_div(keys, std::max<int64_t>(want, 1)), unit) * unit;
   };
   s.own_many = seq_rows > kFewRows;
-  // A sequence with at least a tile of rows of its own reads the prefix with them: nothing is gained by
-  // stacking its rows with others'.
-  // Nor where all keys are few: one launch and no join (a token behind 512 + 100 keys 17 -> 13 us with
-  // the host's share; on the GPU alone even at about that many keys).
+  // A sequence with at least a tile of rows of its own may read the prompt with them, which saves the join.
+  // But each of a batch's sequences reads it then, in whole tiles: their tiles (at most a ragged one a
+  // sequence more than the stacked rows have) against the join's two parts.  A round of 512 tiles takes
+  // 3.9 us a 64 keys of 128 dims, 0.46 of that with one a CU or less.  64 requests of 32 / 8 heads, one of
+  // them with 512 new tokens and 63 with one: behind 8192 keys 667 us, stacked 184, behind 64 keys 85,
+  // stacked 89; 8 of them with 512 tokens: behind 8192 keys 1087, stacked 940, behind 512 keys 171, stacked
+  // 225; 16 of 33 tokens: behind 2048 keys 79, stacked 69, behind 512 keys 38, stacked 43.
+  // Nor is anything stacked where all keys are few: one launch and no join (a token behind 512 + 100 keys
+  // 17 -> 13 us with the host's share; on the GPU alone even at about that many keys).
+  const int64_t stacked_tiles = ceil_div(all_rows, kManyRows);
+  const int64_t fused_tiles =
+      std::min<int64_t>((int64_t)p.batch * ceil_div(seq_rows, kManyRows), stacked_tiles + p.batch);
+  const float per_round = 2.0f * kCus / (float)p.n_kv_heads;  // tiles of one key head
+  const float rounds = std::max((float)fused_tiles / per_round, 0.46f) - (float)stacked_tiles / per_round;
+  const float again_us =
+      rounds * (float)ceil_div(p.prefix_len, kManyKeys) * 3.9f * (float)p.head_dim / 128.0f;
+  const bool own_reads = seq_rows >= kManyRows && again_us <= 3.0f + 2.0f * (part_us - 0.1f);
   const bool short_keys = !s.own_many && p.prefix_len + (int64_t)max_length <= kShortKeys;
-  s.fused = p.prefix_len == 0 || seq_rows >= kManyRows || (p.batch == 1 && s.own_many) || short_keys;
+  s.fused = p.prefix_len == 0 || own_reads || (p.batch == 1 && s.own_many) || short_keys;
   if (!s.fused) {
     s.prefix_many = s.own_many || (int64_t)p.tokens * p.n_heads > kStackedFew;
     s.prefix_tiles = ceil_div(all_rows, s.prefix_many ? kManyRows : kFewRows);

@@ -277,7 +277,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      out: torch.Tensor | None = None, return_lse: bool = False):
     """Causal attention of a batch of sequences that share one prompt: every query of ``q``
     ``[T, heads, head dim]`` sees all of ``prefix_k``/``prefix_v`` ``[P, kv heads, head dim]`` and
-    its own sequence's cached keys up to itself; the prompt is read once for the whole batch.
+    its own sequence's cached keys up to itself.  The prompt is read for the rows of the whole batch
+    together, or by each sequence with its own keys where these are texts and that is faster.
 
     The caches are ``[sessions, capacity, kv heads, head dim]`` (64 or 128) at any strides;
     sequence ``b`` reads session ``slots[b]`` (``b`` without ``slots``), its ``lengths[b]`` keys
@@ -285,7 +286,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ``cu_q`` every sequence has ``T / len(lengths)``.  Rows past ``cu_q[-1]`` are not read, and
     their rows of ``out`` stay as they are (whatever the memory held, without ``out``).  ``max_q`` and
     ``max_length`` bound the queries and keys of a sequence and shape the launch (they default to
-    ``T`` and the capacity); batches that pass them are still computed.
+    what one sequence has if the others have a query each, and to the capacity); batches that pass
+    them are still computed.
     ``scale`` defaults to ``head dim ** -0.5``.  A query that sees no key gives zeros.  Returns
     the output, or with ``return_lse`` also the log sums of exponentials, fp32 ``[T, heads]``."""
     code = _dtype(q, "q")
@@ -307,7 +309,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                              "sequences")
         max_q = max(tokens // batch, 1)
     elif max_q is None:
-        max_q = max(tokens, 1)
+        max_q = max(tokens - batch + 1, 1)
     slot_ptr = 0 if slots is None else _indices(slots, "slots", batch, q)
     if slots is None and batch > sessions:
         raise ValueError(f"{batch} sequences need slots: the caches hold {sessions} sessions")
