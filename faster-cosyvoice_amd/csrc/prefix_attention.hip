@@ -42,7 +42,11 @@ constexpr int kFewRows = 32;    // queries of a row tile whose waves share the k
 constexpr int kFewKeys = 32;    // keys of a wave's tile there
 constexpr int kManyRows = 128;  // queries of a row tile whose waves share its queries out, 32 each
 constexpr int kManyKeys = 64;   // keys of a workgroup's tile there
-constexpr int kStackedFew = 4096;  // rows of all key heads up to which stacked rows are taken 32 at a time
+// Rows of all key heads times dims up to which stacked rows of few queries a sequence are taken 32 at a time.
+// Above, tiles of 128 need a launch of their own (us, 32 at a time / 128): 16384 rows of 128 dims behind 1024
+// keys 89 / 108, 4096 keys 127 / 134, 16384 keys 296 / 266; 32768 rows 164 / 167, 242 / 228, 580 / 500; 32768
+// rows of 64 dims behind 4096 keys 110 / 114, 65536 211 / 202.
+constexpr int64_t kStackedFew = 1 << 21;
 constexpr int kShortKeys = 768;    // prefix and own keys up to which tiles of 32 queries take them all at once
 constexpr int kMaxKeys = 1 << 29;  // of the prefix and of a session: their sum and a tile more fit 31 bits
 constexpr int kMaxParts = 64;      // lanes of the joining wave
@@ -935,7 +939,7 @@ Shape shape_of(const FcvLmAttention& p) {
   const bool short_keys = !s.own_many && p.prefix_len + (int64_t)max_length <= kShortKeys;
   s.fused = p.prefix_len == 0 || own_reads || (p.batch == 1 && s.own_many) || short_keys;
   if (!s.fused) {
-    s.prefix_many = s.own_many || (int64_t)p.tokens * p.n_heads > kStackedFew;
+    s.prefix_many = s.own_many || (int64_t)p.tokens * p.n_heads * p.head_dim > kStackedFew;
     s.prefix_tiles = ceil_div(all_rows, s.prefix_many ? kManyRows : kFewRows);
     s.prefix_step = cut(p.prefix_len, s.prefix_many ? kManyKeys : kWaves * kFewKeys, 0.6f,
                         (int64_t)s.prefix_tiles * p.n_kv_heads, 2 * kCus, 32);

@@ -33,11 +33,10 @@ def test_the_results_rounding_alone(fcv, news, lengths, prefix, hq, hk, dim, dty
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("batch", [63, 66])
-def test_a_large_batch_keeps_a_tokens_precision(fcv, batch, dtype):
-    """63 and 66 requests of 64 heads lie on both sides of 4096 stacked rows, where the prompt's tiles
-    change."""
-    say(f"[attn] rounding, {batch} tokens x 64 heads {dtype}")
+@pytest.mark.parametrize("batch,hq,hk,dim", [(66, 64, 8, 128), (129, 128, 8, 128), (65, 512, 16, 64)])
+def test_a_large_batch_keeps_a_tokens_precision(fcv, batch, hq, hk, dim, dtype):
+    """Stacked rows on both sides of 2^21 elements, where the prompt's tiles change."""
+    say(f"[attn] rounding, {batch} tokens x {hq} heads x {dim} {dtype}")
     lengths = [1 + 13 * i % 70 for i in range(batch)]
-    a = make([1] * batch, lengths, 900, 64, 8, 128, dtype)
+    a = make([1] * batch, lengths, 900, hq, hk, dim, dtype)
     check(fcv, a, "stacked", parts=2, max_q=1, max_length=max(lengths))
