@@ -61,6 +61,11 @@ struct Bf16 {
   }
 };
 
+// Whether 16-byte accesses fit a dimension of `count` entries; the stride of a single one says nothing.
+inline bool stride_fits(int64_t stride, int64_t count) {
+  return count <= 1 || (stride >= 0 && stride % 8 == 0);
+}
+
 inline bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
 constexpr int kCus = 256;  // compute units of the MI355X

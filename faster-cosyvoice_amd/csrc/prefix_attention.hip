@@ -985,20 +985,28 @@ int check(const FcvLmAttention* p) {
   FCV_CHECK(p->max_q >= 1 && p->max_length >= 0, FCV_ERR_INVALID, "need max_q >= 1 and max_length >= 0");
   FCV_CHECK(p->scale > 0.0f && p->scale < __builtin_inff(), FCV_ERR_INVALID,
             "scale must be positive and finite");
-  const int64_t strides[] = {p->q_row, p->q_head, p->out_row, p->out_head, p->pk_row, p->pk_head,
-                             p->pv_row, p->pv_head, p->k_session, p->k_row, p->k_head, p->v_session,
-                             p->v_row, p->v_head};
-  for (int64_t v : strides)
-    FCV_CHECK(v >= 0 && v % 8 == 0, FCV_ERR_INVALID, "strides must be multiples of 8 elements, >= 0");
-  FCV_CHECK(std::max({p->k_row, p->v_row, p->pk_row, p->pv_row}) < (1LL << 24), FCV_ERR_INVALID,
-            "a key's row stride must be below 2^24 elements");
+  const int64_t rows_of_keys[][2] = {{p->k_row, p->capacity}, {p->v_row, p->capacity},
+                                     {p->pk_row, p->prefix_len}, {p->pv_row, p->prefix_len}};
+  const int64_t others[][2] = {{p->q_row, p->tokens},        {p->q_head, p->n_heads},
+                               {p->out_row, p->tokens},      {p->out_head, p->n_heads},
+                               {p->pk_head, p->n_kv_heads},  {p->pv_head, p->n_kv_heads},
+                               {p->k_session, p->sessions},  {p->k_head, p->n_kv_heads},
+                               {p->v_session, p->sessions},  {p->v_head, p->n_kv_heads}};
+  for (const auto& v : rows_of_keys)
+    FCV_CHECK(stride_fits(v[0], v[1]), FCV_ERR_INVALID, "strides must be multiples of 8 elements, >= 0");
+  for (const auto& v : others)
+    FCV_CHECK(stride_fits(v[0], v[1]), FCV_ERR_INVALID, "strides must be multiples of 8 elements, >= 0");
+  for (const auto& v : rows_of_keys)
+    FCV_CHECK(v[1] <= 1 || v[0] < (1LL << 24), FCV_ERR_INVALID,
+              "a key's row stride must be below 2^24 elements");
   if (p->tokens == 0) return FCV_OK;
   FCV_CHECK(p->q && p->k_cache && p->v_cache && p->lengths && p->out, FCV_ERR_INVALID, "null argument");
   FCV_CHECK(p->prefix_len == 0 || (p->prefix_k && p->prefix_v), FCV_ERR_INVALID, "null prefix");
   FCV_CHECK(aligned(p->q, 16) && aligned(p->out, 16) && aligned(p->k_cache, 16) &&
                 aligned(p->v_cache, 16) && aligned(p->prefix_k, 16) && aligned(p->prefix_v, 16),
             FCV_ERR_INVALID, "q, out, the prefix and the caches must start on 16-byte boundaries");
-  FCV_CHECK((p->n_heads == 1 || p->out_head >= p->head_dim) && (p->tokens == 1 || p->out_row >= p->head_dim),
+  FCV_CHECK((p->n_heads == 1 || p->out_head >= p->head_dim) &&
+                (p->tokens == 1 || p->out_row >= p->head_dim),
             FCV_ERR_INVALID, "rows of out overlap");
   const Shape s = shape_of(*p);
   FCV_CHECK(s.prefix_blocks + s.own_blocks <= (1 << 23), FCV_ERR_INVALID,

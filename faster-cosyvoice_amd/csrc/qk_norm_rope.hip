@@ -179,13 +179,16 @@ int check(const FcvLmQkNormRope* p) {
                 aligned(p->q_weight, 16) && aligned(p->k_weight, 16),
             FCV_ERR_INVALID,
             "qkv, q_out, the caches, the tables and the weights must start on 16-byte boundaries");
-  FCV_CHECK((p->qkv_row | p->q_row | p->k_session | p->k_row | p->k_head | p->v_session | p->v_row |
-             p->v_head) % 8 == 0,
-            FCV_ERR_INVALID, "strides must be multiples of 8 elements");
-  FCV_CHECK(p->qkv_row >= 0 && p->q_row >= (int64_t)p->n_heads * p->head_dim &&
-                p->k_session >= 0 && p->k_row >= 0 && p->k_head >= 0 && p->v_session >= 0 &&
-                p->v_row >= 0 && p->v_head >= 0,
-            FCV_ERR_INVALID, "negative stride, or rows of q_out that overlap");
+  const int64_t strides[][2] = {{p->qkv_row, p->tokens},     {p->q_row, p->tokens},
+                                {p->k_session, p->sessions}, {p->k_row, p->capacity},
+                                {p->k_head, p->n_kv_heads},  {p->v_session, p->sessions},
+                                {p->v_row, p->capacity},     {p->v_head, p->n_kv_heads}};
+  for (const auto& v : strides) {
+    FCV_CHECK(v[1] <= 1 || v[0] >= 0, FCV_ERR_INVALID, "negative stride");
+    FCV_CHECK(stride_fits(v[0], v[1]), FCV_ERR_INVALID, "strides must be multiples of 8 elements");
+  }
+  FCV_CHECK(p->tokens == 1 || p->q_row >= (int64_t)p->n_heads * p->head_dim, FCV_ERR_INVALID,
+            "rows of q_out overlap");
   return FCV_OK;
 }
 

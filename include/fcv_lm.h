@@ -14,7 +14,8 @@
  * fcv_last_error()), no allocation.  The calls are stateless and asynchronous on `stream`, which
  * belongs to the current device; they may be captured into a hipGraph, and calls on different
  * streams need different workspaces.  fp16 and bf16 tensors, sums and softmax statistics in fp32.
- * Strides are in elements, and the innermost dimension is contiguous.  Results do not depend on
+ * Strides are in elements, and the innermost dimension is contiguous; what is said of strides is not
+ * asked of a dimension of one entry.  Results do not depend on
  * earlier calls or on timing; they may differ in the last bits between batch sizes, because the
  * order of a sum follows the sizes.
  */
