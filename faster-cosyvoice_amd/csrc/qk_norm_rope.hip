@@ -35,6 +35,18 @@ __device__ __forceinline__ void load8(const void* w, bool f32, int i, float (&ou
   }
 }
 
+// Sum of squares of a head, whose L lanes have 16 elements each.
+template <int L>
+__device__ __forceinline__ float squares(const float (&a)[8], const float (&b)[8]) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
+  ss += dpp_f<0xB1>(ss);                  // lanes 1 apart, then 2
+  ss += dpp_f<0x4E>(ss);
+  if constexpr (L == 8) ss += dpp_f<0x141>(ss);  // the other four of eight
+  return ss;
+}
+
 // heads_inv: 2^32 / heads, rounded up.
 template <class E, int D>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const FcvLmQkNormRope p, uint32_t total,
@@ -101,13 +113,19 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const FcvLmQkNor
     }
     const void* w = is_q ? p.q_weight : p.k_weight;
     if (w) {
-      float ss = 0.0f;
+      float mean = fmaf(squares<L>(a, b), 1.0f / D, p.eps);
+      if (mean > 0x1p100f || mean < 0x1p-60f) {
+        // The squares of bf16's largest values pass fp32 and those of its smallest vanish: x s has the norm
+        // of x where eps is eps s^2.  Seldom runs.
+        const float s = mean > 1.0f ? 0x1p-70f : 0x1p70f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
-      ss += dpp_f<0xB1>(ss);                  // lanes 1 apart, then 2
-      ss += dpp_f<0x4E>(ss);
-      if constexpr (L == 8) ss += dpp_f<0x141>(ss);  // the other four of eight
-      const float inv = 1.0f / sqrtf(fmaf(ss, 1.0f / D, p.eps));
+        for (int e = 0; e < 8; ++e) {
+          a[e] *= s;
+          b[e] *= s;
+        }
+        mean = fmaf(squares<L>(a, b), 1.0f / D, p.eps * s * s);
+      }
+      const float inv = 1.0f / sqrtf(mean);
       const bool wf = p.weight_dtype == FCV_LM_F32;
       float wa[8], wb[8];
       load8<E>(w, wf, c0 * 8, wa);
