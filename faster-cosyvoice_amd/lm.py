@@ -110,6 +110,34 @@ def _rows(t: torch.Tensor, name: str, width: int) -> tuple[int, int]:
     return n, ld if n > 1 else max(ld, width)
 
 
+def _extent(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to behind its last."""
+    return (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether the memory of two tensors may overlap.  Rows at one stride in one buffer whose columns
+    lie apart do not; other shapes that interleave are taken to."""
+    if t.numel() == 0 or out.numel() == 0:
+        return False
+    first, other = out.data_ptr(), t.data_ptr()
+    if other >= first + _extent(out) or other + _extent(t) <= first:
+        return False
+    steps = {x.stride(0) * x.element_size() for x in (out, t) if x.dim() > 1 and x.shape[0] > 1}
+    if len(steps) != 1 or 0 in steps:
+        return True
+    step = steps.pop()
+    widths = [_extent(x[0] if x.dim() > 1 else x) for x in (out, t)]
+    at = (other - first) % step
+    return at < widths[0] or at + widths[1] > step
+
+
+def _check_apart(out: torch.Tensor, **inputs: torch.Tensor | None) -> None:
+    for name, t in inputs.items():
+        if t is not None and _overlap(out, t):
+            raise ValueError(f"out overlaps {name}")
+
+
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                  activation: str | None = None, residual: torch.Tensor | None = None,
                  out: torch.Tensor | None = None,
@@ -138,7 +166,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if act is None:
         raise ValueError(f"unknown activation {activation!r}")
     shape = (m, n) if x.dim() == 2 else (*x.shape[:-1], n)
-    if out is None:
+    given = out is not None
+    if not given:
         if out_dtype is None or out_dtype == x.dtype:
             out_code = code
         elif out_dtype == torch.float32:
@@ -172,6 +201,9 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         res_ptr = residual.data_ptr()
     if m == 0:
         return out
+    if given:
+        in_place = res_ptr == out.data_ptr() and ldr == ldy and res_code == out_code
+        _check_apart(out, x=x, weight=weight, bias=bias, residual=None if in_place else residual)
     try:
         args = _LINEAR.pack(
             x.data_ptr(), weight.data_ptr(), bias_ptr, res_ptr, out.data_ptr(), ldx, ldw, ldr, ldy,
@@ -217,8 +249,10 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
     (a negative row or one past the end: nowhere).  ``cos``/``sin`` are fp32 tables
     ``[positions, rotated / 2]``; ``interleaved`` rotates pairs ``(2 i, 2 i + 1)``, otherwise
     ``(i, i + rotated / 2)``.  ``q_weight``/``k_weight`` ``[head dim]`` scale the norms; without
-    them heads are not normed.  Returns the queries ``[T, n_heads, head dim]``.  A prompt that a
-    batch shares is written with one session's caches (``prefix[None]``)."""
+    them heads are not normed.  Returns the queries ``[T, n_heads, head dim]``, in ``out`` if given,
+    which may be their own columns of ``qkv`` and overlaps nothing else.  The caches overlap neither
+    each other nor an input.  A prompt that a batch shares is written with one session's caches
+    (``prefix[None]``)."""
     code = _dtype(qkv, "qkv")
     (sessions, capacity, n_kv, dim), ks, vs = _caches(k_cache, v_cache, qkv)
     if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * dim or n_heads < 1:
@@ -247,7 +281,8 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
     if 0 in ks and any(n > 1 and st == 0 for n, st in zip(k_cache.shape, ks)) \
             or 0 in vs and any(n > 1 and st == 0 for n, st in zip(v_cache.shape, vs)):
         raise ValueError("k_cache or v_cache is expanded: its rows share memory")
-    if out is None:
+    given = out is not None
+    if not given:
         out = qkv.new_empty((tokens, n_heads, dim))
     elif out.dtype != qkv.dtype or out.device != qkv.device or out.shape != (tokens, n_heads, dim) \
             or out.stride(2) != 1 or (n_heads > 1 and out.stride(1) != dim):
@@ -255,6 +290,10 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
                          f"{qkv.device} whose heads are contiguous")
     if tokens == 0:
         return out
+    if given:
+        in_place = out.data_ptr() == qkv.data_ptr() and (tokens == 1 or out.stride(0) == qkv_row)
+        _check_apart(out, qkv=None if in_place else qkv, k_cache=k_cache, v_cache=v_cache, cos=cos,
+                     sin=sin, q_weight=q_weight, k_weight=k_weight)
     try:
         args = _QK_NORM_ROPE.pack(
             qkv.data_ptr(), pos_ptr, row_ptr, cos.data_ptr(), sin.data_ptr(),
@@ -288,8 +327,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ``max_length`` bound the queries and keys of a sequence and shape the launch (they default to
     what one sequence has if the others have a query each, and to the capacity); batches that pass
     them are still computed.
-    ``scale`` defaults to ``head dim ** -0.5``.  A query that sees no key gives zeros.  Returns
-    the output, or with ``return_lse`` also the log sums of exponentials, fp32 ``[T, heads]``."""
+    ``scale`` defaults to ``head dim ** -0.5``.  A query that sees no key gives zeros.  ``out`` may be
+    ``q`` itself and overlaps no other input.  Returns the output, or with ``return_lse`` also the log sums of exponentials, fp32 ``[T, heads]``."""
     code = _dtype(q, "q")
     (sessions, capacity, n_kv, dim), ks, vs = _caches(k_cache, v_cache, q)
     if q.dim() != 3 or q.shape[2] != dim or q.shape[1] % n_kv or q.shape[1] < 1:
@@ -328,7 +367,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         if prefix_len:
             pk_ptr, pv_ptr = prefix_k.data_ptr(), prefix_v.data_ptr()
             pk, pv = prefix_k.stride(), prefix_v.stride()
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.device != q.device or out.shape != q.shape \
             or out.stride(2) != 1:
@@ -342,6 +382,10 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if tokens == 0:
         return (out, lse) if return_lse else out
     qs, os = q.stride(), out.stride()
+    if given:
+        in_place = out.data_ptr() == q.data_ptr() and qs == os
+        _check_apart(out, q=None if in_place else q, k_cache=k_cache, v_cache=v_cache,
+                     prefix_k=prefix_k, prefix_v=prefix_v)
     try:
         args = _ATTENTION.pack(
             q.data_ptr(), pk_ptr, pv_ptr, k_cache.data_ptr(), v_cache.data_ptr(), cu_ptr, len_ptr,

@@ -84,7 +84,8 @@ int fcv_lm_linear(const FcvLmLinear* args, void* workspace, size_t workspace_byt
  * cache row is negative or past the caches writes no key and no value (a padded batch).  Of tokens
  * that name the same cache row any one's values may remain, elementwise.  A position outside the
  * tables reads their first or last row.  rope_dim is a multiple of 16 from 16 to head_dim; all
- * strides are multiples of 8 and all tensors start on 16-byte boundaries. */
+ * strides are multiples of 8 and all tensors start on 16-byte boundaries.  q_out may be the queries' own
+ * columns of qkv (same start and row stride); it and the caches overlap nothing else. */
 typedef struct FcvLmQkNormRope {
   const void* qkv;           /* [tokens][(n_heads + 2 n_kv_heads) head_dim], row stride qkv_row */
   const int32_t* positions;  /* [tokens] */
@@ -136,7 +137,7 @@ int fcv_lm_qk_norm_rope(const FcvLmQkNormRope* args, hipStream_t stream);
  * a batch that passes them is computed all the same, more slowly.
  * prefix_len and capacity are at most 2^29, tokens * n_heads is below 2^26; head_dim is 64 or 128;
  * strides are multiples of 8 and tensors start on 16-byte boundaries; a key's or value's row stride is
- * below 2^24. */
+ * below 2^24.  out may be q itself (same strides); it overlaps nothing else. */
 typedef struct FcvLmAttention {
   const void* q;          /* [tokens][n_heads][head_dim], strides q_row, q_head */
   const void* prefix_k;   /* [prefix_len][n_kv_heads][head_dim] */
