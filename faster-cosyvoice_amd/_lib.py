@@ -164,6 +164,7 @@ SIGNATURES = {
     # include/fcv_lm.h
     "fcv_lm_linear_workspace_bytes": (c_size_t, [POINTER(FcvLmLinear)]),
     "fcv_lm_linear": (c_int32, [POINTER(FcvLmLinear), c_void_p, c_size_t, c_void_p]),
+    "fcv_lm_linear_plan": (c_int32, [POINTER(FcvLmLinear), POINTER(c_int32), POINTER(c_int32)]),
     "fcv_lm_qk_norm_rope": (c_int32, [POINTER(FcvLmQkNormRope), c_void_p]),
     "fcv_lm_prefix_attention_workspace_bytes": (c_size_t, [POINTER(FcvLmAttention)]),
     "fcv_lm_prefix_attention": (c_int32, [POINTER(FcvLmAttention), c_void_p, c_size_t, c_void_p]),

@@ -686,9 +686,11 @@ int check(const FcvLmLinear* p) {
 //   rounds (slices slice_us + tile_us) + 3 us,   rounds = blocks over the CUs, `per_cu` each, rounded up,
 // and for a cut K a second launch that reads the ranges' sums.  slice_us and tile_us are fits to full
 // rounds of each shape at K 512, 2048 and 8192 (alone: one block a CU of those that share one).
-// 128x128 tiles have three stages while one a CU holds them all (88 against 115 us at 2048 x 8192 x
-// 2048) and two, two a CU, above (146 us for 4096 x 8192 x 2048).
-enum Form { kAny, kFew, kTile64, kTile64x128, kTile128, kTile128x256, kTile192x256, kTile256 };
+// 128x128 tiles have three stages (kTile128Deep) while one a CU holds them all (88 against 115 us at 2048 x
+// 8192 x 2048) and two, two a CU, above (146 us for 4096 x 8192 x 2048).
+enum Form {
+  kAny, kFew, kTile64, kTile64x128, kTile128, kTile128x256, kTile192x256, kTile256, kTile128Deep
+};
 
 struct Shape {
   Form form;
@@ -747,6 +749,7 @@ Plan plan_of(const FcvLmLinear& p) {
       consider(s.form, splits, 3.0f + rounds * (per * (alone ? s.alone_us : s.slice_us) + s.tile_us));
     }
   }
+  if (best.form == kTile128 && tiles_of(p, 128, 128) * best.splits <= kCus) best.form = kTile128Deep;
   return best;
 }
 
@@ -783,12 +786,8 @@ void launch(const FcvLmLinear& p, const Plan& plan, void* workspace, hipStream_t
       break;
     case kTile64: launch_tiles<E, Tile<64, 64, 2, 2, 4>>(a, stream); break;
     case kTile64x128: launch_tiles<E, Tile<64, 128, 2, 2, 3>>(a, stream); break;
-    case kTile128:
-      if (tiles_of(p, 128, 128) * a.splits <= kCus)
-        launch_tiles<E, Tile<128, 128, 2, 2, 3>>(a, stream);
-      else
-        launch_tiles<E, Tile<128, 128, 2, 2, 2>>(a, stream);
-      break;
+    case kTile128: launch_tiles<E, Tile<128, 128, 2, 2, 2>>(a, stream); break;
+    case kTile128Deep: launch_tiles<E, Tile<128, 128, 2, 2, 3>>(a, stream); break;
     case kTile128x256: launch_tiles<E, Tile<128, 256, 2, 4, 3>>(a, stream); break;
     case kTile192x256: launch_tiles<E, Tile<192, 256, 2, 4, 2>>(a, stream); break;
     case kTile256: launch_tiles<E, Tile<256, 256, 2, 4, 2>>(a, stream); break;
@@ -807,6 +806,15 @@ void launch(const FcvLmLinear& p, const Plan& plan, void* workspace, hipStream_t
 extern "C" size_t fcv_lm_linear_workspace_bytes(const FcvLmLinear* args) {
   if (fcv::lm::check(args) || args->m == 0) return 0;
   return fcv::lm::workspace_bytes(*args, fcv::lm::plan_of(*args));
+}
+
+extern "C" int fcv_lm_linear_plan(const FcvLmLinear* args, int32_t* form, int32_t* ranges) {
+  if (int rc = fcv::lm::check(args)) return rc;
+  FCV_CHECK(form && ranges, FCV_ERR_INVALID, "null argument");
+  const fcv::lm::Plan plan = fcv::lm::plan_of(*args);
+  *form = plan.form;
+  *ranges = plan.splits;
+  return FCV_OK;
 }
 
 extern "C" int fcv_lm_linear(const FcvLmLinear* args, void* workspace, size_t workspace_bytes,

@@ -73,6 +73,10 @@ typedef struct FcvLmLinear {
 size_t fcv_lm_linear_workspace_bytes(const FcvLmLinear* args);
 int fcv_lm_linear(const FcvLmLinear* args, void* workspace, size_t workspace_bytes,
                   hipStream_t stream);
+/* Which kernel a call takes and into how many ranges it cuts k, for logs and tests.  form: 0 any
+ * alignment, 1 up to 16 rows, else tiles of 2 64 x 64, 3 64 x 128, 4 128 x 128, 5 128 x 256, 6 192 x 256,
+ * 7 256 x 256, 8 128 x 128 in launches of few. */
+int fcv_lm_linear_plan(const FcvLmLinear* args, int32_t* form, int32_t* ranges);
 
 /* Token t's row of qkv holds n_heads query heads, n_kv_heads key heads and n_kv_heads value heads
  * of head_dim (64 or 128) elements.  Every query and key head x becomes
