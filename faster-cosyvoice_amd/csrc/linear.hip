@@ -14,7 +14,9 @@
 // (1.20 PFLOP/s; 61 % of the cycles at the clock the card holds under it, and the same within 10 % with
 // three to five slices of 32, with the copies asked for at once, and with four waves of 128 x 128); 9184 x
 // 1024 x 2048 with tanh-GELU 58 us, half of it rounds that are not full and stores that all CUs send at
-// once.  Small products by what a CU takes in (about 55 B/ns of copies): 32 x 4096 x 4096 12 us.
+// once (gemm.hip's 128 x 128 form takes 52 us for that one; of the shapes here 192 x 256 is the fastest, 128 x
+// 128 takes 70).  Small products by the latency of the few slices that one workgroup a CU has in flight, and
+// 32 rows are copied as 64: 32 x 4096 x 4096 12 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -446,7 +448,8 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
     constexpr int kPhases = S == 2 ? KS - 1 : KS;  // two stages: the copies need the last step's time to land
     constexpr int kPer = (C::kCopies + kPhases - 1) / kPhases;
     auto copies = [&](int phase) {
-      if (kt + S - 1 < KT) issue(kt + S - 1, stage == 0 ? S - 1 : stage - 1, phase * kPer, phase * kPer + kPer);
+      if (kt + S - 1 < KT)
+        issue(kt + S - 1, stage == 0 ? S - 1 : stage - 1, phase * kPer, phase * kPer + kPer);
     };
     auto head = [&](int st) {
 #pragma unroll

@@ -18,7 +18,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // Element types: bits <-> fp32 (to the nearest, ties to even) and D = A B + C on fragments.
 struct Half {
   typedef f16x2 T2;
-  static constexpr short kOne = 0x3C00;        // 1.0
   static constexpr short kInf = 0x7C00;        // +inf, and the exponent's mask
   // Softmax: a row's running maximum follows the true one when that is kLag (in powers of two) above
   // it, so that sums are rescaled seldom, and weights are held at 2^kShift times their size.  fp16:
@@ -41,7 +40,6 @@ struct Half {
 
 struct Bf16 {
   typedef __bf16 T2 __attribute__((ext_vector_type(2)));
-  static constexpr short kOne = 0x3F80;
   static constexpr short kInf = 0x7F80;
   // bf16 has fp32's range: sums of 2^16 of its largest values do not pass fp32's
   static constexpr float kShift = -24.0f, kLag = 8.0f;

@@ -18,15 +18,16 @@
 // Keys and values are copied straight into LDS.
 //
 // Bound and rate, 32 / 8 heads x 128 in bf16:
-//   64 queries behind a prompt of 8192 and 200 to 2000 own keys each: 95 to 105 us, 3.3 TB/s of the bytes
-//     that have to be read (the own keys alone 79 us, 3.75 TB/s; the prompt's product runs beside them);
-//   4 texts of 300 to 1024 tokens behind 4096 keys: 306 us, 0.71 PFLOP/s.  The vector pipe (32 exponentials
-//     and about 120 other instructions a wave and tile of 64 keys) and the matrix pipe (32 products) take
-//     their turns rather than overlap, and 77 % of the CU time is in blocks.  A tile's scores taken ahead
-//     beside the weights of the one before was slower (358 us: more registers, or half the tile), and so
-//     were fewer keys a barrier.  What cost most on the way were reloads of spilled registers: each waits
-//     for the copies in flight (522 to 308 us without).
-//   A token behind 512 + 100 keys: 9 us on the GPU.
+//   64 queries behind a prompt of 8192 and 200 to 2000 own keys each: 111 to 115 us, 3.0 TB/s of the bytes
+//     that have to be read (the own keys alone 90 us, 3.3 TB/s; the prompt alone 38 us: its blocks come first
+//     and leave little room beside them).
+//   4 texts of 300 to 1024 tokens behind 4096 keys: 397 to 406 us, 0.54 PFLOP/s.  The vector pipe (32
+//     exponentials and about 230 other instructions a wave and tile of 64 keys) and the matrix pipe (48
+//     products) take their turns rather than overlap: the matrix pipes are busy for 37 % of the cycles, CUs
+//     for 74 %, as the last round of tiles is not full.  A tile's scores taken ahead beside the weights of
+//     the one before was slower (more registers, or half the tile), and so were fewer keys a barrier.  What
+//     costs most are reloads of spilled registers in the key loops: each waits for the copies in flight.
+//   A token behind 512 + 100 keys: 10 us on the GPU.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -47,7 +48,7 @@ constexpr int kManyKeys = 64;   // keys of a workgroup's tile there
 // keys 89 / 108, 4096 keys 127 / 134, 16384 keys 296 / 266; 32768 rows 164 / 167, 242 / 228, 580 / 500; 32768
 // rows of 64 dims behind 4096 keys 110 / 114, 65536 211 / 202.
 constexpr int64_t kStackedFew = 1 << 21;
-constexpr int kShortKeys = 768;    // prefix and own keys up to which tiles of 32 queries take them all at once
+constexpr int kShortKeys = 768;  // prefix and own keys up to which tiles of 32 queries take them all at once
 constexpr int kMaxKeys = 1 << 29;  // of the prefix and of a session: their sum and a tile more fit 31 bits
 constexpr int kMaxParts = 64;      // lanes of the joining wave
 constexpr float kLog2e = 1.4426950408889634f;
@@ -76,7 +77,8 @@ struct Args {
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ const short* scalar(const short* p) {
   const uint64_t u = (uint64_t)p;
-  return (const short*)((uint64_t)(uint32_t)scalar((int)u) | (uint64_t)(uint32_t)scalar((int)(u >> 32)) << 32);
+  return (const short*)((uint64_t)(uint32_t)scalar((int)u) |
+                        (uint64_t)(uint32_t)scalar((int)(u >> 32)) << 32);
 }
 
 __device__ __forceinline__ float half_max(float v) {

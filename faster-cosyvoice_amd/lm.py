@@ -3,7 +3,8 @@
 cache append, and attention of a batch whose requests share one voice's prompt.
 
 The reference runs that model in an engine of its own (faster_cosyvoice/llm/engine.py:94-141);
-these are what a decoder layer beside Token2Wav needs:
+these are a decoder layer's products, rotation, cache append and attention.  Norms of whole rows and
+a gate's product with its branch are not among them:
 
     qkv = fused_linear(x, w_qkv, b_qkv)
     q = qk_norm_rope(qkv, positions, cos, sin, k_cache, v_cache, rows, n_heads=32)
@@ -328,7 +329,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     what one sequence has if the others have a query each, and to the capacity); batches that pass
     them are still computed.
     ``scale`` defaults to ``head dim ** -0.5``.  A query that sees no key gives zeros.  ``out`` may be
-    ``q`` itself and overlaps no other input.  Returns the output, or with ``return_lse`` also the log sums of exponentials, fp32 ``[T, heads]``."""
+    ``q`` itself and overlaps no other input.  Returns the output, or with ``return_lse`` also the
+    log sums of exponentials, fp32 ``[T, heads]``."""
     code = _dtype(q, "q")
     (sessions, capacity, n_kv, dim), ks, vs = _caches(k_cache, v_cache, q)
     if q.dim() != 3 or q.shape[2] != dim or q.shape[1] % n_kv or q.shape[1] < 1:

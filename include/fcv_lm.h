@@ -1,6 +1,7 @@
 /*
- * fcv_lm.h -- C ABI of the speech language model's operators in libfcvdit.so: what a decoder layer
- * of the model that writes the speech tokens runs beside Token2Wav.  The reference leaves that
+ * fcv_lm.h -- C ABI of the speech language model's operators in libfcvdit.so: a decoder layer's
+ * products, rotation, cache append and attention.  Norms of whole rows and a gate's product with its
+ * branch are not among them.  The reference leaves that
  * model to a separate engine process (faster_cosyvoice/llm/engine.py:94-141), so nothing here
  * mirrors one of its interfaces.
  *
@@ -15,8 +16,8 @@
  * belongs to the current device; they may be captured into a hipGraph, and calls on different
  * streams need different workspaces.  fp16 and bf16 tensors, sums and softmax statistics in fp32.
  * Strides are in elements, and the innermost dimension is contiguous; what is said of strides is not
- * asked of a dimension of one entry.  Results do not depend on
- * earlier calls or on timing; they may differ in the last bits between batch sizes, because the
+ * asked of a dimension of one entry.  Results do not depend on earlier calls or on timing (but for two
+ * tokens that name one cache row); they may differ in the last bits between batch sizes, because the
  * order of a sum follows the sizes.
  */
 #ifndef FCV_LM_H
@@ -133,8 +134,8 @@ int fcv_lm_qk_norm_rope(const FcvLmQkNormRope* args, hipStream_t stream);
  *   out = sum exp(s) v / sum exp(s),   lse = log sum exp(s).
  * A query that sees no key gives out = 0 and lse = -inf; keys and values that a query does not see
  * do not touch its result, whatever they hold.  Of the values that it sees an infinity is what it
- * gets, however small the weight, and NaN for NaN or both infinities.  Query head h reads key head h / (n_heads /
- * n_kv_heads).  Rows of q past cu_q[batch] are not read, and their rows of out and lse stay as they
+ * gets, however small the weight, and NaN for NaN or both infinities.  Query head h reads key head
+ * h / (n_heads / n_kv_heads).  Rows of q past cu_q[batch] are not read, and their rows of out and lse stay as they
  * were.  cu_q NULL: tokens / batch rows for every sequence; slots NULL: sequence b has session b.
  * lengths are clipped to [0, capacity], and a slot outside [0, sessions) has no keys.
  * max_q and max_length bound the new tokens and the keys of a sequence: they shape the launch, and
