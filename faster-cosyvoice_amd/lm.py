@@ -116,21 +116,41 @@ def _extent(t: torch.Tensor) -> int:
     return (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()
 
 
+def _pieces(t: torch.Tensor, at: int, step: int) -> list[tuple[int, int]]:
+    """The ranges of bytes that rows ``step`` apart of a tensor at byte ``at`` take in a period."""
+    row = t[0] if t.dim() > 1 else t
+    width, starts = _extent(row), [at % step]
+    if row.dim() == 2 and row.stride(0):  # heads
+        width, stride = _extent(row[0]), row.stride(0) * t.element_size()
+        starts = [(at + i * stride) % step for i in range(row.shape[0])]
+    if width >= step:
+        return [(0, step)]
+    ranges = [(first, min(first + width, step)) for first in starts]
+    ranges += [(0, first + width - step) for first in starts if first + width > step]
+    return sorted(ranges)
+
+
 def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
     """Whether the memory of two tensors may overlap.  Rows at one stride in one buffer whose columns
-    lie apart do not; other shapes that interleave are taken to."""
+    or heads lie apart do not; other shapes that interleave are taken to."""
     if t.numel() == 0 or out.numel() == 0:
         return False
     first, other = out.data_ptr(), t.data_ptr()
     if other >= first + _extent(out) or other + _extent(t) <= first:
         return False
     steps = {x.stride(0) * x.element_size() for x in (out, t) if x.dim() > 1 and x.shape[0] > 1}
-    if len(steps) != 1 or 0 in steps:
+    if len(steps) > 1 or 0 in steps:
         return True
-    step = steps.pop()
-    widths = [_extent(x[0] if x.dim() > 1 else x) for x in (out, t)]
-    at = (other - first) % step
-    return at < widths[0] or at + widths[1] > step
+    step = steps.pop() if steps else 1 << 62  # one row each: no period
+    ours, theirs = _pieces(out, 0, step), _pieces(t, other - first, step)
+    while ours and theirs:
+        if ours[-1][0] >= theirs[-1][1]:
+            ours.pop()
+        elif theirs[-1][0] >= ours[-1][1]:
+            theirs.pop()
+        else:
+            return True
+    return False
 
 
 def _check_apart(out: torch.Tensor, **inputs: torch.Tensor | None) -> None:
@@ -203,8 +223,9 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if m == 0:
         return out
     if given:
-        in_place = res_ptr == out.data_ptr() and ldr == ldy and res_code == out_code
-        _check_apart(out, x=x, weight=weight, bias=bias, residual=None if in_place else residual)
+        in_place = res_ptr == out.data_ptr() and (m == 1 or ldr == ldy) and res_code == out_code
+        _check_apart(out.view(-1, n), x=x.view(-1, k), weight=weight, bias=bias,
+                     residual=None if in_place or residual is None else residual.view(-1, n))
     try:
         args = _LINEAR.pack(
             x.data_ptr(), weight.data_ptr(), bias_ptr, res_ptr, out.data_ptr(), ldx, ldw, ldr, ldy,
@@ -385,7 +406,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         return (out, lse) if return_lse else out
     qs, os = q.stride(), out.stride()
     if given:
-        in_place = out.data_ptr() == q.data_ptr() and qs == os
+        in_place = out.data_ptr() == q.data_ptr() and (tokens == 1 or qs[0] == os[0]) \
+            and (heads == 1 or qs[1] == os[1])
         _check_apart(out, q=None if in_place else q, k_cache=k_cache, v_cache=v_cache,
                      prefix_k=prefix_k, prefix_v=prefix_v)
     try:

@@ -88,3 +88,37 @@ def test_both_infinities_meet_where_a_row_sees_both(fcv, n, dtype):
         a["v_cache"][slot, n + 18, 1, 3] = NAN
         got, _ = check(fcv, a, "both", max_q=n)
         assert (got[:n - 1, :3, 2] == INF).all() and got[n - 1, :3, 2].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("max_q", [1, 50])
+def test_in_tiles_taken_in_turn(fcv, max_q, dim, dtype):
+    """Sequences that pass the bound on their new tokens: a workgroup has several row tiles, each of
+    which looks for itself."""
+    say(f"[visible] several tiles, bound {max_q} x {dim} {dtype}")
+    a = make([300, 1, 90], [320, 9, 700], 70, 6, 2, dim, dtype)
+    slot = a["slots"].tolist()
+    for key in (5, 77, 150, 260, 319):
+        a["v_cache"][slot[0], key, 0, key % dim] = INF
+        a["v_cache"][slot[0], key, 1, key % 64] = NAN
+    a["v_cache"][slot[2], 650, 0, 1] = -INF
+    check(fcv, a, "several", max_q=max_q, max_length=700)
+    a["prefix_v"][69, 0, 2] = -INF
+    check(fcv, a, "and the prompt", max_q=max_q, max_length=60)
+
+
+@pytest.mark.parametrize("n", [1, 40, 200])
+def test_a_query_that_is_not_finite_stays_alone(fcv, n):
+    for dim in (64, 128):
+        a = make([n, 3], [n + 300, 70], 130, 6, 2, dim, torch.bfloat16)
+        want = fcv.prefix_attention(**a, max_q=n)
+        a["q"][0, 1, 3] = NAN
+        a["v_cache"][int(a["slots"][0]), 2, 0, 4] = INF
+        got = fcv.prefix_attention(**a, max_q=n)
+        assert got[0, 1].isnan().all()                     # the infinity does not stand over its NaN
+        rest = torch.ones_like(got, dtype=torch.bool)
+        rest[0, 1] = False
+        rest[:n, :3, 4] = False
+        assert torch.equal(got[rest], want[rest])
+        assert (got[1:n, :3, 4] == INF).all() and got[0, [0, 2], 4].tolist() == [INF, INF]

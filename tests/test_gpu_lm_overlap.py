@@ -74,3 +74,27 @@ def test_linear_refuses_what_overlaps(fcv):
     h[:, :64] = x
     want = fcv.fused_linear(x, w, b)
     assert torch.equal(fcv.fused_linear(h[:, :64], w, b, out=h[:, 64:]), want)
+
+
+def test_views_that_lie_apart_or_are_the_same(fcv):
+    x, w, b, r = linear.make(12, 64, 64, torch.bfloat16, bias=torch.bfloat16, residual=torch.bfloat16)
+    want = fcv.fused_linear(x, w, b, residual=r)
+    buf = torch.zeros(3, 4, 192, dtype=torch.bfloat16, device=DEV)   # leading dimensions
+    buf[..., :64], buf[..., 64:128] = x.view(3, 4, 64), r.view(3, 4, 64)
+    got = fcv.fused_linear(buf[..., :64], w, b, residual=buf[..., 64:128], out=buf[..., 128:])
+    assert torch.equal(got.reshape(12, 64), want)
+    got = fcv.fused_linear(buf[..., :64], w, b, residual=buf[..., 64:128], out=buf[..., 64:128])
+    assert torch.equal(got.reshape(12, 64), want)
+    wide = torch.zeros(2, 80, dtype=torch.bfloat16, device=DEV)      # one row, told at two strides
+    wide[0, :64] = r[0]
+    got = fcv.fused_linear(x[:1], w, b, residual=wide[:1, :64], out=wide[0][None, :64])
+    assert torch.equal(got[0], fcv.fused_linear(x[:1], w, b, residual=r[:1])[0])
+    a = attn.make([1], [20], 30, 6, 2, 64, torch.bfloat16)
+    want = fcv.prefix_attention(**a)
+    rows = torch.zeros(2, 8, 64, dtype=torch.bfloat16, device=DEV)
+    rows[0, :6] = a["q"][0]
+    got = fcv.prefix_attention(**dict(a, q=rows[:1, :6]), out=rows[0][None, :6])
+    assert torch.equal(got, want)
+    heads = torch.zeros(1, 6, 2, 64, dtype=torch.bfloat16, device=DEV)  # outputs between the queries
+    heads[:, :, 0] = a["q"]
+    assert torch.equal(fcv.prefix_attention(**dict(a, q=heads[:, :, 0]), out=heads[:, :, 1]), want)

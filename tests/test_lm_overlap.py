@@ -32,3 +32,13 @@ def test_together(overlap):
     assert overlap(buf[1:, :32], buf.view(-1)[63:63 + 64 * 9].view(9, 64)[:, :32])
     assert overlap(buf[:, :8], buf.view(20, 32)[:, 8:16])        # at other strides: taken to
     assert overlap(buf[:1].expand(10, 64), buf[0])
+
+
+def test_heads_between_heads(overlap):
+    buf = torch.zeros(5, 6, 3, 8)                                # tokens, heads, q k v, dim
+    q, k, v = buf[:, :, 0], buf[:, :, 1], buf[:, :, 2]
+    assert not overlap(q, k) and not overlap(k, q) and not overlap(v, q) and not overlap(q[2:3], k)
+    assert overlap(q, q[1:]) and overlap(q, q[:, 2:]) and overlap(v, v[3:4, 5:])
+    assert overlap(q, buf[:, :, 0, 4:]) and overlap(buf[1:, :, 0], buf.flatten(1)[:4, 40:])
+    last = buf.view(-1)[buf.stride(0) - 4:].as_strided((3, 8), (buf.stride(0), 1))  # past a row's end
+    assert overlap(q[1:], last) and overlap(last, q[1:]) and not overlap(last, k[1:])
