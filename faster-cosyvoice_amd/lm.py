@@ -21,6 +21,7 @@ looked at on the host (include/fcv_lm.h says what the kernels make of each).
 from __future__ import annotations
 
 import struct
+from operator import mul
 
 import torch
 
@@ -83,6 +84,10 @@ def _side(t: torch.Tensor, name: str, like: torch.Tensor, code: int) -> int:
     if t.dtype == torch.float32:
         return _F32
     raise ValueError(f"{name} must be {like.dtype} or float32, got {t.dtype}")
+
+
+def _size(code: int) -> int:
+    return 4 if code == _F32 else 2
 
 
 def _indices(t: torch.Tensor, name: str, n: int, like: torch.Tensor) -> int:
@@ -153,10 +158,15 @@ def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
     return False
 
 
-def _check_apart(out: torch.Tensor, **inputs: torch.Tensor | None) -> None:
-    for name, t in inputs.items():
-        if t is not None and _overlap(out, t):
-            raise ValueError(f"out overlaps {name}")
+def _check_apart(out: torch.Tensor, at: int, reach: int, inputs, rows: bool = False) -> None:
+    """Refuses an output over an input.  ``at`` and ``reach``: its address and the bytes from there to
+    behind its last element, as in each of ``inputs``, ``(name, tensor, at, reach)``: integers first,
+    since a small call takes a few microseconds.  ``rows``: tensors are rows of their last dimension."""
+    for name, t, first, length in inputs:
+        if first < at + reach and at < first + length:
+            ours, theirs = (v.view(-1, v.shape[-1]) if rows else v for v in (out, t))
+            if _overlap(ours, theirs):
+                raise ValueError(f"out overlaps {name}")
 
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -222,14 +232,20 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         res_ptr = residual.data_ptr()
     if m == 0:
         return out
+    x_ptr, w_ptr, out_ptr = x.data_ptr(), weight.data_ptr(), out.data_ptr()
     if given:
-        in_place = res_ptr == out.data_ptr() and (m == 1 or ldr == ldy) and res_code == out_code
-        _check_apart(out.view(-1, n), x=x.view(-1, k), weight=weight, bias=bias,
-                     residual=None if in_place or residual is None else residual.view(-1, n))
+        inputs = [("x", x, x_ptr, 2 * ((m - 1) * ldx + k)),
+                  ("weight", weight, w_ptr, 2 * ((n - 1) * ldw + k))]
+        if bias is not None:
+            inputs.append(("bias", bias, bias_ptr, _size(bias_code) * n))
+        if residual is not None and (res_ptr != out_ptr or (m > 1 and ldr != ldy)
+                                     or res_code != out_code):
+            inputs.append(("residual", residual, res_ptr, _size(res_code) * ((m - 1) * ldr + n)))
+        _check_apart(out, out_ptr, _size(out_code) * ((m - 1) * ldy + n), inputs, rows=True)
     try:
         args = _LINEAR.pack(
-            x.data_ptr(), weight.data_ptr(), bias_ptr, res_ptr, out.data_ptr(), ldx, ldw, ldr, ldy,
-            m, n, k, code, bias_code, res_code, out_code, act)
+            x_ptr, w_ptr, bias_ptr, res_ptr, out_ptr, ldx, ldw, ldr, ldy, m, n, k, code, bias_code,
+            res_code, out_code, act)
     except struct.error as e:
         raise _out_of_range(e) from e
     need = _entry("fcv_lm_linear_workspace_bytes", 0)(args)
@@ -312,16 +328,20 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, 
                          f"{qkv.device} whose heads are contiguous")
     if tokens == 0:
         return out
+    qkv_ptr, out_ptr = qkv.data_ptr(), out.data_ptr()
+    k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
     if given:
-        in_place = out.data_ptr() == qkv.data_ptr() and (tokens == 1 or out.stride(0) == qkv_row)
-        _check_apart(out, qkv=None if in_place else qkv, k_cache=k_cache, v_cache=v_cache, cos=cos,
-                     sin=sin, q_weight=q_weight, k_weight=k_weight)
+        size = (sessions - 1, capacity - 1, n_kv - 1)
+        inputs = [("k_cache", k_cache, k_ptr, 2 * (sum(map(mul, size, ks)) + dim)),
+                  ("v_cache", v_cache, v_ptr, 2 * (sum(map(mul, size, vs)) + dim))]
+        if out_ptr != qkv_ptr or (tokens > 1 and out.stride(0) != qkv_row):
+            inputs.append(("qkv", qkv, qkv_ptr, 2 * ((tokens - 1) * qkv_row + qkv.shape[1])))
+        _check_apart(out, out_ptr, 2 * ((tokens - 1) * out.stride(0) + n_heads * dim), inputs)
     try:
         args = _QK_NORM_ROPE.pack(
-            qkv.data_ptr(), pos_ptr, row_ptr, cos.data_ptr(), sin.data_ptr(),
+            qkv_ptr, pos_ptr, row_ptr, cos.data_ptr(), sin.data_ptr(),
             0 if q_weight is None else q_weight.data_ptr(),
-            0 if k_weight is None else k_weight.data_ptr(), out.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), qkv_row, out.stride(0) if tokens > 1 else n_heads * dim, *ks[:3],
+            0 if k_weight is None else k_weight.data_ptr(), out_ptr, k_ptr, v_ptr, qkv_row, out.stride(0) if tokens > 1 else n_heads * dim, *ks[:3],
             *vs[:3], tokens, n_heads, n_kv, dim, 2 * table[1], table[0], sessions, capacity, code,
             w_code, bool(interleaved), eps)
     except struct.error as e:
@@ -405,17 +425,25 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if tokens == 0:
         return (out, lse) if return_lse else out
     qs, os = q.stride(), out.stride()
+    q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+    k_ptr, v_ptr = k_cache.data_ptr(), v_cache.data_ptr()
     if given:
-        in_place = out.data_ptr() == q.data_ptr() and (tokens == 1 or qs[0] == os[0]) \
-            and (heads == 1 or qs[1] == os[1])
-        _check_apart(out, q=None if in_place else q, k_cache=k_cache, v_cache=v_cache,
-                     prefix_k=prefix_k, prefix_v=prefix_v)
+        size, rows = (sessions - 1, capacity - 1, n_kv - 1), (tokens - 1, heads - 1)
+        inputs = [("k_cache", k_cache, k_ptr, 2 * (sum(map(mul, size, ks)) + dim)),
+                  ("v_cache", v_cache, v_ptr, 2 * (sum(map(mul, size, vs)) + dim))]
+        if prefix_len:
+            keys = (prefix_len - 1, n_kv - 1)
+            inputs += [("prefix_k", prefix_k, pk_ptr, 2 * (sum(map(mul, keys, pk)) + dim)),
+                       ("prefix_v", prefix_v, pv_ptr, 2 * (sum(map(mul, keys, pv)) + dim))]
+        if out_ptr != q_ptr or any(n and a != b for n, a, b in zip(rows, qs, os)):
+            inputs.append(("q", q, q_ptr, 2 * (sum(map(mul, rows, qs)) + dim)))
+        _check_apart(out, out_ptr, 2 * (sum(map(mul, rows, os)) + dim), inputs)
     try:
         args = _ATTENTION.pack(
-            q.data_ptr(), pk_ptr, pv_ptr, k_cache.data_ptr(), v_cache.data_ptr(), cu_ptr, len_ptr,
-            slot_ptr, out.data_ptr(), 0 if lse is None else lse.data_ptr(), qs[0], qs[1], os[0], os[1],
-            pk[0], pk[1], pv[0], pv[1], *ks[:3], *vs[:3], tokens, batch, heads, n_kv, dim, prefix_len,
-            sessions, capacity, max_q, capacity if max_length is None else max_length, code,
+            q_ptr, pk_ptr, pv_ptr, k_ptr, v_ptr, cu_ptr, len_ptr, slot_ptr, out_ptr,
+            0 if lse is None else lse.data_ptr(), qs[0], qs[1], os[0], os[1], pk[0], pk[1], pv[0],
+            pv[1], *ks[:3], *vs[:3], tokens, batch, heads, n_kv, dim, prefix_len, sessions, capacity,
+            max_q, capacity if max_length is None else max_length, code,
             dim ** -0.5 if scale is None else scale)
     except struct.error as e:
         raise _out_of_range(e) from e
