@@ -10,10 +10,10 @@
 //   linear_few_kernel   up to 16 rows, W read once into registers;
 //   linear_any_kernel   more rows off 16-byte boundaries, or K no multiple of 8: through registers.
 //
-// Bound and rate: large products by the matrix pipes, 8192 x 4096 x 8192 bf16 with bias and SiLU 460 us
-// (1.20 PFLOP/s; 61 % of the cycles at the clock the card holds under it, and the same within 10 % with
-// three to five slices of 32, with the copies asked for at once, and with four waves of 128 x 128); 9184 x
-// 1024 x 2048 with tanh-GELU 58 us, half of it rounds that are not full and stores that all CUs send at
+// Bound and rate: large products by the matrix pipes, 8192 x 4096 x 8192 bf16 with bias and SiLU 446 to 490
+// us (1.1 to 1.2 PFLOP/s; 61 to 66 % of the cycles at the clock the card holds under it, and the same within
+// 10 % with three to five slices of 32, with the copies asked for at once, and with four waves of 128 x 128);
+// 9184 x 1024 x 2048 with tanh-GELU 60 us, half of it rounds that are not full and stores that all CUs send at
 // once (gemm.hip's 128 x 128 form takes 52 us for that one; of the shapes here 192 x 256 is the fastest, 128 x
 // 128 takes 70).  Small products by the latency of the few slices that one workgroup a CU has in flight, and
 // 32 rows are copied as 64: 32 x 4096 x 4096 12 us.
