@@ -15,6 +15,11 @@ Public surface (mirrors faster_cosyvoice.token2wav.flashinfer_dit / flashinfer_f
   HiFTVocoder             -- the HiFT vocoder (CausalHiFTGenerator counterpart), packed batches
   fused_linear, qk_norm_rope, prefix_attention
                           -- decoder-layer operators of the model that writes the speech tokens
+  quantize_fp4, fused_linear_fp4
+                          -- its linear layers over 4-bit weights
+  new_fp4_pages, qk_norm_rope_fp4, paged_attention_fp4, read_fp4_pages
+                          -- its key/value cache in pages of 4-bit numbers
+  copy_pages, CachePages  -- copies of a cache's pages, and the book of which session has which
 """
 
 from .estimator import DiTEstimator, rope_tables
@@ -24,11 +29,16 @@ from .streaming import CFMDecoder, StreamingFlow
 from .checkpoint import load_flow
 from .hift import HiFTVocoder
 from .lm import fused_linear, prefix_attention, qk_norm_rope
+from .lm_fp4 import (fused_linear_fp4, new_fp4_pages, paged_attention_fp4, qk_norm_rope_fp4,
+                     quantize_fp4, read_fp4_pages)
+from .pages import CachePages, copy_pages
 from . import synthetic
 
-__all__ = ["CFMDecoder", "DiTEstimator", "FlowFrontEnd", "HiFTVocoder", "StreamingFlow",
-           "apply_mi355x",
+__all__ = ["CFMDecoder", "CachePages", "DiTEstimator", "FlowFrontEnd", "HiFTVocoder", "StreamingFlow",
+           "apply_mi355x", "copy_pages",
            "euler_schedule",
-           "flow_inference_batched", "flow_inference_batched_streaming", "fused_linear", "load_flow",
-           "prefix_attention", "qk_norm_rope", "rope_tables",
+           "flow_inference_batched", "flow_inference_batched_streaming", "fused_linear",
+           "fused_linear_fp4", "load_flow", "new_fp4_pages", "paged_attention_fp4",
+           "prefix_attention", "qk_norm_rope", "qk_norm_rope_fp4", "quantize_fp4", "read_fp4_pages",
+           "rope_tables",
            "solve_euler_batched", "solve_euler_packed", "synthetic"]

@@ -1,5 +1,5 @@
-"""ctypes bindings of libfcvdit.so (declared in include/fcv_dit.h, fcv_flow.h, fcv_hift.h and
-fcv_lm.h).
+"""ctypes bindings of libfcvdit.so (declared in include/fcv_dit.h, fcv_flow.h, fcv_hift.h, fcv_lm.h
+and fcv_fp4.h).
 
 The library is the only compute path: if it is missing, importing the estimator raises,
 there is no fallback.  Error codes map to the exceptions the reference raises for the same
@@ -97,6 +97,44 @@ class FcvLmAttention(ctypes.Structure):
                 + [("scale", c_float)])
 
 
+class FcvFp4Quantize(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("w", "codes", "scales")]
+                + [(n, c_int64) for n in ("ldw", "ld_codes", "ld_scales")]
+                + [(n, c_int32) for n in ("n", "k", "dtype")])
+
+
+class FcvFp4Linear(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "codes", "scales", "bias", "residual", "y")]
+                + [(n, c_int64) for n in ("ldx", "ld_codes", "ld_scales", "ldr", "ldy")]
+                + [(n, c_int32) for n in ("m", "n", "k", "dtype", "bias_dtype", "residual_dtype",
+                                          "y_dtype", "activation")])
+
+
+class FcvFp4Append(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("qkv", "positions", "cache_rows", "rope_cos", "rope_sin",
+                                         "q_weight", "k_weight", "q_out", "pages")]
+                + [(n, c_int64) for n in ("qkv_row", "q_row", "page_stride", "head_stride")]
+                + [(n, c_int32) for n in ("tokens", "n_heads", "n_kv_heads", "head_dim", "rope_dim",
+                                          "max_pos", "n_pages", "dtype", "weight_dtype",
+                                          "interleaved")]
+                + [("eps", c_float)])
+
+
+class FcvFp4Read(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("pages", "rows", "k", "v")]
+                + [(n, c_int64) for n in ("page_stride", "head_stride", "k_row", "v_row")]
+                + [(n, c_int32) for n in ("tokens", "n_kv_heads", "head_dim", "n_pages", "dtype")])
+
+
+class FcvFp4Attention(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("q", "pages", "table", "lengths", "cu_q", "out", "lse")]
+                + [(n, c_int64) for n in ("q_row", "q_head", "out_row", "out_head", "page_stride",
+                                          "head_stride", "table_row")]
+                + [(n, c_int32) for n in ("tokens", "batch", "n_heads", "n_kv_heads", "head_dim",
+                                          "n_pages", "max_pages", "max_q", "max_length", "dtype")]
+                + [("scale", c_float)])
+
+
 # (name, restype, argtypes) of every exported entry point
 SIGNATURES = {
     "fcv_last_error": (ctypes.c_char_p, []),
@@ -168,6 +206,17 @@ SIGNATURES = {
     "fcv_lm_qk_norm_rope": (c_int32, [POINTER(FcvLmQkNormRope), c_void_p]),
     "fcv_lm_prefix_attention_workspace_bytes": (c_size_t, [POINTER(FcvLmAttention)]),
     "fcv_lm_prefix_attention": (c_int32, [POINTER(FcvLmAttention), c_void_p, c_size_t, c_void_p]),
+    # include/fcv_fp4.h
+    "fcv_fp4_quantize": (c_int32, [POINTER(FcvFp4Quantize), c_void_p]),
+    "fcv_fp4_linear_workspace_bytes": (c_size_t, [POINTER(FcvFp4Linear)]),
+    "fcv_fp4_linear": (c_int32, [POINTER(FcvFp4Linear), c_void_p, c_size_t, c_void_p]),
+    "fcv_fp4_page_bytes": (c_size_t, [c_int32]),
+    "fcv_fp4_append": (c_int32, [POINTER(FcvFp4Append), c_void_p]),
+    "fcv_fp4_read": (c_int32, [POINTER(FcvFp4Read), c_void_p]),
+    "fcv_fp4_attention_workspace_bytes": (c_size_t, [POINTER(FcvFp4Attention)]),
+    "fcv_fp4_attention": (c_int32, [POINTER(FcvFp4Attention), c_void_p, c_size_t, c_void_p]),
+    "fcv_copy_pages": (c_int32, [c_void_p, c_int32, c_int64, c_int32, c_int64, c_int64,
+                                 POINTER(c_int32), POINTER(c_int32), c_int32, c_void_p]),
 }
 
 STAGES = ("qkv", "attention", "out_proj", "ff1", "ff2", "ln_mod", "conv", "adaln", "in_proj",

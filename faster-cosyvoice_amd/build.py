@@ -21,7 +21,8 @@ ARCH = "gfx950"
 
 SOURCES = ["gemm.hip", "gemv.hip", "attention.hip", "conv.hip", "elementwise.hip", "frontend.hip",
            "hift.hip", "hift_split.hip", "hift_capi.hip", "linear.hip", "qk_norm_rope.hip",
-           "prefix_attention.hip", "capi.hip"]
+           "prefix_attention.hip", "linear_fp4.hip", "kv_fp4.hip", "attention_fp4.hip", "pages.hip",
+           "capi.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -52,7 +53,8 @@ def library_path() -> Path:
 # not in others, so an element's fp16 bits would depend on the GEMM tile shape, and with it on
 # the batch a document is packed with.
 EXACT_SOURCES = {"gemm.hip", "gemv.hip", "attention.hip", "conv.hip", "elementwise.hip", "capi.hip",
-                 "hift_split.hip", "linear.hip", "qk_norm_rope.hip", "prefix_attention.hip"}
+                 "hift_split.hip", "linear.hip", "qk_norm_rope.hip", "prefix_attention.hip",
+                 "linear_fp4.hip", "kv_fp4.hip", "attention_fp4.hip"}
 EXACT_FLAGS = ["-ffp-contract=off"]
 
 
