@@ -210,6 +210,7 @@ SIGNATURES = {
     "fcv_fp4_quantize": (c_int32, [POINTER(FcvFp4Quantize), c_void_p]),
     "fcv_fp4_linear_workspace_bytes": (c_size_t, [POINTER(FcvFp4Linear)]),
     "fcv_fp4_linear": (c_int32, [POINTER(FcvFp4Linear), c_void_p, c_size_t, c_void_p]),
+    "fcv_fp4_linear_plan": (c_int32, [POINTER(FcvFp4Linear), POINTER(c_int32), POINTER(c_int32)]),
     "fcv_fp4_page_bytes": (c_size_t, [c_int32]),
     "fcv_fp4_append": (c_int32, [POINTER(FcvFp4Append), c_void_p]),
     "fcv_fp4_read": (c_int32, [POINTER(FcvFp4Read), c_void_p]),

@@ -25,14 +25,14 @@ namespace {
 
 constexpr int kPage = FCV_FP4_PAGE;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// bf16's weights times values are held at 2^-24 times their size: sums of 2^24 of its largest values do not
-// pass fp32's.
+// bf16's values are held at 2^-24 times their size: sums of 2^24 of its largest values do not pass fp32's.
 template <class E>
 constexpr float kHeld = std::is_same<E, Bf16>::value ? 0x1p-24f : 1.0f;
 
 struct AttendArgs {
   FcvFp4Attention p;
   int group;                 // query heads of a key head
+  int each;                  // rows of every sequence without cu_q
   int row_tiles;             // tiles of 16 rows of a sequence's longest query range
   int splits, pages_per;     // ranges of keys, and the pages of one
   float* part;               // [splits][tokens][n_heads][D]
@@ -62,7 +62,9 @@ struct Raw {
   u32x4 vs;
 };
 
-template <class E, int D>
+// ROWS 8: the tile has 8 rows, each in two columns, so that one product takes the weights' first parts in
+// columns 0 .. 7 and their second parts in 8 .. 15.
+template <class E, int D, int ROWS>
 __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) {
   using P = Page<D>;
   constexpr int kWaves = 4, kU = D / 32, kJ = D / 32;  // value tiles; steps of 32 of the first product
@@ -71,30 +73,36 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
   const FcvFp4Attention& p = a.p;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15, blk = lane >> 4;
+  const uint32_t col = lane & 15, blk = lane >> 4;
   int b, first, n;  // the sequence, its first row of q, its queries
   const int kv = blockIdx.x % p.n_kv_heads, tile = blockIdx.x / p.n_kv_heads % a.row_tiles;
   b = blockIdx.x / p.n_kv_heads / a.row_tiles;
+  // What the whole workgroup asks for first, in one go.  Nothing writes it while the kernel runs: scalar loads.
+  typedef const int32_t __attribute__((address_space(4))) * Uniform;
+  const Uniform table = (Uniform)(uintptr_t)(p.table + (int64_t)b * p.table_row);
+  const Uniform ends = (Uniform)(uintptr_t)(p.cu_q ? p.cu_q + b : p.table);
+  const int page_first = blockIdx.y * a.pages_per + wave;
+  const int id_first = table[min(page_first, p.max_pages - 1)];
+  const int id_second = table[min(page_first + kWaves, p.max_pages - 1)];
+  const int keys = ((Uniform)(uintptr_t)p.lengths)[b], end0 = ends[0], end1 = ends[p.cu_q ? 1 : 0];
   if (p.cu_q) {
-    first = min(max(p.cu_q[b], 0), p.tokens);
-    n = min(max(p.cu_q[b + 1], first), p.tokens) - first;
+    first = min(max(end0, 0), p.tokens);
+    n = min(max(end1, first), p.tokens) - first;
   } else {
-    n = p.tokens / p.batch;
+    n = a.each;
     first = b * n;
   }
-  const int64_t rows = (int64_t)n * a.group;
-  const int length = min(max(p.lengths[b], 0), (int)min((int64_t)p.max_pages * kPage, (int64_t)0x7fffffff));
-  const int32_t* table = p.table + (int64_t)b * p.table_row;
+  const int rows = n * a.group;  // below 2^26
+  const int length = min(max(keys, 0), (int)min((int64_t)p.max_pages * kPage, (int64_t)0x7fffffff));
   const uint8_t* pool = p.pages + (int64_t)kv * p.head_stride;
 
   // a batch whose sequence has more rows than max_q said: the tiles take turns
-  for (int64_t row0 = (int64_t)tile * 16; row0 < rows; row0 += (int64_t)a.row_tiles * 16) {
-    const int64_t row = row0 + col;
-    const bool there = row < rows;
-    const int token = (int)(min(row, rows - 1) / a.group);
-    const int head = kv * a.group + (int)(min(row, rows - 1) % a.group);
+  for (int row0 = tile * ROWS; row0 < rows; row0 += a.row_tiles * ROWS) {
+    const bool there = row0 + (int)(col % ROWS) < rows;
+    const int row = min(row0 + (int)(col % ROWS), rows - 1);
+    const int token = row / a.group, head = kv * a.group + row - token * a.group;
     const int limit = there ? length - n + token + 1 : 0;  // the row's visible keys
-    const int last_token = (int)(min(row0 + 15, rows - 1) / a.group);
+    const int last_token = min(row0 + ROWS - 1, rows - 1) / a.group;
     const int reach = min(max(length - n + last_token + 1, 0), length);  // of the whole tile
     const int all_pages = (reach + kPage - 1) / kPage;
     int page0 = blockIdx.y * a.pages_per, page1 = min(page0 + a.pages_per, all_pages);
@@ -114,106 +122,157 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
       for (int h = 0; h < 2; ++h) o[u][h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -__builtin_inff(), l = 0.0f;
 
-    for (int page = page0 + wave; page < page1; page += kWaves) {
-      int id = table[page];
-      const bool good = id >= 0 && id < p.n_pages;
-      if (!good) continue;
-      const uint8_t* at = pool + (int64_t)id * p.page_stride;
-      Raw<D> r;
-      const int key0 = 16 * (col >> 2) + (col & 3);
+    Raw<D> r;
+    // 32-bit offsets from a page's address, which all lanes share
+    const uint32_t key0 = 16 * (col >> 2) + (col & 3);
+    const uint32_t at_k = key0 * P::kKey + blk * (D / 8);
+    const uint32_t at_ks = P::kScales + key0 * P::kKeyScales + (D == 128 ? blk : blk >> 1);
+    const uint32_t at_v = P::kValues + col * kPage + 16 * blk, at_vs = P::kValueScales + 16 * blk;
+    auto load_keys = [&](int id) {
+      const uint8_t* page = pool + (int64_t)id * p.page_stride;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int key = key0 + 4 * t;
         if constexpr (D == 128) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(at + key * P::kKey + blk * 16);
+          const u32x4 w = *reinterpret_cast<const u32x4*>(page + (at_k + 4 * t * P::kKey));
 #pragma unroll
           for (int j = 0; j < 4; ++j) r.k[t][j] = w[j];
         } else {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(at + key * P::kKey + blk * 8);
+          const u32x2 w = *reinterpret_cast<const u32x2*>(page + (at_k + 4 * t * P::kKey));
           r.k[t][0] = w[0];
           r.k[t][1] = w[1];
         }
-        r.ks[t] = at[P::kScales + key * P::kKeyScales + (D == 128 ? blk : blk >> 1)];
+        r.ks[t] = page[at_ks + 4 * t * P::kKeyScales];
       }
+    };
+    auto load_values = [&](int id) {
+      const uint8_t* page = pool + (int64_t)id * p.page_stride;
 #pragma unroll
       for (int u = 0; u < kU; ++u)
-        r.v[u] = *reinterpret_cast<const u32x4*>(at + P::kValues + (16 * u + col) * kPage + 16 * blk);
-      r.vs = *reinterpret_cast<const u32x4*>(at + P::kValueScales + 16 * blk);
-
-      f32x4 s[4];
+        r.v[u] = *reinterpret_cast<const u32x4*>(page + (at_v + 16 * u * kPage));
+      r.vs = *reinterpret_cast<const u32x4*>(page + at_vs);
+    };
+    // page `page`'s number, -1 where it has no keys
+    auto checked = [&](int page, int id) { return page < page1 && id < p.n_pages ? id : -1; };
+    auto number = [&](int page) { return checked(page, table[min(page, p.max_pages - 1)]); };
+    f32x4 s[4];
+    auto scores = [&](bool there) {
+      // a page that is not there: page 0's bytes with scales of 0, so that its scores are numbers
+      const uint32_t keep = there ? ~0u : 0u;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) r.ks[t] &= keep;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         const float ks = scale_of(r.ks[t]);
 #pragma unroll
         for (int j = 0; j < kJ; ++j) s[t] = E::mfma16(fp4_octet<E>(r.k[t][j], ks), fq[j], s[t]);
+        __builtin_amdgcn_sched_barrier(0);  // conversions of one tile at a time: registers
       }
-      const int seen = limit - page * kPage - 16 * blk;  // the lane's visible keys of its 16
+    };
+    // `masked`: some rows do not see all of the page's keys
+    auto weigh = [&](int page, bool there, auto masked) {
+      if constexpr (decltype(masked)::value) {  // hidden keys: no score, and a scale that is a number
+        const int seen = limit - page * kPage - 16 * (int)blk;  // the lane's visible keys of its 16
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[t][j] = 4 * t + j < seen ? s[t][j] : -__builtin_inff();
+          const int n = min(max(seen - 4 * t, 0), 4);
+          r.vs[t] &= n == 4 ? ~0u : (1u << (8 * n)) - 1;
+        }
+      }
       float top = -__builtin_inff();
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[t][j] = 4 * t + j < seen ? s[t][j] * scale : -__builtin_inff();
-          top = fmaxf(top, s[t][j]);
-        }
-      top = across_max(top);
-      const float next = fmaxf(m, top);
-      const float base = next == -__builtin_inff() ? 0.0f : next;
-      const float alpha = hw_exp2(m - base);  // 0 before the first visible key
-      m = next;
-      l *= alpha;
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, s[t][j]);
+      top = there ? across_max(top) * scale : -__builtin_inff();
+      if (__any(top > m)) {  // seldom, once a few pages have passed
+        const float next = fmaxf(m, top);
+        const float alpha = next == -__builtin_inff() ? 1.0f : hw_exp2(m - next);
+        m = next;
+        l *= alpha;
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        o[u][0] *= alpha;
-        o[u][1] *= alpha;
-      }
-      uint32_t hi[2][4], lo[2][4];  // the weights of keys 8 s .. 8 s + 7 of the lane's 16
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        float w[4], rest[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool vis = 4 * t + j < seen;
-          const float e = vis ? hw_exp2(s[t][j] - base) : 0.0f;
-          l += e;
-          w[j] = vis ? e * kHeld<E> * scale_of((r.vs[t] >> (8 * j)) & 255) : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-          const uint32_t u = bf16_pair(w[j], w[j + 1]);
-          rest[j] = w[j] - __uint_as_float(u << 16);
-          rest[j + 1] = w[j + 1] - __uint_as_float(u & 0xffff0000u);
-          hi[t >> 1][(t & 1) * 2 + j / 2] = u;
-          lo[t >> 1][(t & 1) * 2 + j / 2] = bf16_pair(rest[j], rest[j + 1]);
+        for (int u = 0; u < kU; ++u) {
+          o[u][0] *= alpha;
+          o[u][1] *= alpha;
         }
       }
+      const float base = there ? (m == -__builtin_inff() ? 0.0f : m) : __builtin_inff();
+      const uint32_t keep = there ? ~0u : 0u;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) r.vs[t] &= keep;
+      uint32_t hi[2][4], lo[2][4];  // the weights of keys 8 st .. + 7 of the lane's 16, in pairs i and i + 4
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float w[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float e = hw_exp2(fmaf(s[2 * st + i][j], scale, -base));
+            l += e;
+            w[i] = e * scale_of((r.vs[2 * st + i] >> (8 * j)) & 255);
+          }
+          const uint32_t u = bf16_pair(w[0], w[1]);
+          const uint32_t v =
+              bf16_pair(w[0] - __uint_as_float(u << 16), w[1] - __uint_as_float(u & 0xffff0000u));
+          hi[st][j] = ROWS == 8 && col >= 8 ? v : u;
+          lo[st][j] = v;
+        }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         const s16x8 ph = __builtin_bit_cast(s16x8, u32x4{hi[st][0], hi[st][1], hi[st][2], hi[st][3]});
         const s16x8 pl = __builtin_bit_cast(s16x8, u32x4{lo[st][0], lo[st][1], lo[st][2], lo[st][3]});
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-          u32x4 even, odd;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t w = r.v[u][2 * st + i];
-            const uint32_t x0 = fp4_pair<Bf16, 0>(w, 1.0f), x1 = fp4_pair<Bf16, 1>(w, 1.0f);
-            const uint32_t x2 = fp4_pair<Bf16, 2>(w, 1.0f), x3 = fp4_pair<Bf16, 3>(w, 1.0f);
-            even[2 * i] = __builtin_amdgcn_perm(x1, x0, 0x05040100);
-            even[2 * i + 1] = __builtin_amdgcn_perm(x3, x2, 0x05040100);
-            odd[2 * i] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
-            odd[2 * i + 1] = __builtin_amdgcn_perm(x3, x2, 0x07060302);
-          }
-          const s16x8 ve = __builtin_bit_cast(s16x8, even), vo = __builtin_bit_cast(s16x8, odd);
+          // codes of one element of keys i and i + 4 side by side, as one byte
+          const uint32_t w0 = r.v[u][2 * st], w1 = r.v[u][2 * st + 1];
+          const uint32_t we = (w0 & 0x0f0f0f0fu) | (w1 << 4 & 0xf0f0f0f0u);
+          const uint32_t wo = (w0 >> 4 & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
+          const s16x8 ve = fp4_octet<Bf16>(we, kHeld<E>), vo = fp4_octet<Bf16>(wo, kHeld<E>);
           o[u][0] = Bf16::mfma16(ve, ph, o[u][0]);
           o[u][1] = Bf16::mfma16(vo, ph, o[u][1]);
-          o[u][0] = Bf16::mfma16(ve, pl, o[u][0]);
-          o[u][1] = Bf16::mfma16(vo, pl, o[u][1]);
+          if constexpr (ROWS == 16) {
+            o[u][0] = Bf16::mfma16(ve, pl, o[u][0]);
+            o[u][1] = Bf16::mfma16(vo, pl, o[u][1]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
+    };
+    // The next page's keys are asked for once this one's are used up, its values likewise (page 0's where there
+    // is none: without a branch around the loads the waits for them are exact).
+    if (page0 + wave < page1) {
+      int id = checked(page_first, id_first), next = checked(page_first + kWaves, id_second);
+      load_keys(max(id, 0));
+      load_values(max(id, 0));
+      // pages that the tile's first row, and with it every other, sees all of; then the others
+      const int full = min(page1, max(length - n + row0 / a.group + 1, 0) / kPage);
+      int page = page0 + wave;
+      auto step = [&](auto masked) {
+        const int after = number(page + 2 * kWaves);
+        scores(id >= 0);
+        load_keys(max(next, 0));
+        weigh(page, id >= 0, masked);
+        load_values(max(next, 0));
+        id = next;
+        next = after;
+        page += kWaves;
+      };
+      const bool all_there = row0 + ROWS <= rows;
+      while (all_there && page < full) step(std::false_type{});
+      while (page < page1) step(std::true_type{});
     }
 
+    if constexpr (ROWS == 8) {  // the two parts' columns
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[u][h][j] += dpp_f<0x128>(o[u][h][j]);  // rotated by 8 in rows of 16
+    }
     // the waves' sums, in their order
     l = across_sum(l);
     if (blk == 0) {
@@ -253,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
           r[u][1] += *reinterpret_cast<const f32x4*>(from + 4) * f;
         }
       }
-      if (there) {
+      if (there && col < ROWS) {
         const int64_t at = (int64_t)(first + token) * p.n_heads + head;
         if (a.splits > 1) {
           const int64_t i = (int64_t)blockIdx.y * p.tokens * p.n_heads + at;
@@ -287,34 +346,65 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
   }
 }
 
-// The ranges' sums, in their order.  A thread has 8 elements of a row's head.
+// The ranges' sums.  A workgroup has one row's head: a thread 4 elements of every kGroups-th range, in their
+// order, and the groups are summed in theirs.
 template <class E, int D>
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ __attribute__((aligned(16))) float so[kGroups][D];
+  __shared__ float sm[kGroups], sl[kGroups];
   const FcvFp4Attention& p = a.p;
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / (D / 8);
-  const int d = threadIdx.x % (D / 8) * 8;
-  const int64_t n = (int64_t)p.tokens * p.n_heads;
-  if (i >= n) return;
-  const int token = (int)(i / p.n_heads), head = (int)(i % p.n_heads);
+  const int token = blockIdx.x / p.n_heads, head = blockIdx.x - token * p.n_heads;
   if (p.cu_q && token >= p.cu_q[p.batch]) return;  // behind the last sequence
-  float top = -__builtin_inff();
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * n + i)]);
-  const float base = top == -__builtin_inff() ? 0.0f : top;
-  float l = 0.0f;
-  f32x4 r0 = {0.0f, 0.0f, 0.0f, 0.0f}, r1 = r0;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = hw_exp2(a.part_ml[2 * (s * n + i)] - base);
-    l += a.part_ml[2 * (s * n + i) + 1] * f;
-    const float* from = a.part + (s * n + i) * D + d;
-    r0 += *reinterpret_cast<const f32x4*>(from) * f;
-    r1 += *reinterpret_cast<const f32x4*>(from + 4) * f;
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / (l * kHeld<E>);
-  s16x8 v;
+  const int64_t i = blockIdx.x, n = (int64_t)p.tokens * p.n_heads;
+  const int g = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+  float m = -__builtin_inff(), l = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = g; s0 < a.splits; s0 += 2 * kGroups) {  // two asked for at once
+    float pm[2], pl[2];
+    f32x4 po[2];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = E::from_f32((e < 4 ? r0[e % 4] : r1[e % 4]) * inv);
-  *reinterpret_cast<s16x8*>(static_cast<short*>(p.out) + (int64_t)token * p.out_row +
-                            (int64_t)head * p.out_head + d) = v;
+    for (int k = 0; k < 2; ++k) {
+      const int s = s0 + k * kGroups;
+      const int64_t at = (s < a.splits ? s : s0) * n + i;
+      pm[k] = s < a.splits ? a.part_ml[2 * at] : -__builtin_inff();
+      pl[k] = a.part_ml[2 * at + 1];
+      po[k] = *reinterpret_cast<const f32x4*>(a.part + at * D + d);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (pm[k] == -__builtin_inff() && pl[k] == 0.0f) continue;  // a range without keys, or none
+      if (s0 + k * kGroups >= a.splits) continue;
+      const float next = fmaxf(m, pm[k]), base = next == -__builtin_inff() ? 0.0f : next;
+      const float f0 = hw_exp2(m - base), f1 = hw_exp2(pm[k] - base);
+      m = next;
+      l = l * f0 + pl[k] * f1;
+      o = o * f0 + po[k] * f1;
+    }
+  }
+  *reinterpret_cast<f32x4*>(&so[g][d]) = o;
+  if (d == 0) {
+    sm[g] = m;
+    sl[g] = l;
+  }
+  __syncthreads();
+  if (g > 0) return;
+  float top = m;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) top = fmaxf(top, sm[k]);
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+  l = 0.0f;
+  o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) {
+    const float f = hw_exp2(sm[k] - base);
+    l += sl[k] * f;
+    o += *reinterpret_cast<const f32x4*>(&so[k][d]) * f;
+  }
+  o *= l == 0.0f ? 0.0f : 1.0f / (l * kHeld<E>);
+  *reinterpret_cast<s16x4*>(static_cast<short*>(p.out) + (int64_t)token * p.out_row +
+                            (int64_t)head * p.out_head + d) =
+      s16x4{E::from_f32(o[0]), E::from_f32(o[1]), E::from_f32(o[2]), E::from_f32(o[3])};
   if (p.lse && d == 0) p.lse[i] = (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
@@ -328,8 +418,8 @@ int check(const FcvFp4Attention* p) {
   FCV_CHECK(p->tokens >= 0 && p->batch >= 1 && p->n_heads >= 1 && p->n_kv_heads >= 1 &&
                 p->n_heads % p->n_kv_heads == 0,
             FCV_ERR_INVALID, "need tokens >= 0, batch >= 1 and query heads a multiple of the key heads");
-  FCV_CHECK((int64_t)p->tokens * p->n_heads < (1LL << 26), FCV_ERR_INVALID,
-            "too many rows: tokens * n_heads must stay below 2^26");
+  FCV_CHECK((int64_t)p->tokens * p->n_heads < (1LL << 24), FCV_ERR_INVALID,
+            "too many rows: tokens * n_heads must stay below 2^24");
   FCV_CHECK(p->cu_q || p->tokens % p->batch == 0, FCV_ERR_INVALID,
             "without cu_q the rows must divide by the sequences");
   FCV_CHECK(p->n_pages >= 1 && p->n_pages <= (1 << 24), FCV_ERR_INVALID,
@@ -354,21 +444,28 @@ int check(const FcvFp4Attention* p) {
 }
 
 struct Plan {
+  int rows;  // of a tile
   int64_t row_tiles;
   int splits, pages_per;
 };
 
 Plan plan_of(const FcvFp4Attention& p) {
   const int group = p.n_heads / p.n_kv_heads;
-  const int64_t all = std::max<int64_t>(((int64_t)std::min(p.max_q, p.tokens) * group + 15) / 16, 1);
+  const int64_t most_rows = (int64_t)std::min(p.max_q, p.tokens) * group;
+  const int rows = most_rows <= 8 ? 8 : 16;
+  const int64_t all = std::max<int64_t>((most_rows + rows - 1) / rows, 1);
   // tiles past a launch's size take turns
   const int64_t tiles = std::min(all, std::max<int64_t>(1, (1 << 22) / ((int64_t)p.batch * p.n_kv_heads)));
   const int64_t blocks = tiles * p.batch * p.n_kv_heads;
   const int64_t most = (int64_t)p.max_pages * kPage;
   const int pages = (int)std::max<int64_t>((std::min<int64_t>(p.max_length, most) + kPage - 1) / kPage, 1);
-  const int64_t want = std::max<int64_t>(1, 4 * kCus / blocks);
+  // Ranges of pages: two workgroups a CU; a workgroup's beginning and end cost about 5 us.  32 heads of 128 over
+  // 8, 64 sequences of 1000 to 8000 keys (512 workgroups): one, two, three and four ranges take 83, 90, 87 and
+  // 92 us; 14 over 2 of 64, 64 of 500 to 4000: one, two, four and eight 20, 16, 15.5 and 16.5; one of 7000 keys
+  // in ranges of 4, 8 and 16 pages 8.2, 8.8 and 10.6.
+  const int64_t want = std::max<int64_t>(1, 2 * kCus / blocks);
   const int per = (int)std::max<int64_t>((pages + want - 1) / want, 4);
-  return Plan{tiles, (pages + per - 1) / per, per};
+  return Plan{rows, tiles, (pages + per - 1) / per, per};
 }
 
 size_t workspace_bytes(const FcvFp4Attention& p, const Plan& plan) {
@@ -376,13 +473,15 @@ size_t workspace_bytes(const FcvFp4Attention& p, const Plan& plan) {
 }
 
 template <class E, int D>
-void launch(const AttendArgs& a, hipStream_t stream) {
+void launch(const AttendArgs& a, int rows, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.row_tiles * a.p.batch * a.p.n_kv_heads), (unsigned)a.splits);
-  hipLaunchKernelGGL((attend_fp4_kernel<E, D>), grid, dim3(256), 0, stream, a);
+  if (rows == 8)
+    hipLaunchKernelGGL((attend_fp4_kernel<E, D, 8>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attend_fp4_kernel<E, D, 16>), grid, dim3(256), 0, stream, a);
   if (a.splits > 1) {
-    const int64_t threads = (int64_t)a.p.tokens * a.p.n_heads * (D / 8);
-    hipLaunchKernelGGL((attend_join_kernel<E, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0,
-                       stream, a);
+    hipLaunchKernelGGL((attend_join_kernel<E, D>), dim3((unsigned)(a.p.tokens * a.p.n_heads)), dim3(256),
+                       0, stream, a);
   }
 }
 
@@ -409,14 +508,15 @@ extern "C" int fcv_fp4_attention(const FcvFp4Attention* args, void* workspace, s
   FCV_CHECK((int64_t)args->batch * args->n_kv_heads <= (1 << 23), FCV_ERR_INVALID,
             "batch * n_kv_heads is limited to 2^23");
   float* part = static_cast<float*>(workspace);
-  const AttendArgs a{*args, args->n_heads / args->n_kv_heads, (int)plan.row_tiles, plan.splits,
+  const AttendArgs a{*args, args->n_heads / args->n_kv_heads, args->tokens / args->batch,
+                     (int)plan.row_tiles, plan.splits,
                      plan.pages_per, part,
                      part ? part + (size_t)plan.splits * args->tokens * args->n_heads * args->head_dim
                           : nullptr};
   if (args->dtype == FCV_LM_F16)
-    args->head_dim == 64 ? launch<Half, 64>(a, stream) : launch<Half, 128>(a, stream);
+    args->head_dim == 64 ? launch<Half, 64>(a, plan.rows, stream) : launch<Half, 128>(a, plan.rows, stream);
   else
-    args->head_dim == 64 ? launch<Bf16, 64>(a, stream) : launch<Bf16, 128>(a, stream);
+    args->head_dim == 64 ? launch<Bf16, 64>(a, plan.rows, stream) : launch<Bf16, 128>(a, plan.rows, stream);
   FCV_HIP(hipGetLastError());
   return FCV_OK;
 }

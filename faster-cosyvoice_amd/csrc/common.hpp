@@ -123,6 +123,13 @@ __device__ __forceinline__ void lds_dma16_at(const void* addr, uint32_t lds) {
                : "s"(lds), "v"(addr)
                : "memory", "m0");
 }
+// 4 bytes a lane: lane l's to bytes [4 l, 4 l + 4) from `lds`.
+__device__ __forceinline__ void lds_dma4(const void* base, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(lds), "v"(voff), "s"(base)
+               : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 }  // namespace fcv

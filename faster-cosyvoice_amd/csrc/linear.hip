@@ -296,7 +296,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_tile_ker
     mma(1);
   }
 
-  store_tile<E, C, (int)sizeof(smem)>(a, acc, smem, m0, n0, wm0, wn0, split);
+  store_tile<E, C, (int)sizeof(smem)>(a, acc, smem, split, n0, wn0, wm0, m0);
 }
 
 // ---- up to 16 rows: the weights straight into registers -------------------------------------------

@@ -164,7 +164,7 @@ struct Tile {
 // LDS position of 16-byte chunk c of row r: 16 rows read at one chunk index touch all banks.
 template <int BK>
 __device__ __forceinline__ int swz(int r, int c) {
-  return BK == 64 ? c ^ ((r >> 1) & 7) : c ^ ((r >> 2) & 3);
+  return BK == 128 ? c ^ (r & 15) : BK == 64 ? c ^ ((r >> 1) & 7) : c ^ ((r >> 2) & 3);
 }
 
 template <int N>
@@ -192,10 +192,10 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 // The epilogue of a tile kernel whose waves have TM x TN blocks of 32 x 32 outputs each in `acc`: waves at
-// (wm0, wn0) of the tile at (m0, n0), `smem` the workgroup's LDS (its `lds` bytes are free).
+// (wm0, wn0) of the tile at row m0 and column n0, `smem` the workgroup's LDS (its kLds bytes are free).
 template <class E, class C, int kLds>
 __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[C::TM][C::TN], short* smem,
-                                           int m0, int n0, int wm0, int wn0, int split) {
+                                           int split, int n0, int wn0, int wm0, int m0) {
   constexpr int TM = C::TM, TN = C::TN;
   const FcvLmLinear& p = a.p;
   const int lane = threadIdx.x & 63;

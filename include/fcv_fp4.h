@@ -55,7 +55,7 @@ int fcv_fp4_quantize(const FcvFp4Quantize* args, hipStream_t stream);
 /* y[i][j] = act(sum_k x[i][k] w[j][k] + bias[j]) + residual[i][j] as fcv_lm_linear computes it, where
  * w[j][k] is code k of row j times the scale of its group of 32, rounded to x's type (exact within the
  * limits above).  Codes past k are not looked at.  m and n up to 2^22, their product up to 2^34, k up
- * to 2^26. */
+ * to 2^21, ld_codes and ld_scales below 2^24. */
 typedef struct FcvFp4Linear {
   const void* x;         /* [m][k], row stride ldx */
   const uint8_t* codes;  /* [n][16 ceil(k / 32)], row stride ld_codes */
@@ -82,6 +82,9 @@ typedef struct FcvFp4Linear {
 size_t fcv_fp4_linear_workspace_bytes(const FcvFp4Linear* args);
 int fcv_fp4_linear(const FcvFp4Linear* args, void* workspace, size_t workspace_bytes,
                    hipStream_t stream);
+/* Which kernel a call takes and into how many ranges it cuts k, for logs and tests.  form: 0 up to 32 rows,
+ * else tiles of 1 64 x 64, 2 64 x 128, 3 128 x 128, 4 128 x 256, 5 256 x 256. */
+int fcv_fp4_linear_plan(const FcvFp4Linear* args, int32_t* form, int32_t* ranges);
 
 /* Pages: a pool [pages][n_kv_heads][page bytes], strides page_stride and head_stride in bytes,
  * multiples of 16 and on 16-byte boundaries.  A page holds 64 tokens; per head, with D = head_dim,
@@ -155,7 +158,7 @@ int fcv_fp4_read(const FcvFp4Read* args, hipStream_t stream);
  * cu_q[batch] are not read, and their rows of out and lse stay as they were.  cu_q NULL: tokens / batch
  * rows for every sequence.  max_q and max_length bound the new tokens and the keys of a sequence: they
  * shape the launch, and a batch that passes them is computed all the same, more slowly.  Pages may be
- * shared between sequences.  tokens * n_heads is below 2^26, n_pages at most 2^24.  Numbers of the
+ * shared between sequences.  tokens * n_heads is below 2^24, n_pages at most 2^24.  Numbers of the
  * pages are rounded to q's type (exact within the limits above for pages written in that type). */
 typedef struct FcvFp4Attention {
   const void* q;          /* [tokens][n_heads][head_dim], strides q_row, q_head */

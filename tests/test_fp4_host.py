@@ -73,7 +73,8 @@ def _linear(fcv, **kw):
     (dict(ld_scales=-2), "negative"), (dict(ldy=31), "shorter"), (dict(ldr=-8), "negative"),
     (dict(x=None), "null"), (dict(codes=None), "null"), (dict(scales=None), "null"),
     (dict(codes=BIG + 8), "16-byte"), (dict(ld_codes=40), "16-byte"), (dict(x=BIG + 1), "boundary"),
-    (dict(y=BIG + 2, y_dtype=2), "boundary"), (dict(m=1 << 23), "limited"), (dict(k=1 << 27), "2\\^26"),
+    (dict(y=BIG + 2, y_dtype=2), "boundary"), (dict(m=1 << 23), "limited"), (dict(k=1 << 22), "2\\^21"),
+    (dict(ld_codes=1 << 24), "2\\^24"), (dict(ld_scales=1 << 24), "2\\^24"),
     (dict(m=1 << 20, n=1 << 20, ldy=1 << 20), "limited")])
 def test_linear_refuses(fcv, bad, match):
     _refuse(fcv, _linear(fcv, **bad), match)
@@ -134,7 +135,7 @@ def _attention(fcv, ws=BIG, ws_bytes=1 << 40, **kw):
 
 @pytest.mark.parametrize("bad,match", [
     (dict(dtype=2), "dtype"), (dict(head_dim=96), "head_dim"), (dict(batch=0), "batch"),
-    (dict(n_heads=3), "multiple"), (dict(tokens=-1), "tokens"), (dict(tokens=1 << 25), "2\\^26"),
+    (dict(n_heads=3), "multiple"), (dict(tokens=-1), "tokens"), (dict(tokens=1 << 25), "2\\^24"),
     (dict(tokens=5), "divide"), (dict(n_pages=0), "n_pages"), (dict(max_pages=0), "max_pages"),
     (dict(max_pages=1 << 25), "max_pages"), (dict(max_q=0), "max_q"), (dict(max_length=-1), "max_length"),
     (dict(scale=0.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(q=None), "null"),
