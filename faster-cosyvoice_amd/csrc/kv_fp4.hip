@@ -3,14 +3,15 @@
 //
 // Per head x of D elements:  y = x / sqrt(mean(x^2) + eps) * w;  the first R elements are rotated in pairs,
 // (a, b) -> (a cos - b sin, b cos + a sin).  Queries are rounded to 16 bits once; keys go to 4 bits in
-// groups of 32, values of a head in one group.  All of it runs in 64 bits: a value next to the border of
-// two codes, whose step is a third of it, goes where the formula puts it, and squares have the room.
+// groups of 32, values of a head in one group.  Keys are computed in 64 bits: one next to the border of two
+// codes, whose step is a third of it, goes where the formula puts it.
 //
 // Bound: bandwidth (each element is read once and written once), or the launch itself for a few tokens.
-// Split: a head takes D / 16 lanes, each with 16 consecutive elements; it reads the chunks that hold the
-// other members of its pairs, too (from cache: they are a neighbour's), so that nothing is exchanged but the
-// head's sum of squares and the groups' largest magnitudes.
+// Split: a head takes D / 16 lanes with two chunks of 8 each (rope.hpp), so that nothing is exchanged but the
+// head's sum of squares and its groups' largest magnitudes.  A workgroup has heads of one kind; of keys and
+// values a wave has 8 neighbouring tokens of a head, whose bytes lie side by side in a page.
 #include "fp4.hpp"
+#include "rope.hpp"
 
 namespace fcv {
 namespace lm {
@@ -38,50 +39,59 @@ __device__ __forceinline__ float to_odd(double v) {
   return __uint_as_float(u);
 }
 
-template <class E>
-__device__ __forceinline__ float weight(const void* w, bool f32, int i) {
-  return f32 ? static_cast<const float*>(w)[i] : E::to_f32(static_cast<const short*>(w)[i]);
+// Keys and values are dealt out 8 tokens of a head at a time: unit -> (token, head).
+constexpr int kTokens = 8;
+struct Unit {
+  uint32_t token;
+  int head;
+};
+__device__ __forceinline__ Unit unit_of(uint32_t u, uint32_t heads) {
+  const uint32_t v = u / kTokens, block = v / heads;
+  return Unit{block * kTokens + u % kTokens, (int)(v - block * heads)};
 }
+int64_t units_of(int64_t tokens, int64_t heads) { return (tokens + kTokens - 1) / kTokens * kTokens * heads; }
 
-// 8 elements from `at` of a head, normed.
-template <class E>
-__device__ __forceinline__ void normed8(const short* head, int at, const void* w, bool wf, double inv,
-                                        double (&out)[8]) {
-  const s16x8 v = *reinterpret_cast<const s16x8*>(head + at);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    out[e] = E::to_f32(v[e]);
-    if (w) out[e] *= inv * (double)weight<E>(w, wf, at + e);
-  }
-}
+// Workgroups of keys, of values, then of queries.
+struct AppendArgs {
+  FcvFp4Append p;
+  uint32_t kv_blocks;  // of the keys, and of the values
+};
 
-// Heads in order: every token's query heads, then its key heads, then its value heads.
 template <class E, int D>
-__global__ __launch_bounds__(kThreads) void append_fp4_kernel(const FcvFp4Append p) {
-  constexpr int L = D / 16;  // lanes of a head
+__global__ __launch_bounds__(kThreads) void append_fp4_kernel(const AppendArgs a) {
+  constexpr int L = D / 16, kHeads = kThreads / L, kChunks = D / 8;
   constexpr bool kHalf = std::is_same<E, Half>::value;
   using P = Page<D>;
-  const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / L;
-  const int j = threadIdx.x % L;
-  const int64_t n_q = (int64_t)p.tokens * p.n_heads, n_kv = (int64_t)p.tokens * p.n_kv_heads;
-  if (unit >= n_q + 2 * n_kv) return;  // whole heads: lanes that meet leave together
-  const bool is_q = unit < n_q, is_v = unit >= n_q + n_kv;
-  const uint32_t local = (uint32_t)(is_q ? unit : is_v ? unit - n_q - n_kv : unit - n_q);
-  const uint32_t heads = is_q ? p.n_heads : p.n_kv_heads;
-  const uint32_t token = local / heads;
-  const int h = (int)(local - token * heads);
-  const short* head = static_cast<const short*>(p.qkv) + (int64_t)token * p.qkv_row +
-                      (int64_t)(is_q ? h : is_v ? p.n_heads + p.n_kv_heads + h : p.n_heads + h) * D;
+  __shared__ __attribute__((aligned(16))) uint32_t tops[kHeads][kChunks];
+  const FcvFp4Append& p = a.p;
+  const int j = threadIdx.x % L, local = threadIdx.x / L;
+  const int half_chunks = p.rope_dim / 16;  // chunks of half the rotated part
+  const bool turned = j < half_chunks;
+  const int c0 = turned ? j : 2 * j, c1 = turned ? j + half_chunks : 2 * j + 1;
 
-  uint8_t* page = nullptr;
-  int place = 0;
-  if (!is_q) {
-    const int32_t row = p.cache_rows[token];
-    if (row >= 0 && row / P::kTokens < p.n_pages) {
-      page = p.pages + (int64_t)(row / P::kTokens) * p.page_stride + (int64_t)h * p.head_stride;
-      place = row % P::kTokens;
-    }
+  if (blockIdx.x >= 2 * a.kv_blocks) {
+    const uint32_t unit = (blockIdx.x - 2 * a.kv_blocks) * kHeads + local;
+    if (unit >= (uint32_t)p.tokens * (uint32_t)p.n_heads) return;  // whole heads leave together
+    const uint32_t token = unit / (uint32_t)p.n_heads, h = unit - token * (uint32_t)p.n_heads;
+    const short* src = static_cast<const short*>(p.qkv) + (int64_t)token * p.qkv_row + (int64_t)h * D;
+    s16x8 x0 = *reinterpret_cast<const s16x8*>(src + c0 * 8);
+    s16x8 x1 = *reinterpret_cast<const s16x8*>(src + c1 * 8);
+    norm_rotate<E, D>(p, token, p.q_weight, turned, c0, c1, x0, x1);
+    short* to = static_cast<short*>(p.q_out) + (int64_t)token * p.q_row + (int64_t)h * D;
+    *reinterpret_cast<s16x8*>(to + c0 * 8) = x0;
+    *reinterpret_cast<s16x8*>(to + c1 * 8) = x1;
+    return;
   }
+
+  const bool is_v = blockIdx.x >= a.kv_blocks;
+  const Unit u = unit_of((blockIdx.x - (is_v ? a.kv_blocks : 0)) * kHeads + local, p.n_kv_heads);
+  if (u.token >= (uint32_t)p.tokens) return;
+  const int32_t row = p.cache_rows[u.token];
+  if (row < 0 || row / P::kTokens >= p.n_pages) return;
+  uint8_t* page = p.pages + (int64_t)(row / P::kTokens) * p.page_stride + (int64_t)u.head * p.head_stride;
+  const int place = row % P::kTokens;
+  const short* head = static_cast<const short*>(p.qkv) + (int64_t)u.token * p.qkv_row +
+                      (int64_t)(p.n_heads + (is_v ? p.n_kv_heads : 0) + u.head) * D;
 
   if (is_v) {
     const s16x8 v0 = *reinterpret_cast<const s16x8*>(head + 16 * j);
@@ -102,7 +112,6 @@ __global__ __launch_bounds__(kThreads) void append_fp4_kernel(const FcvFp4Append
       c[0] = fp4_word(v, scale_of(b));
       c[1] = fp4_word(v + 8, scale_of(b));
     }
-    if (!page) return;
     uint8_t* to = page + P::kValues + 8 * j * P::kTokens + place;
 #pragma unroll
     for (int e = 0; e < 8; ++e) to[e * P::kTokens] = (uint8_t)(c[e / 4] >> (8 * (e % 4)));
@@ -110,98 +119,100 @@ __global__ __launch_bounds__(kThreads) void append_fp4_kernel(const FcvFp4Append
     return;
   }
 
-  const void* w = is_q ? p.q_weight : p.k_weight;
-  const bool wf = p.weight_dtype == FCV_LM_F32;
-  double inv = 1.0;
-  if (w) {
-    const s16x8 v0 = *reinterpret_cast<const s16x8*>(head + 16 * j);
-    const s16x8 v1 = *reinterpret_cast<const s16x8*>(head + 16 * j + 8);
+  const s16x8 x0 = *reinterpret_cast<const s16x8*>(head + c0 * 8);
+  const s16x8 x1 = *reinterpret_cast<const s16x8*>(head + c1 * 8);
+  double k0[8], k1[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    k0[e] = E::to_f32(x0[e]);
+    k1[e] = E::to_f32(x1[e]);
+  }
+  if (p.k_weight) {
     double ss = 0.0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double a = E::to_f32(v0[e]), b = E::to_f32(v1[e]);
-      ss = fma(a, a, fma(b, b, ss));
-    }
+    for (int e = 0; e < 8; ++e) ss = fma(k0[e], k0[e], fma(k1[e], k1[e], ss));
     ss += dpp_d<0xB1>(ss);
     ss += dpp_d<0x4E>(ss);
     if constexpr (L == 8) ss += dpp_d<0x141>(ss);
-    inv = 1.0 / sqrt(ss / D + (double)p.eps);
-  }
-  const int pos = min(max(p.positions[token], 0), p.max_pos - 1);
-  const float* cos_row = p.rope_cos + (int64_t)pos * (p.rope_dim / 2);
-  const float* sin_row = p.rope_sin + (int64_t)pos * (p.rope_dim / 2);
-  const int half = p.rope_dim / 2;
-  float y[16];
+    const double inv = 1.0 / sqrt(ss / D + (double)p.eps);
+    const bool wf = p.weight_dtype == FCV_LM_F32;
+    float w0[8], w1[8];
+    load8<E>(p.k_weight, wf, c0 * 8, w0);
+    load8<E>(p.k_weight, wf, c1 * 8, w1);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int at = 16 * j + 8 * i;  // rope_dim / 2 is a multiple of 8: a chunk is on one side of it
-    double a[8];
-    normed8<E>(head, at, w, wf, inv, a);
-    if (at < p.rope_dim) {
-      if (p.interleaved) {
+    for (int e = 0; e < 8; ++e) {
+      k0[e] *= inv * (double)w0[e];
+      k1[e] *= inv * (double)w1[e];
+    }
+  }
+  if (turned) {
+    const int pos = min(max(p.positions[u.token], 0), p.max_pos - 1);
+    const float* cos_row = p.rope_cos + (int64_t)pos * (p.rope_dim / 2);
+    const float* sin_row = p.rope_sin + (int64_t)pos * (p.rope_dim / 2);
+    if (p.interleaved) {
+      auto turn = [&](double (&k)[8], int c) {
+        const f32x4 cs = *reinterpret_cast<const f32x4*>(cos_row + c * 4);
+        const f32x4 sn = *reinterpret_cast<const f32x4*>(sin_row + c * 4);
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const double c = cos_row[at / 2 + e / 2], s = sin_row[at / 2 + e / 2];
-          const double u = a[e], v = a[e + 1];
-          a[e] = fma(u, c, -(v * s));
-          a[e + 1] = fma(v, c, u * s);
+          const double x = k[e], y = k[e + 1], cd = cs[e / 2], sd = sn[e / 2];
+          k[e] = fma(x, cd, -(y * sd));
+          k[e + 1] = fma(y, cd, x * sd);
         }
-      } else {
-        const bool second = at >= half;
-        const int t = second ? at - half : at;
-        double o[8];
-        normed8<E>(head, second ? t : at + half, w, wf, inv, o);
+      };
+      turn(k0, c0);
+      turn(k1, c1);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const double c = cos_row[t + e], s = sin_row[t + e];
-          a[e] = fma(a[e], c, second ? o[e] * s : -(o[e] * s));
+      for (int q = 0; q < 8; q += 4) {
+        const f32x4 cs = *reinterpret_cast<const f32x4*>(cos_row + c0 * 8 + q);
+        const f32x4 sn = *reinterpret_cast<const f32x4*>(sin_row + c0 * 8 + q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const double x = k0[q + e], y = k1[q + e], cd = cs[e], sd = sn[e];
+          k0[q + e] = fma(x, cd, -(y * sd));
+          k1[q + e] = fma(y, cd, x * sd);
         }
       }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[8 * i + e] = is_q ? (float)a[e] : to_odd(a[e]);
   }
-  if (is_q) {
-    short* to = static_cast<short*>(p.q_out) + (int64_t)token * p.q_row + (int64_t)h * D + 16 * j;
-    s16x8 r[2];
+  float y0[8], y1[8];
+  uint32_t t0 = 0, t1 = 0;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) r[e / 8][e % 8] = E::from_f32(y[e]);
-    *reinterpret_cast<s16x8*>(to) = r[0];
-    *reinterpret_cast<s16x8*>(to + 8) = r[1];
-    return;
+  for (int e = 0; e < 8; ++e) {
+    y0[e] = to_odd(k0[e]);
+    y1[e] = to_odd(k1[e]);
+    t0 = max(t0, __float_as_uint(y0[e]) & 0x7fffffffu);
+    t1 = max(t1, __float_as_uint(y1[e]) & 0x7fffffffu);
   }
-  uint32_t top = 0;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
-  top = max(top, dpp_u<0xB1>(top));
-  const uint32_t b = fp4_scale_byte(top, kHalf);
-  u32x2 c = {0, 0};
-  if (b != 255) {
-    c[0] = fp4_word(y, scale_of(b));
-    c[1] = fp4_word(y + 8, scale_of(b));
-  }
-  if (!page) return;
-  *reinterpret_cast<u32x2*>(page + place * P::kKey + 8 * j) = c;
-  if (j % 2 == 0) page[P::kScales + place * P::kKeyScales + j / 2] = (uint8_t)b;
+  // a group's four chunks may be in any lanes of the head
+  tops[local][c0] = t0;
+  tops[local][c1] = t1;
+  wave_fence();
+  auto store = [&](const float (&y)[8], int c) {
+    const u32x4 t = *reinterpret_cast<const u32x4*>(&tops[local][c & ~3]);
+    const uint32_t b = fp4_scale_byte(max(max(t[0], t[1]), max(t[2], t[3])), kHalf);
+    *reinterpret_cast<uint32_t*>(page + place * P::kKey + 4 * c) = b == 255 ? 0 : fp4_word(y, scale_of(b));
+    if (c % 4 == 0) page[P::kScales + place * P::kKeyScales + c / 4] = (uint8_t)b;
+  };
+  store(y0, c0);
+  store(y1, c1);
 }
 
 // A thread has 16 elements of a token's key head or value head.
 template <class E, int D>
-__global__ __launch_bounds__(kThreads) void read_fp4_kernel(const FcvFp4Read p) {
-  constexpr int L = D / 16;
+__global__ __launch_bounds__(kThreads) void read_fp4_kernel(const FcvFp4Read p, uint32_t blocks) {
+  constexpr int L = D / 16, kHeads = kThreads / L;
   using P = Page<D>;
-  const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / L;
   const int j = threadIdx.x % L;
-  const int64_t n = (int64_t)p.tokens * p.n_kv_heads;
-  if (unit >= 2 * n) return;
-  const bool is_v = unit >= n;
-  const uint32_t local = (uint32_t)(is_v ? unit - n : unit);
-  const uint32_t token = local / p.n_kv_heads;
-  const int h = (int)(local - token * p.n_kv_heads);
-  const int32_t row = p.rows[token];
+  const bool is_v = blockIdx.x >= blocks;
+  const Unit u = unit_of((blockIdx.x - (is_v ? blocks : 0)) * kHeads + threadIdx.x / L, p.n_kv_heads);
+  if (u.token >= (uint32_t)p.tokens) return;
+  const int32_t row = p.rows[u.token];
   s16x8 r[2] = {};
   if (row >= 0 && row / P::kTokens < p.n_pages) {
-    const uint8_t* page = p.pages + (int64_t)(row / P::kTokens) * p.page_stride + (int64_t)h * p.head_stride;
+    const uint8_t* page =
+        p.pages + (int64_t)(row / P::kTokens) * p.page_stride + (int64_t)u.head * p.head_stride;
     const int place = row % P::kTokens;
     u32x2 c = {0, 0};
     uint32_t b;
@@ -217,8 +228,8 @@ __global__ __launch_bounds__(kThreads) void read_fp4_kernel(const FcvFp4Read p) 
     r[0] = fp4_octet<E>(c[0], scale_of(b));
     r[1] = fp4_octet<E>(c[1], scale_of(b));
   }
-  short* to = static_cast<short*>(is_v ? p.v : p.k) + (int64_t)token * (is_v ? p.v_row : p.k_row) +
-              (int64_t)h * D + 16 * j;
+  short* to = static_cast<short*>(is_v ? p.v : p.k) + (int64_t)u.token * (is_v ? p.v_row : p.k_row) +
+              (int64_t)u.head * D + 16 * j;
   *reinterpret_cast<s16x8*>(to) = r[0];
   *reinterpret_cast<s16x8*>(to + 8) = r[1];
 }
@@ -284,26 +295,28 @@ int check(const FcvFp4Read* p) {
   return FCV_OK;
 }
 
+uint32_t blocks_of(int64_t units, int head_dim) {
+  const int heads = kThreads * 16 / head_dim;
+  return (uint32_t)((units + heads - 1) / heads);
+}
+
 template <class E>
 void launch(const FcvFp4Append& p, hipStream_t stream) {
-  const int64_t units = (int64_t)p.tokens * (p.n_heads + 2 * p.n_kv_heads);
-  const int per_block = kThreads * 16 / p.head_dim;
-  const dim3 grid((unsigned)((units + per_block - 1) / per_block));
+  const AppendArgs a{p, blocks_of(units_of(p.tokens, p.n_kv_heads), p.head_dim)};
+  const dim3 grid(2 * a.kv_blocks + blocks_of((int64_t)p.tokens * p.n_heads, p.head_dim));
   if (p.head_dim == 64)
-    hipLaunchKernelGGL((append_fp4_kernel<E, 64>), grid, dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((append_fp4_kernel<E, 64>), grid, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((append_fp4_kernel<E, 128>), grid, dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((append_fp4_kernel<E, 128>), grid, dim3(kThreads), 0, stream, a);
 }
 
 template <class E>
 void launch(const FcvFp4Read& p, hipStream_t stream) {
-  const int64_t units = 2 * (int64_t)p.tokens * p.n_kv_heads;
-  const int per_block = kThreads * 16 / p.head_dim;
-  const dim3 grid((unsigned)((units + per_block - 1) / per_block));
+  const uint32_t blocks = blocks_of(units_of(p.tokens, p.n_kv_heads), p.head_dim);
   if (p.head_dim == 64)
-    hipLaunchKernelGGL((read_fp4_kernel<E, 64>), grid, dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((read_fp4_kernel<E, 64>), dim3(2 * blocks), dim3(kThreads), 0, stream, p, blocks);
   else
-    hipLaunchKernelGGL((read_fp4_kernel<E, 128>), grid, dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((read_fp4_kernel<E, 128>), dim3(2 * blocks), dim3(kThreads), 0, stream, p, blocks);
 }
 
 template <class A>

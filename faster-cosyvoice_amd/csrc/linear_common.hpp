@@ -184,13 +184,6 @@ __device__ __forceinline__ void wait_ahead(int ahead) {
   }
 }
 
-// LDS written by a wave is read by the same wave: in order, once the compiler keeps it so.
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // The epilogue of a tile kernel whose waves have TM x TN blocks of 32 x 32 outputs each in `acc`: waves at
 // (wm0, wn0) of the tile at row m0 and column n0, `smem` the workgroup's LDS (its kLds bytes are free).
 template <class E, class C, int kLds>

@@ -59,6 +59,13 @@ struct Bf16 {
   }
 };
 
+// LDS written by a wave is read by the same wave: in order, once the compiler keeps it so.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Whether 16-byte accesses fit a dimension of `count` entries; the stride of a single one says nothing.
 inline bool stride_fits(int64_t stride, int64_t count) {
   return count <= 1 || (stride >= 0 && stride % 8 == 0);

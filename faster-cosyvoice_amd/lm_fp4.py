@@ -203,10 +203,10 @@ def qk_norm_rope_fp4(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tens
 
     Token ``t``'s key and value go to place ``cache_rows[t] % 64`` of page ``cache_rows[t] // 64`` of
     ``pages`` (a layer of ``new_fp4_pages``); a negative row or one past the pool goes nowhere.  Keys
-    are quantized after norm and rotation, in groups of 32, values in one group a head, both in 64
-    bits (``quantize_fp4`` has the rule).  Of tokens that name the same row any one's bytes may remain.
+    are quantized after norm and rotation, computed in 64 bits, in groups of 32, values in one group a
+    head (``quantize_fp4`` has the rule).  Of tokens that name the same row any one's bytes may remain.
     Everything else is ``qk_norm_rope``'s.  Returns the queries ``[T, n_heads, head dim]``, in ``out`` if
-    given, which overlaps neither ``qkv`` nor the pages."""
+    given, which may be their own columns of ``qkv`` and overlaps nothing else."""
     code = _dtype(qkv, "qkv")
     n_pages, n_kv, dim, page_stride, head_stride = _pool(pages, qkv.device)
     if qkv.dim() != 2 or n_heads < 1 or qkv.shape[1] != (n_heads + 2 * n_kv) * dim:
@@ -245,9 +245,10 @@ def qk_norm_rope_fp4(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tens
     qkv_ptr, out_ptr, pages_ptr = qkv.data_ptr(), out.data_ptr(), pages.data_ptr()
     q_row = out.stride(0) if tokens > 1 else n_heads * dim
     if given:
-        _check_apart(out, out_ptr, 2 * ((tokens - 1) * q_row + n_heads * dim),
-                     [("pages", pages, pages_ptr, _reach(pages)),
-                      ("qkv", qkv, qkv_ptr, 2 * ((tokens - 1) * qkv_row + qkv.shape[1]))])
+        inputs = [("pages", pages, pages_ptr, _reach(pages))]
+        if out_ptr != qkv_ptr or (tokens > 1 and q_row != qkv_row):
+            inputs.append(("qkv", qkv, qkv_ptr, 2 * ((tokens - 1) * qkv_row + qkv.shape[1])))
+        _check_apart(out, out_ptr, 2 * ((tokens - 1) * q_row + n_heads * dim), inputs)
     args = _pack(_APPEND, qkv_ptr, pos_ptr, row_ptr, cos.data_ptr(), sin.data_ptr(), qw_ptr, kw_ptr,
                  out_ptr, pages_ptr, qkv_row, q_row, page_stride, head_stride, tokens, n_heads,
                  n_kv, dim, 2 * table[1], table[0], n_pages, code, w_code, bool(interleaved), eps)

@@ -97,7 +97,8 @@ size_t fcv_fp4_page_bytes(int32_t head_dim);
 
 /* fcv_lm_qk_norm_rope over pages: token t's key and value go to place cache_rows[t] % 64 of page
  * cache_rows[t] / 64, in 4 bits; a negative row or one past the pool goes nowhere.  A key's norm and
- * rotation are computed in 64 bits, so that its codes are those of the formula. */
+ * rotation are computed in 64 bits, so that its codes are those of the formula.  q_out may be the queries' own
+ * columns of qkv (same start and row stride); it and the pages overlap nothing else. */
 typedef struct FcvFp4Append {
   const void* qkv;           /* [tokens][(n_heads + 2 n_kv_heads) head_dim], row stride qkv_row */
   const int32_t* positions;  /* [tokens] */

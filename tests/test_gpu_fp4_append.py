@@ -198,6 +198,17 @@ def test_strides(fcv):
     assert int(pool[0].sum()) + int(pool[2].sum()) + int(pool[1, :, n].sum()) == 0
 
 
+def test_queries_in_place(fcv):
+    """The queries' own columns of qkv as the output: keys and values read theirs."""
+    for d, hq, hk in ((64, 6, 2), (128, 4, 4)):
+        st = make(130, hq, hk, d, torch.bfloat16, normed=True)
+        ref = {k: v.clone() for k, v in st.items()}
+        want = append(fcv, ref, hq)
+        got = append(fcv, st, hq, out=st["qkv"].view(130, hq + 2 * hk, d)[:, :hq])
+        assert torch.equal(got, want) and torch.equal(st["pages"], ref["pages"])
+        assert torch.equal(st["qkv"][:, hq * d:], ref["qkv"][:, hq * d:])
+
+
 def test_captured_and_no_tokens(fcv):
     st = make(16, 4, 2, 128, torch.bfloat16, normed=True)
     graph = torch.cuda.CUDAGraph()
@@ -234,7 +245,7 @@ def test_refusals(fcv):
         (dict(rows=st["rows"].long()), "int32"), (dict(positions=st["positions"][:3]), "int32"),
         (dict(kw=None), "together"), (dict(cos=st["cos"].half()), "float32 table"),
         (dict(cos=st["cos"][:, :4].contiguous(), sin=st["sin"][:, :4].contiguous()), "rope_dim"),
-        (dict(out=st["qkv"].view(4, 8, 64)[:, :4]), "out overlaps qkv"),
+        (dict(out=st["qkv"].view(4, 8, 64)[:, 1:5]), "out overlaps qkv"),
         (dict(pages=over, out=over.view(-1)[:2048].view(torch.float16).view(4, 4, 64)), "out overlaps pages"),
         (dict(pages=st["pages"][:1].expand(5, -1, -1)), "none over another"),
         (dict(eps=-1.0), "eps"), (dict(qkv=st["qkv"].float()), "float16 or bfloat16"),
