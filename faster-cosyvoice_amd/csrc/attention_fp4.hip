@@ -29,6 +29,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 template <class E>
 constexpr float kHeld = std::is_same<E, Bf16>::value ? 0x1p-24f : 1.0f;
 
+constexpr int kTileRows = 128;  // of a workgroup of many rows
+
 struct AttendArgs {
   FcvFp4Attention p;
   int group;                 // query heads of a key head
@@ -346,6 +348,254 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
   }
 }
 
+// ---- many rows -------------------------------------------------------------------------------------
+//
+// 128 rows of a sequence's key head to a workgroup, 32 to a wave (v_mfma_f32_32x32x16).  Each page's codes become
+// 16-bit numbers once, in LDS: keys [64][D], values [D][64] in the order of the S^T tiles' rows, so that a
+// lane's weights are its right operand again.  Two pages' room: one barrier a page.
+template <int D>
+__device__ __forceinline__ int key_chunk(int row, int c) {  // 16 rows read at one chunk touch all banks
+  return D == 128 ? c ^ (row & 15) : c ^ ((row >> 1) & 7);
+}
+__device__ __forceinline__ int value_chunk(int row, int c) { return c ^ ((row >> 1) & 7); }
+
+template <class E, int D>
+__global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArgs a) {
+  using P = Page<D>;
+  constexpr int kRows = kTileRows, kSteps = D / 16, kDT = D / 32;
+  __shared__ __attribute__((aligned(16))) short sk[2][kPage * D];
+  __shared__ __attribute__((aligned(16))) short sv[2][D * kPage];
+  __shared__ __attribute__((aligned(16))) uint32_t svs[2][kPage / 4];
+  const FcvFp4Attention& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 31, fh = lane >> 5;
+  const int kv = blockIdx.x % p.n_kv_heads, turn = blockIdx.x / p.n_kv_heads % a.row_tiles;
+  const int b = blockIdx.x / p.n_kv_heads / a.row_tiles;
+  typedef const int32_t __attribute__((address_space(4))) * Uniform;  // nothing writes these: scalar loads
+  const Uniform table = (Uniform)(uintptr_t)(p.table + (int64_t)b * p.table_row);
+  int first, n;
+  if (p.cu_q) {
+    const Uniform ends = (Uniform)(uintptr_t)(p.cu_q + b);
+    first = min(max(ends[0], 0), p.tokens);
+    n = min(max(ends[1], first), p.tokens) - first;
+  } else {
+    n = a.each;
+    first = b * n;
+  }
+  const int keys = ((Uniform)(uintptr_t)p.lengths)[b];
+  const int rows = n * a.group;  // below 2^24
+  const int length = min(max(keys, 0), (int)min((int64_t)p.max_pages * kPage, (int64_t)0x7fffffff));
+  const uint8_t* pool = p.pages + (int64_t)kv * p.head_stride;
+  const float scale = p.scale * kLog2e;
+  // the tiles with the most keys first
+  const int tiles = (rows + kRows - 1) / kRows;
+  for (int t0 = turn; t0 < tiles; t0 += a.row_tiles) {
+    const int row0 = (tiles - 1 - t0) * kRows;
+    const int mine = row0 + 32 * wave;  // the wave's first row
+    const bool there = mine + fr < rows;
+    const int row = min(mine + fr, rows - 1);
+    const int token = row / a.group, head = kv * a.group + row - token * a.group;
+    const int limit = there ? length - n + token + 1 : 0;  // the row's visible keys
+    auto sees = [&](int r) { return min(max(length - n + min(r, rows - 1) / a.group + 1, 0), length); };
+    const int reach = mine < rows ? sees(mine + 31) : 0;   // of the wave
+    const int all_pages = (sees(row0 + kRows - 1) + kPage - 1) / kPage;
+    const int page0 = blockIdx.y * a.pages_per;
+    int page1 = min(page0 + a.pages_per, all_pages);
+    if (blockIdx.y == (unsigned)a.splits - 1) page1 = all_pages;  // and what max_length left out
+
+    s16x8 fq[kSteps];
+    {
+      const short* q = static_cast<const short*>(p.q) + (int64_t)(first + token) * p.q_row +
+                       (int64_t)head * p.q_head + 8 * fh;
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) fq[j] = *reinterpret_cast<const s16x8*>(q + 16 * j);
+    }
+    f32x16 o[kDT];
+#pragma unroll
+    for (int d = 0; d < kDT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;
+
+    // a thread's share of a page: D / 4 codes of a key, 16 bytes of a byte row of the values
+    uint32_t kw[D / 32], ks, vsw = 0;
+    u32x4 vw = {0, 0, 0, 0};
+    auto load = [&](int id) {
+      const uint8_t* page = pool + (int64_t)max(id, 0) * p.page_stride;
+      if constexpr (D == 128) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(page + (uint32_t)tid * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kw[j] = w[j];
+        ks = page[P::kScales + (uint32_t)tid];
+        vw = *reinterpret_cast<const u32x4*>(page + P::kValues + (uint32_t)tid * 16);
+      } else {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(page + (uint32_t)tid * 8);
+        kw[0] = w[0];
+        kw[1] = w[1];
+        ks = page[P::kScales + (uint32_t)tid / 2];
+        if (tid < 128) vw = *reinterpret_cast<const u32x4*>(page + P::kValues + (uint32_t)tid * 16);
+      }
+      if (tid < kPage / 4)
+        vsw = *reinterpret_cast<const uint32_t*>(page + P::kValueScales + (uint32_t)tid * 4);
+    };
+    auto unpack = [&](int buf) {
+      const int key = tid / 4;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+        *reinterpret_cast<s16x8*>(&sk[buf][key * D + key_chunk<D>(key, tid % 4 * (D / 32) + j) * 8]) =
+            fp4_octet<E>(kw[j], scale_of(ks));
+      if (D == 128 || tid < 128) {
+        // key 8 g + 4 h + j of 16: half h's slot pair j, as codes of one element side by side in a byte
+        const int pair = tid / 4, step = tid % 4;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w0 = vw[h], w1 = vw[2 + h];
+          const uint32_t we = (w0 & 0x0f0f0f0fu) | (w1 << 4 & 0xf0f0f0f0u);
+          const uint32_t wo = (w0 >> 4 & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
+          *reinterpret_cast<s16x8*>(
+              &sv[buf][2 * pair * kPage + value_chunk(2 * pair, 2 * step + h) * 8]) =
+              fp4_octet<Bf16>(we, kHeld<E>);
+          *reinterpret_cast<s16x8*>(
+              &sv[buf][(2 * pair + 1) * kPage + value_chunk(2 * pair + 1, 2 * step + h) * 8]) =
+              fp4_octet<Bf16>(wo, kHeld<E>);
+        }
+      }
+      if (tid < kPage / 4) svs[buf][tid % 2 * 8 + tid / 2] = vsw;
+    };
+    auto take = [&](int page, int buf) {
+      f32x16 s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int key = 32 * t + fr;
+          s[t] = E::mfma32(
+              *reinterpret_cast<const s16x8*>(&sk[buf][key * D + key_chunk<D>(key, 2 * j + fh) * 8]), fq[j],
+              s[t]);
+        }
+      // the scales of the lane's keys: 8 g + 4 fh + j in byte j of word g
+      uint32_t vs[8];
+      {
+        const u32x4 v0 = *reinterpret_cast<const u32x4*>(&svs[buf][fh * 8]);
+        const u32x4 v1 = *reinterpret_cast<const u32x4*>(&svs[buf][fh * 8 + 4]);
+#pragma unroll
+        for (int g = 0; g < 8; ++g) vs[g] = g < 4 ? v0[g % 4] : v1[g % 4];
+      }
+      if (!__all(limit >= (page + 1) * kPage)) {  // hidden keys: no score, and a scale that is a number
+        const int seen = limit - page * kPage - 4 * fh;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (8 * g + j >= seen) s[g / 4][g % 4 * 4 + j] = -__builtin_inff();
+          const int k = min(max(seen - 8 * g, 0), 4);
+          vs[g] &= k == 4 ? ~0u : (1u << (8 * k)) - 1;
+        }
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
+      {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false,
+                                                        false);
+        top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * scale;
+      }
+      if (__any(top > m)) {
+        const float next = fmaxf(m, top);
+        const float alpha = next == -__builtin_inff() ? 1.0f : hw_exp2(m - next);
+        m = next;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) o[d] *= alpha;
+      }
+      const float base = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {  // 16 keys: words 2 st and 2 st + 1 of the lane's eight
+        u32x4 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float w[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int g = 2 * st + i;
+            const float e = hw_exp2(fmaf(s[g / 4][g % 4 * 4 + j], scale, -base));
+            l += e;
+            w[i] = e * scale_of((vs[g] >> (8 * j)) & 255);
+          }
+          const uint32_t u = bf16_pair(w[0], w[1]);
+          hi[j] = u;
+          lo[j] = bf16_pair(w[0] - __uint_as_float(u << 16), w[1] - __uint_as_float(u & 0xffff0000u));
+        }
+        const s16x8 ph = __builtin_bit_cast(s16x8, hi), pl = __builtin_bit_cast(s16x8, lo);
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) {
+          const int r = 32 * d + fr;
+          const s16x8 v =
+              *reinterpret_cast<const s16x8*>(&sv[buf][r * kPage + value_chunk(r, 2 * st + fh) * 8]);
+          o[d] = Bf16::mfma32(v, ph, o[d]);
+          o[d] = Bf16::mfma32(v, pl, o[d]);
+        }
+      }
+    };
+
+    if (page0 < page1) {
+      auto number = [&](int page) {
+        const int id = table[min(page, p.max_pages - 1)];
+        return page < page1 && id < p.n_pages ? id : -1;
+      };
+      int id = number(page0), next = number(page0 + 1);
+      load(id);
+      for (int page = page0; page < page1; ++page) {
+        const int buf = (page - page0) & 1;
+        const int after = number(page + 2);
+        unpack(buf);
+        __syncthreads();
+        load(next);
+        if (id >= 0 && page * kPage < reach) take(page, buf);
+        id = next;
+        next = after;
+      }
+    }
+    l = swap32_sum(l);
+    if (there) {
+      const int64_t at = (int64_t)(first + token) * p.n_heads + head;
+      if (a.splits > 1) {
+        const int64_t i = (int64_t)blockIdx.y * p.tokens * p.n_heads + at;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(a.part + i * D + 32 * d + 8 * g + 4 * fh) =
+                f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+        if (fh == 0) {
+          a.part_ml[2 * i] = m;
+          a.part_ml[2 * i + 1] = l;
+        }
+      } else {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / (l * kHeld<E>);
+        short* to = static_cast<short*>(p.out) + (int64_t)(first + token) * p.out_row +
+                    (int64_t)head * p.out_head + 4 * fh;
+#pragma unroll
+        for (int d = 0; d < kDT; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<s16x4*>(to + 32 * d + 8 * g) =
+                s16x4{E::from_f32(o[d][4 * g] * inv), E::from_f32(o[d][4 * g + 1] * inv),
+                      E::from_f32(o[d][4 * g + 2] * inv), E::from_f32(o[d][4 * g + 3] * inv)};
+        if (p.lse && fh == 0) p.lse[at] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+      }
+    }
+    __syncthreads();  // the next tile's pages go where this one's were
+  }
+}
+
 // The ranges' sums.  A workgroup has one row's head: a thread 4 elements of every kGroups-th range, in their
 // order, and the groups are summed in theirs.
 template <class E, int D>
@@ -452,7 +702,11 @@ struct Plan {
 Plan plan_of(const FcvFp4Attention& p) {
   const int group = p.n_heads / p.n_kv_heads;
   const int64_t most_rows = (int64_t)std::min(p.max_q, p.tokens) * group;
-  const int rows = most_rows <= 8 ? 8 : 16;
+  // Tiles of 128 rows where they give every CU two workgroups: 4000 tokens of 32 heads of 128 over 8 (1000
+  // tiles) take 225 us by them, 304 by 16 rows; 8 x 300 behind a cache (640) 196 and 216; 8 x 128 (256) 102 and
+  // 103, 8 x 300 of 14 over 2 of 64 (272) 96 and 70.
+  const int64_t many = (most_rows + kTileRows - 1) / kTileRows * p.batch * p.n_kv_heads;
+  const int rows = most_rows <= 8 ? 8 : many < 2 * kCus ? 16 : kTileRows;
   const int64_t all = std::max<int64_t>((most_rows + rows - 1) / rows, 1);
   // tiles past a launch's size take turns
   const int64_t tiles = std::min(all, std::max<int64_t>(1, (1 << 22) / ((int64_t)p.batch * p.n_kv_heads)));
@@ -477,8 +731,10 @@ void launch(const AttendArgs& a, int rows, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.row_tiles * a.p.batch * a.p.n_kv_heads), (unsigned)a.splits);
   if (rows == 8)
     hipLaunchKernelGGL((attend_fp4_kernel<E, D, 8>), grid, dim3(256), 0, stream, a);
-  else
+  else if (rows == 16)
     hipLaunchKernelGGL((attend_fp4_kernel<E, D, 16>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attend_fp4_tile_kernel<E, D>), grid, dim3(256), 0, stream, a);
   if (a.splits > 1) {
     hipLaunchKernelGGL((attend_join_kernel<E, D>), dim3((unsigned)(a.p.tokens * a.p.n_heads)), dim3(256),
                        0, stream, a);
