@@ -217,7 +217,7 @@ SIGNATURES = {
     "fcv_fp4_attention_workspace_bytes": (c_size_t, [POINTER(FcvFp4Attention)]),
     "fcv_fp4_attention": (c_int32, [POINTER(FcvFp4Attention), c_void_p, c_size_t, c_void_p]),
     "fcv_copy_pages": (c_int32, [c_void_p, c_int32, c_int64, c_int32, c_int64, c_int64,
-                                 POINTER(c_int32), POINTER(c_int32), c_int32, c_void_p]),
+                                 c_void_p, c_void_p, c_int32, c_void_p]),
 }
 
 STAGES = ("qkv", "attention", "out_proj", "ff1", "ff2", "ln_mod", "conv", "adaln", "in_proj",

@@ -28,7 +28,7 @@ struct Fp4Args {
 // workgroup has NT blocks of 16 rows of W and all rows of x (MT blocks of 16); its waves take turns in K, the
 // codes of kAhead spans asked for at once, and are summed through LDS.
 //
-// Bound: a CU takes in about 40 B/ns, and a workgroup reads all of x beside its rows of W: of 32 rows eight
+// Bound: a CU takes in about 48 B/ns, and a workgroup reads all of x beside its rows of W: of 32 rows eight
 // times what 16 rows of W are.  Hence NT, and K cut over workgroups (blockIdx.y, joined by
 // linear_join_kernel), where that leaves each CU less to read.
 constexpr int kFewN = 16, kFewWaves = 8, kSpan = 128;
@@ -504,8 +504,10 @@ int check(const FcvFp4Linear* p) {
 //   tiles of 64 x 64 23, by few rows 19.
 // Few rows, up to 32:  2.9 + what W takes, 3.5 TB/s from all CUs or 18 B/ns to one, + 21 ns for each KB of x
 //   that a CU reads.  In us by blocks of 16, 32 and 64 rows of W: 1 x 4096 x 4096 5.3, 7.2 and 11; 32 x 4096 x
-//   16384 39, 26 and 19; 32 x 4096 x 4096 12, 13 and 17, with K in 1, 2 and 4 ranges 12, 11 and 9.8.
-// A cut K adds the join's 1.8 and its sums' way, operands off their boundaries the pass that lays them out
+//   16384 39, 26 and 19; 32 x 4096 x 4096 11.8, 13.5 and 17.5, with K in 1, 2 and 4 ranges 11.8, 10.7 and 9.8.
+//   (x loaded in whole lines, W's words changing places between lanes instead: no faster.)
+// A cut K adds the join's 1.8 (3.5 to few rows: what the second launch takes of the host, which calls that
+// short wait for) and its sums' way, operands off their boundaries the pass that lays them out
 // (the same for every tile).
 enum Form { kFew, kTile64, kTile64x128, kTile128, kTile128x256, kTile256 };
 
@@ -533,7 +535,7 @@ int part_ld(int n) { return (n + 3) / 4 * 4; }
 int64_t groups_of(const FcvFp4Linear& p) { return (p.k + FCV_FP4_GROUP - 1) / FCV_FP4_GROUP; }
 
 float join_us(const FcvFp4Linear& p, int splits) {
-  return splits > 1 ? 1.8f + (float)p.m * (float)p.n * 8.0f * splits / 5.0e6f : 0.0f;
+  return splits > 1 ? (p.m <= kFewMost ? 3.5f : 1.8f) + (float)p.m * (float)p.n * 8.0f * splits / 5.0e6f : 0.0f;
 }
 
 Plan plan_of(const FcvFp4Linear& p) {

@@ -9,7 +9,7 @@ writes into the last, partly filled one, which is then copied.
 from __future__ import annotations
 
 import heapq
-from ctypes import c_int32
+from array import array
 
 import torch
 
@@ -40,14 +40,15 @@ def copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
             raise ValueError(f"a page's bytes must be contiguous, got strides {pages.stride()}")
         step *= n
     try:
-        lists = [(c_int32 * len(v))(*v) for v in (src, dst)]
+        lists = array("i", src), array("i", dst)
+    except OverflowError as e:
+        raise ValueError(f"a page is outside the pool of {n_pages}") from e
     except TypeError as e:
         raise ValueError(f"src and dst must be lists of page numbers: {e}") from e
-    if any(a != b for ints, v in zip(lists, (src, dst)) for a, b in zip(ints, v)):
-        raise ValueError(f"a page is outside the pool of {n_pages}")
     _launch(_lib.load().fcv_copy_pages, pages.device.index, pages.data_ptr(), layers,
             pages.stride(0) * size, n_pages, pages.stride(1) * size if n_pages > 1 else step * size,
-            step * size, lists[0], lists[1], len(src))
+            step * size, lists[0].buffer_info()[0],
+            lists[1].buffer_info()[0], len(src))
 
 
 class CachePages:

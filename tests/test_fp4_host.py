@@ -163,6 +163,31 @@ def test_workspaces_grow_with_the_call(fcv):
     assert attention(tokens=4096, batch=4096) == 0
 
 
+def _copy(fcv, src=(0, 1), dst=(2, 3), pages=BIG, layers=2, layer_stride=6400, n_pages=10, page_stride=640,
+          page_bytes=640, count=None):
+    a = (ctypes.c_int32 * len(src))(*src) if src is not None else None
+    b = (ctypes.c_int32 * len(dst))(*dst) if dst is not None else None
+    return fcv._lib.load().fcv_copy_pages(pages, layers, layer_stride, n_pages, page_stride, page_bytes, a, b,
+                                          len(src or dst) if count is None else count, None)
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(src=(0, 10)), "outside"), (dict(dst=(-1, 3)), "outside"), (dict(dst=(2, 2)), "page 2 is a destination twice"),
+    (dict(src=(0, 2)), "page 2 is both"), (dict(src=(5, 5), dst=(5, 6)), "both"), (dict(pages=None), "null pages"),
+    (dict(src=None), "null page lists"), (dict(dst=None), "null page lists"), (dict(count=-1), "negative"),
+    (dict(layers=-1), "negative"), (dict(layers=1 << 17), "65535"), (dict(page_stride=639), "pages overlap"),
+    (dict(layer_stride=639), "layers overlap"), (dict(layer_stride=1280), "layers overlap"),
+    (dict(page_bytes=1 << 40), "page_bytes"), (dict(page_stride=1 << 50), "too far"), (dict(n_pages=0), "outside")])
+def test_copy_pages_refuses(fcv, bad, match):
+    _refuse(fcv, _copy(fcv, **bad), match)
+
+
+def test_copies_of_nothing_launch_nothing(fcv):
+    assert _copy(fcv, src=(), dst=(), count=0, pages=None) == 0
+    assert _copy(fcv, layers=0, pages=None) == 0
+    assert _copy(fcv, page_bytes=0, pages=None) == 0
+
+
 def test_cpu_tensors_are_refused(fcv):
     x = torch.zeros(2, 64, dtype=torch.float16)
     codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
