@@ -49,6 +49,11 @@ __device__ __forceinline__ float across_max(float v) {  // over the lane blocks 
 }
 __device__ __forceinline__ float across_sum(float v) { return swap32_sum(swap16_sum(v)); }
 
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xF, 0xF, false);
+}
+
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
   typedef __bf16 b2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b});
@@ -353,6 +358,13 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
 // 128 rows of a sequence's key head to a workgroup, 32 to a wave (v_mfma_f32_32x32x16).  Each page's codes become
 // 16-bit numbers once, in LDS: keys [64][D], values [D][64] in the order of the S^T tiles' rows, so that a
 // lane's weights are its right operand again.  Two pages' room: one barrier a page.
+//
+// Bound: the matrix pipes (with two parts of a weight a page takes a wave 0.84 us, of which its 48 products
+// 0.82 at the clock the card holds under them).  Results in bf16 are off by 2^-8 from their rounding, and one
+// fp16 number, off by 2^-11, is all that their weights go in as here: times 2^kTop and their values' scales over
+// the largest of the pages so far (one below 2^-28 of that loses bits, one below 2^-39 is 0).  Weights of
+// fp16 results go in as two bf16 numbers as above.
+constexpr int kTop = 14;
 template <int D>
 __device__ __forceinline__ int key_chunk(int row, int c) {  // 16 rows read at one chunk touch all banks
   return D == 128 ? c ^ (row & 15) : c ^ ((row >> 1) & 7);
@@ -363,9 +375,12 @@ template <class E, int D>
 __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArgs a) {
   using P = Page<D>;
   constexpr int kRows = kTileRows, kSteps = D / 16, kDT = D / 32;
+  constexpr bool kOne = std::is_same<E, Bf16>::value;  // one fp16 number a weight
+  using V = typename std::conditional<kOne, Half, Bf16>::type;
   __shared__ __attribute__((aligned(16))) short sk[2][kPage * D];
   __shared__ __attribute__((aligned(16))) short sv[2][D * kPage];
   __shared__ __attribute__((aligned(16))) uint32_t svs[2][kPage / 4];
+  __shared__ int sunit[2];  // kOne: the scale byte that the page's are told over
   const FcvFp4Attention& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -417,6 +432,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
+    int unit = 0, my_unit = 0;  // of the pages so far, and of this wave's sums
 
     // a thread's share of a page: D / 4 codes of a key, 16 bytes of a byte row of the values
     uint32_t kw[D / 32], ks, vsw = 0;
@@ -439,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       if (tid < kPage / 4)
         vsw = *reinterpret_cast<const uint32_t*>(page + P::kValueScales + (uint32_t)tid * 4);
     };
-    auto unpack = [&](int buf) {
+    auto unpack = [&](int buf, int page, bool here) {
       const int key = tid / 4;
 #pragma unroll
       for (int j = 0; j < D / 32; ++j)
@@ -455,13 +471,34 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
           const uint32_t wo = (w0 >> 4 & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
           *reinterpret_cast<s16x8*>(
               &sv[buf][2 * pair * kPage + value_chunk(2 * pair, 2 * step + h) * 8]) =
-              fp4_octet<Bf16>(we, kHeld<E>);
+              fp4_octet<V>(we, kOne ? 1.0f : kHeld<E>);
           *reinterpret_cast<s16x8*>(
               &sv[buf][(2 * pair + 1) * kPage + value_chunk(2 * pair + 1, 2 * step + h) * 8]) =
-              fp4_octet<Bf16>(wo, kHeld<E>);
+              fp4_octet<V>(wo, kOne ? 1.0f : kHeld<E>);
         }
       }
-      if (tid < kPage / 4) svs[buf][tid % 2 * 8 + tid / 2] = vsw;
+      if (tid < kPage / 4) {
+        if constexpr (kOne) {  // 16 lanes of one row
+          const int left = here ? length - page * kPage - 4 * tid : 0;  // keys that are the sequence's
+          uint32_t byte[4], top = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            byte[j] = j < left ? vsw >> (8 * j) & 255 : 0;
+            top = max(top, byte[j] == 255 ? 0 : byte[j]);
+          }
+          top = max(top, dpp_u<0xB1>(top));
+          top = max(top, dpp_u<0x4E>(top));
+          top = max(top, dpp_u<0x141>(top));
+          top = max(top, dpp_u<0x140>(top));
+          unit = max(unit, (int)top);
+          vsw = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            vsw |= (byte[j] == 255 ? 255u : (uint32_t)max((int)byte[j] + 127 + kTop - unit, 0)) << (8 * j);
+          if (tid == 0) sunit[buf] = unit;
+        }
+        svs[buf][tid % 2 * 8 + tid / 2] = vsw;
+      }
     };
     auto take = [&](int page, int buf) {
       f32x16 s[2];
@@ -515,10 +552,19 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
 #pragma unroll
         for (int d = 0; d < kDT; ++d) o[d] *= alpha;
       }
+      if constexpr (kOne) {
+        const int now = __builtin_amdgcn_readfirstlane(sunit[buf]);
+        if (now > my_unit) {
+          const float f = scale_of((uint32_t)max(127 + my_unit - now, 0));
+#pragma unroll
+          for (int d = 0; d < kDT; ++d) o[d] *= f;
+          my_unit = now;
+        }
+      }
       const float base = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
       for (int st = 0; st < 4; ++st) {  // 16 keys: words 2 st and 2 st + 1 of the lane's eight
-        u32x4 hi, lo;
+        u32x4 hi, lo = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float w[2];
@@ -529,18 +575,23 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
             l += e;
             w[i] = e * scale_of((vs[g] >> (8 * j)) & 255);
           }
-          const uint32_t u = bf16_pair(w[0], w[1]);
-          hi[j] = u;
-          lo[j] = bf16_pair(w[0] - __uint_as_float(u << 16), w[1] - __uint_as_float(u & 0xffff0000u));
+          if constexpr (kOne) {
+            hi[j] = __builtin_bit_cast(uint32_t, f2h2(w[0], w[1]));
+          } else {
+            const uint32_t u = bf16_pair(w[0], w[1]);
+            hi[j] = u;
+            lo[j] = bf16_pair(w[0] - __uint_as_float(u << 16), w[1] - __uint_as_float(u & 0xffff0000u));
+          }
         }
-        const s16x8 ph = __builtin_bit_cast(s16x8, hi), pl = __builtin_bit_cast(s16x8, lo);
+        const s16x8 ph = __builtin_bit_cast(s16x8, hi);
+        [[maybe_unused]] const s16x8 pl = __builtin_bit_cast(s16x8, lo);
 #pragma unroll
         for (int d = 0; d < kDT; ++d) {
           const int r = 32 * d + fr;
           const s16x8 v =
               *reinterpret_cast<const s16x8*>(&sv[buf][r * kPage + value_chunk(r, 2 * st + fh) * 8]);
-          o[d] = Bf16::mfma32(v, ph, o[d]);
-          o[d] = Bf16::mfma32(v, pl, o[d]);
+          o[d] = V::mfma32(v, ph, o[d]);
+          if constexpr (!kOne) o[d] = V::mfma32(v, pl, o[d]);
         }
       }
     };
@@ -555,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       for (int page = page0; page < page1; ++page) {
         const int buf = (page - page0) & 1;
         const int after = number(page + 2);
-        unpack(buf);
+        unpack(buf, page, id >= 0);
         __syncthreads();
         load(next);
         if (id >= 0 && page * kPage < reach) take(page, buf);
@@ -564,6 +615,11 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       }
     }
     l = swap32_sum(l);
+    if constexpr (kOne) {  // back to the units of the other kernel's sums
+      const float f = scale_of((uint32_t)my_unit) * (kHeld<E> / (1 << kTop));
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) o[d] *= f;
+    }
     if (there) {
       const int64_t at = (int64_t)(first + token) * p.n_heads + head;
       if (a.splits > 1) {

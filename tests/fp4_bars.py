@@ -21,6 +21,16 @@ def attention(out, mass, score, keys, dim, dtype):
     return (err + bars.rounding(out.abs() + err, dtype)) * (1 + 2 ** -8)
 
 
+def attention_one(out, mass, score, keys, dim, v_max):
+    """bf16 by tiles of 128 rows: a weight times its value's scale goes in as one fp16 number, off by 2^-11 of
+    it at most.  They are held at 2^14 over the largest scale so far, so one that fp16's normal numbers do not
+    reach is off by 2^-25 / 2^14 = 2^-39 of that scale, times a number of 6 at most; the largest scale's
+    group holds a value of 3.5 of it, so 2^-39 6 / 3.5 < 2^-38 of the largest value, for each key."""
+    score, keys = score[..., None], keys[..., None]
+    err = (2.0 ** -11 + 2 * ((dim + 4) * score + 8 + keys + 72) * U) * mass + keys * 2.0 ** -38 * v_max
+    return (err + bars.rounding(out.abs() + err, torch.bfloat16)) * (1 + 2 ** -8)
+
+
 def random_pages(n, heads, d, seed=0, dtype=torch.bfloat16, scale=1.0):
     """A pool whose bytes are those of normal keys and values, on the CPU."""
     g = torch.Generator().manual_seed(seed)
