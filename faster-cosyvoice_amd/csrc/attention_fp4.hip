@@ -357,14 +357,28 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
 //
 // 128 rows of a sequence's key head to a workgroup, 32 to a wave (v_mfma_f32_32x32x16).  Each page's codes become
 // 16-bit numbers once, in LDS: keys [64][D], values [D][64] in the order of the S^T tiles' rows, so that a
-// lane's weights are its right operand again.  Two pages' room: one barrier a page.
+// lane's weights are its right operand again.  Two pages' room: one barrier a page, with the next page's
+// conversions beside this one's first product, and a step's weights between the products of the one before.
+// m follows a row's maximum only where it has risen by kSlack (a power of two: weights up to 2^1.75), so that
+// few pages scale the sums; the other tiles' m is the maximum.
 //
-// Bound: the matrix pipes (with two parts of a weight a page takes a wave 0.84 us, of which its 48 products
-// 0.82 at the clock the card holds under them).  Results in bf16 are off by 2^-8 from their rounding, and one
-// fp16 number, off by 2^-11, is all that their weights go in as here: times 2^kTop and their values' scales over
-// the largest of the pages so far (one below 2^-28 of that loses bits, one below 2^-39 is 0).  Weights of
-// fp16 results go in as two bf16 numbers as above.
+// Bound: instructions.  8 texts of 300 behind 500 to 3000 keys, 32 heads of 128 over 8, run at 0.57 PFLOP/s
+// (bf16, 168 us; 0.53 in fp16): the matrix pipes are busy for two fifths of it, and some 600 other instructions
+// to a wave's page take their turns with the products of the CU's other workgroup.
+//
+// bf16.  Results are off by 2^-8 from their rounding, and one fp16 number, off by 2^-11, is all that a weight
+// times its value's scale goes in as, times 2^kTop and over 2^u (u as a scale byte): one below 2^-28 of
+// 2^u loses bits, one below 2^-39 is 0.  u is the row's, and as large as the page's largest scale, or as the
+// row's largest product of a weight and a scale with kRoom over it where that is less: values that a row hides, or
+// weighs next to nothing, cost the others no bit, however large.  A row's u follows its m's rise (`owed`) once
+// that is more than kRoom.  LDS holds the scales over the largest scale of all pages so far; the factor
+// between the two goes into the exponent, and out of l's terms again.
+// fp16.  Weights go in as two bf16 numbers as above.
+//
+// A value without a scale (its byte is 255) lies in LDS as zeros, and rows that see it become NaN at their end.
 constexpr int kTop = 14;
+constexpr float kSlack = 1.75f;
+constexpr int kRoom = 8;
 template <int D>
 __device__ __forceinline__ int key_chunk(int row, int c) {  // 16 rows read at one chunk touch all banks
   return D == 128 ? c ^ (row & 15) : c ^ ((row >> 1) & 7);
@@ -379,8 +393,9 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
   using V = typename std::conditional<kOne, Half, Bf16>::type;
   __shared__ __attribute__((aligned(16))) short sk[2][kPage * D];
   __shared__ __attribute__((aligned(16))) short sv[2][D * kPage];
-  __shared__ __attribute__((aligned(16))) uint32_t svs[2][kPage / 4];
-  __shared__ int sunit[2];  // kOne: the scale byte that the page's are told over
+  __shared__ __attribute__((aligned(16))) f32x4 svs[2][2][kPage / 8];  // the values' scales, by half waves
+  // of a page: the scale byte that its values' are told over (kOne), and which keys' values have no scale
+  __shared__ __attribute__((aligned(16))) uint32_t about[2][4];
   const FcvFp4Attention& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -407,13 +422,13 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
   const int tiles = (rows + kRows - 1) / kRows;
   for (int t0 = turn; t0 < tiles; t0 += a.row_tiles) {
     const int row0 = (tiles - 1 - t0) * kRows;
-    const int mine = row0 + 32 * wave;  // the wave's first row
-    const bool there = mine + fr < rows;
-    const int row = min(mine + fr, rows - 1);
+    const int row1 = row0 + 32 * wave;  // the wave's first row
+    const bool there = row1 + fr < rows;
+    const int row = min(row1 + fr, rows - 1);
     const int token = row / a.group, head = kv * a.group + row - token * a.group;
     const int limit = there ? length - n + token + 1 : 0;  // the row's visible keys
     auto sees = [&](int r) { return min(max(length - n + min(r, rows - 1) / a.group + 1, 0), length); };
-    const int reach = mine < rows ? sees(mine + 31) : 0;   // of the wave
+    const int reach = row1 < rows ? sees(row1 + 31) : 0;   // of the wave
     const int all_pages = (sees(row0 + kRows - 1) + kPage - 1) / kPage;
     const int page0 = blockIdx.y * a.pages_per;
     int page1 = min(page0 + a.pages_per, all_pages);
@@ -432,7 +447,9 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
-    int unit = 0, my_unit = 0;  // of the pages so far, and of this wave's sums
+    float poison = 1.0f;  // or NaN, of the row
+    float owed = 0.0f;
+    int unit = 0, mine = 1;     // kOne: the largest scale byte of the pages so far, and that of the row's sums
 
     // a thread's share of a page: D / 4 codes of a key, 16 bytes of a byte row of the values
     uint32_t kw[D / 32], ks, vsw = 0;
@@ -477,61 +494,90 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
               fp4_octet<V>(wo, kOne ? 1.0f : kHeld<E>);
         }
       }
-      if (tid < kPage / 4) {
-        if constexpr (kOne) {  // 16 lanes of one row
+      if (tid < kPage / 4) {  // 16 lanes of one row, four keys each
+        int byte[4];
+        uint32_t bad[4];  // the lanes whose j-th key has no scale
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          byte[j] = vsw >> (8 * j) & 255;
+          bad[j] = (uint32_t)__ballot(byte[j] == 255);
+          byte[j] = byte[j] == 255 ? 0 : byte[j];
+        }
+        if constexpr (kOne) {
           const int left = here ? length - page * kPage - 4 * tid : 0;  // keys that are the sequence's
-          uint32_t byte[4], top = 0;
+          uint32_t top = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            byte[j] = j < left ? vsw >> (8 * j) & 255 : 0;
-            top = max(top, byte[j] == 255 ? 0 : byte[j]);
+            if (j >= left) byte[j] = 0;
+            top = max(top, (uint32_t)byte[j]);
           }
           top = max(top, dpp_u<0xB1>(top));
           top = max(top, dpp_u<0x4E>(top));
           top = max(top, dpp_u<0x141>(top));
           top = max(top, dpp_u<0x140>(top));
           unit = max(unit, (int)top);
-          vsw = 0;
+          if (tid == 0) about[buf][3] = top;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            vsw |= (byte[j] == 255 ? 255u : (uint32_t)max((int)byte[j] + 127 + kTop - unit, 0)) << (8 * j);
-          if (tid == 0) sunit[buf] = unit;
+          for (int j = 0; j < 4; ++j) byte[j] = max(byte[j] + 127 + kTop - unit, 0);
         }
-        svs[buf][tid % 2 * 8 + tid / 2] = vsw;
+        if (tid == 0)
+          for (int j = 0; j < 3; ++j)
+            about[buf][j] = j == 0 ? (uint32_t)unit : bad[2 * j - 2] | bad[2 * j - 1] << 16;
+        svs[buf][tid % 2][tid / 2] =
+            f32x4{scale_of(byte[0]), scale_of(byte[1]), scale_of(byte[2]), scale_of(byte[3])};
       }
     };
-    auto take = [&](int page, int buf) {
-      f32x16 s[2];
+    f32x16 s[2];
+    s16x8 kf[2][2];  // the keys' fragments of four steps
+    auto load_kf = [&](int buf, int j) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int key = 32 * t + fr;
+        kf[j % 2][t] =
+            *reinterpret_cast<const s16x8*>(&sk[buf][key * D + key_chunk<D>(key, 2 * j + fh) * 8]);
+      }
+    };
+    auto scores = [&](int buf) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j)
+      for (int j = 0; j < kSteps; ++j) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int key = 32 * t + fr;
-          s[t] = E::mfma32(
-              *reinterpret_cast<const s16x8*>(&sk[buf][key * D + key_chunk<D>(key, 2 * j + fh) * 8]), fq[j],
-              s[t]);
-        }
-      // the scales of the lane's keys: 8 g + 4 fh + j in byte j of word g
-      uint32_t vs[8];
-      {
-        const u32x4 v0 = *reinterpret_cast<const u32x4*>(&svs[buf][fh * 8]);
-        const u32x4 v1 = *reinterpret_cast<const u32x4*>(&svs[buf][fh * 8 + 4]);
-#pragma unroll
-        for (int g = 0; g < 8; ++g) vs[g] = g < 4 ? v0[g % 4] : v1[g % 4];
+        for (int t = 0; t < 2; ++t) s[t] = E::mfma32(kf[j % 2][t], fq[j], s[t]);
+        if (j + 2 < kSteps) load_kf(buf, j + 2);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (!__all(limit >= (page + 1) * kPage)) {  // hidden keys: no score, and a scale that is a number
+    };
+    auto take = [&](int page, int buf) {
+      s16x8 vf[2][kDT];
+      auto load_vf = [&](int st) {
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) {
+          const int r = 32 * d + fr;
+          vf[st & 1][d] =
+              *reinterpret_cast<const s16x8*>(&sv[buf][r * kPage + value_chunk(r, 2 * st + fh) * 8]);
+        }
+      };
+      const u32x4 facts = *reinterpret_cast<const u32x4*>(about[buf]);
+      if (!__all(limit >= (page + 1) * kPage)) {  // hidden keys have no score
+        asm volatile("");  // a branch: the compiler would do this for every page
         const int seen = limit - page * kPage - 4 * fh;
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
+        for (int g = 0; g < 8; ++g)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (8 * g + j >= seen) s[g / 4][g % 4 * 4 + j] = -__builtin_inff();
-          const int k = min(max(seen - 8 * g, 0), 4);
-          vs[g] &= k == 4 ? ~0u : (1u << (8 * k)) - 1;
+      }
+      const uint32_t bad = __builtin_amdgcn_readfirstlane(facts[1] | facts[2]);
+      if (bad != 0) {  // a value without a scale is in LDS as zeros: NaN for the rows that see it
+        const int seen = limit - page * kPage;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lanes = facts[1 + j / 2] >> (16 * (j % 2)) & 0xffffu;
+          const int n = min(max((seen - j + 3) >> 2, 0), 16);
+          if (lanes & ((1u << n) - 1)) poison = __builtin_nanf("");
         }
       }
       float top = -__builtin_inff();
@@ -544,27 +590,62 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
                                                         false);
         top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * scale;
       }
-      if (__any(top > m)) {
+      float shrink = 1.0f;  // of the sums
+      if (__any(top > m + kSlack)) {
         const float next = fmaxf(m, top);
-        const float alpha = next == -__builtin_inff() ? 1.0f : hw_exp2(m - next);
+        const float rise = next == -__builtin_inff() ? 0.0f : next - m;
         m = next;
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < kDT; ++d) o[d] *= alpha;
-      }
-      if constexpr (kOne) {
-        const int now = __builtin_amdgcn_readfirstlane(sunit[buf]);
-        if (now > my_unit) {
-          const float f = scale_of((uint32_t)max(127 + my_unit - now, 0));
-#pragma unroll
-          for (int d = 0; d < kDT; ++d) o[d] *= f;
-          my_unit = now;
+        l *= hw_exp2(-rise);
+        float down = 0.0f;
+        if constexpr (kOne) {
+          owed += fminf(rise, 256.0f);
+          if (owed > kRoom) {
+            const int was = mine;
+            mine = min(mine, max(mine - (int)owed, max((int)facts[0] - 125, 1)));
+            down = (float)(was - mine);
+            owed = 0.0f;
+          }
         }
+        shrink = hw_exp2(down - rise);
       }
-      const float base = m == -__builtin_inff() ? 0.0f : m;
+      float base = m == -__builtin_inff() ? 0.0f : m, back = 1.0f;  // back: out of l's terms
+      if constexpr (kOne) {
+        const int all = __builtin_amdgcn_readfirstlane(facts[0]);
+        const int here = __builtin_amdgcn_readfirstlane(facts[3]);
+        if (__any(max(here, all - 125) > mine && m > -__builtin_inff())) {
+          // the row's largest weight with its value's scale, as a scale byte
+          float most = -__builtin_inff();
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {  // 16 keys: words 2 st and 2 st + 1 of the lane's eight
-        u32x4 hi, lo = {0, 0, 0, 0};
+          for (int g = 0; g < 8; ++g) {
+            const f32x4 v = svs[buf][fh][g];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float byte = (float)(__float_as_uint(v[j]) >> 23);
+              most = fmaxf(most, fmaf(s[g / 4][g % 4 * 4 + j], scale, byte));
+            }
+          }
+          const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false,
+                                                          false);
+          most = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) - base + (all - 127 - kTop);
+          const int want = min(here, (int)fmaxf(most, -512.0f) + kRoom), was = mine;
+          mine = max(max(mine, want), all - 125);
+          owed = mine > was ? 0.0f : owed;
+          shrink *= scale_of((uint32_t)max(127 + was - mine, 0));
+        }
+        // the weights' scales are over `all`: 2^(all - mine) goes in through the exponent, and out of l's
+        base -= (float)(all - mine);
+        back = hw_exp2((float)(mine - all));
+      }
+      if (__any(shrink != 1.0f)) {
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) o[d] *= shrink;
+      }
+      u32x4 hi[2], lo[2];
+      auto weights = [&](int st) {  // of 16 keys: words 2 st and 2 st + 1 of the lane's eight
+        // the scales of the lane's keys: 8 g + 4 fh + j is element j of vs[g % 2]
+        f32x4 vs[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) vs[i] = svs[buf][fh][2 * st + i];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float w[2];
@@ -572,27 +653,40 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
           for (int i = 0; i < 2; ++i) {
             const int g = 2 * st + i;
             const float e = hw_exp2(fmaf(s[g / 4][g % 4 * 4 + j], scale, -base));
-            l += e;
-            w[i] = e * scale_of((vs[g] >> (8 * j)) & 255);
+            l = kOne ? fmaf(e, back, l) : l + e;
+            w[i] = e * vs[i][j];
           }
           if constexpr (kOne) {
-            hi[j] = __builtin_bit_cast(uint32_t, f2h2(w[0], w[1]));
+            hi[st & 1][j] = __builtin_bit_cast(uint32_t, f2h2(w[0], w[1]));
           } else {
             const uint32_t u = bf16_pair(w[0], w[1]);
-            hi[j] = u;
-            lo[j] = bf16_pair(w[0] - __uint_as_float(u << 16), w[1] - __uint_as_float(u & 0xffff0000u));
+            hi[st & 1][j] = u;
+            lo[st & 1][j] =
+                bf16_pair(w[0] - __uint_as_float(u << 16), w[1] - __uint_as_float(u & 0xffff0000u));
           }
         }
-        const s16x8 ph = __builtin_bit_cast(s16x8, hi);
-        [[maybe_unused]] const s16x8 pl = __builtin_bit_cast(s16x8, lo);
+      };
+      load_vf(0);
+      weights(0);
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        if (st < 3) load_vf(st + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        // this step's products, and between them the next one's weights
 #pragma unroll
         for (int d = 0; d < kDT; ++d) {
-          const int r = 32 * d + fr;
-          const s16x8 v =
-              *reinterpret_cast<const s16x8*>(&sv[buf][r * kPage + value_chunk(r, 2 * st + fh) * 8]);
-          o[d] = V::mfma32(v, ph, o[d]);
-          if constexpr (!kOne) o[d] = V::mfma32(v, pl, o[d]);
+          o[d] = V::mfma32(vf[st & 1][d], __builtin_bit_cast(s16x8, hi[st & 1]), o[d]);
+          if constexpr (!kOne) o[d] = V::mfma32(vf[st & 1][d], __builtin_bit_cast(s16x8, lo[st & 1]), o[d]);
         }
+        if (st < 3) {
+          weights(st + 1);
+#pragma unroll
+          for (int i = 0; i < (kOne ? 1 : 2) * kDT; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+            __builtin_amdgcn_sched_group_barrier(0x002, (kOne ? 36 : 60) / ((kOne ? 1 : 2) * kDT), 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
 
@@ -603,20 +697,28 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       };
       int id = number(page0), next = number(page0 + 1);
       load(id);
+      unpack(0, page0, id >= 0);
+      load(next);
       for (int page = page0; page < page1; ++page) {
         const int buf = (page - page0) & 1;
         const int after = number(page + 2);
-        unpack(buf, page, id >= 0);
-        __syncthreads();
-        load(next);
-        if (id >= 0 && page * kPage < reach) take(page, buf);
+        __syncthreads();  // this page is in LDS, and every wave is through with the one before
+        const bool sees_it = id >= 0 && page * kPage < reach;
+        if (sees_it)
+          for (int j = 0; j < 2; ++j) load_kf(buf, j);
+        unpack(buf ^ 1, page + 1, next >= 0);
+        load(after);
+        if (sees_it) {
+          scores(buf);
+          take(page, buf);
+        }
         id = next;
         next = after;
       }
     }
     l = swap32_sum(l);
-    if constexpr (kOne) {  // back to the units of the other kernel's sums
-      const float f = scale_of((uint32_t)my_unit) * (kHeld<E> / (1 << kTop));
+    {  // back to the units of the other kernel's sums
+      const float f = poison * (kOne ? scale_of((uint32_t)mine) * (kHeld<E> / (1 << kTop)) : 1.0f);
 #pragma unroll
       for (int d = 0; d < kDT; ++d) o[d] *= f;
     }
@@ -758,11 +860,12 @@ struct Plan {
 Plan plan_of(const FcvFp4Attention& p) {
   const int group = p.n_heads / p.n_kv_heads;
   const int64_t most_rows = (int64_t)std::min(p.max_q, p.tokens) * group;
-  // Tiles of 128 rows where they give every CU two workgroups: 4000 tokens of 32 heads of 128 over 8 (1000
-  // tiles) take 225 us by them, 304 by 16 rows; 8 x 300 behind a cache (640) 196 and 216; 8 x 128 (256) 102 and
-  // 103, 8 x 300 of 14 over 2 of 64 (272) 96 and 70.
+  // Tiles of 128 rows where they fill the card, which takes more of heads of 64, whose pages are short.  Heads of
+  // 128, 32 over 8, by tiles of 128 and of 16 rows: 4000 tokens (1000 tiles) 176 and 304 us, 2000 (500) 63 and
+  // 98, 8 x 128 behind a cache (256) 80 and 98, 1000 (250) 34 and 36, 4 x 128 (128) 79 and 54.  Heads of 64,
+  // 14 over 2: 7000 (766) 161 and 229, 16 x 300 (544) 112 and 106, 8 x 300 (272) 77 and 64, 2000 (220) 52 and 28.
   const int64_t many = (most_rows + kTileRows - 1) / kTileRows * p.batch * p.n_kv_heads;
-  const int rows = most_rows <= 8 ? 8 : many < 2 * kCus ? 16 : kTileRows;
+  const int rows = most_rows <= 8 ? 8 : many < (p.head_dim == 128 ? kCus : 5 * kCus / 2) ? 16 : kTileRows;
   const int64_t all = std::max<int64_t>((most_rows + rows - 1) / rows, 1);
   // tiles past a launch's size take turns
   const int64_t tiles = std::min(all, std::max<int64_t>(1, (1 << 22) / ((int64_t)p.batch * p.n_kv_heads)));
@@ -775,7 +878,26 @@ Plan plan_of(const FcvFp4Attention& p) {
   // in ranges of 4, 8 and 16 pages 8.2, 8.8 and 10.6.
   // Up to 16 pages one range: it costs a microsecond there (8.5 instead of 7.6 for 600 keys) and saves a launch.
   const int64_t want = pages <= 16 ? 1 : std::max<int64_t>(1, 2 * kCus / blocks);
-  const int per = (int)std::max<int64_t>((pages + want - 1) / want, 4);
+  int per = (int)std::max<int64_t>((pages + want - 1) / want, 4);
+  if (rows == kTileRows) {
+    // Time in pages of a workgroup that shares its CU; one that has it alone takes 0.63 of it, and a tile's
+    // sums of one range cost 0.02.  8 x 128 tokens of 32 heads of 128 over 8 (256 tiles) behind 16000 keys take
+    // 410 us in one range, 331, 343 and 353 in two, three and four, behind 4000 keys 110 and 113; 10 x 128 (320)
+    // behind 8000 288, 264 and 249; 500 tiles behind 8000 273 and 308, 640 behind 16000 906, 805 and 838.
+    // Tiles whose keys are new ones too have lengths of their own, and the short ones fill the ends.
+    const int most_ranges = p.max_q <= p.max_length / 2 ? 3 : 1;
+    double best = 0.0;
+    for (int s = 1; s <= most_ranges; ++s) {
+      const int64_t n = blocks * s, rest = n % (2 * kCus);
+      const int each = (pages + s - 1) / s;
+      const double time = each * (n / (2 * kCus) + (rest == 0 ? 0.0 : rest <= kCus ? 0.63 : 1.0)) +
+                          (s > 1 ? 0.02 * n : 0.0);
+      if (s == 1 || time < best) {
+        best = time;
+        per = each;
+      }
+    }
+  }
   return Plan{rows, tiles, (pages + per - 1) / per, per};
 }
 

@@ -21,13 +21,16 @@ def attention(out, mass, score, keys, dim, dtype):
     return (err + bars.rounding(out.abs() + err, dtype)) * (1 + 2 ** -8)
 
 
-def attention_one(out, mass, score, keys, dim, v_max):
+def attention_one(out, mass, score, keys, dim, v_max, reach):
     """bf16 by tiles of 128 rows: a weight times its value's scale goes in as one fp16 number, off by 2^-11 of
-    it at most.  They are held at 2^14 over the largest scale so far, so one that fp16's normal numbers do not
-    reach is off by 2^-25 / 2^14 = 2^-39 of that scale, times a number of 6 at most; the largest scale's
-    group holds a value of 3.5 of it, so 2^-39 6 / 3.5 < 2^-38 of the largest value, for each key."""
+    it at most.  They are held at 2^14 over a scale 2^u, so one that fp16's normal numbers do not reach is off
+    by 2^-25 / 2^14 = 2^-39 of 2^u, times a number of 6 at most.  2^u is at most the largest scale of the keys
+    and, with `reach` the largest product of a weight and a value among those that the row sees, 2^17 of the
+    largest weight times scale; a scale's group holds a value of 3.5 of it.  So for each key
+    it is 2^-39 6 / 3.5 < 2^-38 of the largest value, and 2^-21 of `reach`."""
     score, keys = score[..., None], keys[..., None]
-    err = (2.0 ** -11 + 2 * ((dim + 4) * score + 8 + keys + 72) * U) * mass + keys * 2.0 ** -38 * v_max
+    least = torch.minimum(2.0 ** -38 * v_max, 2.0 ** -21 * reach[..., None])
+    err = (2.0 ** -11 + 2 * ((dim + 4) * score + 8 + keys + 72) * U) * mass + keys * least
     return (err + bars.rounding(out.abs() + err, torch.bfloat16)) * (1 + 2 ** -8)
 
 

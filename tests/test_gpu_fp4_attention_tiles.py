@@ -43,7 +43,8 @@ def compare(out, lse, st, what=""):
             p = torch.softmax(s, 1).nan_to_num(0)
             want, mass = p @ v[:, g], p @ v[:, g].abs()
             if st["q"].dtype == torch.bfloat16:
-                tol = fp4_bars.attention_one(want, mass, size, count.double(), d, v[:, g].abs().max())
+                tol = fp4_bars.attention_one(want, mass, size, count.double(), d, v[:, g].abs().max(),
+                                             (p * v[:, g].abs().amax(1)).amax(1))
             else:
                 tol = fp4_bars.attention(want, mass, size, count.double(), d, st["q"].dtype)
             lm_bars.assert_within(out[rows, h], want, tol, f"{what} {b} {h}")
@@ -120,3 +121,60 @@ def test_nan_in_place_and_rows_behind(fcv):
     assert bool(nan[494:600, 3].all()) and int(nan.sum()) == 106 * 128
     same = ~nan
     assert torch.equal(got[:3200][same], want[:3200][same])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("step", [1.0, 1.5, -1.0])
+def test_scores_that_rise_page_by_page(fcv, dtype, d, step):
+    """Every page's largest score a little above, or below, that of the one before."""
+    g = torch.Generator().manual_seed(3)
+    st = make([260] * 12, [320] * 12, 16, 16, d, dtype)
+    n = st["pages"].shape[0]
+    k = torch.randn(n, 16, F.PAGE, d, generator=g) / 4
+    v = torch.randn(n, 16, F.PAGE, d, generator=g)
+    for b in range(12):
+        for i in range(5):
+            k[st["table"][b, i], ..., 0] = step * i
+    st["pages"] = fp4_bars.pack(k, v, dtype)
+    st["q"][..., 0] = d ** 0.5
+    compare(*run(fcv, st, return_lse=True), st, f"rising {step}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_without_a_scale(fcv, dtype, d):
+    """NaN for the rows that see the key, also where its weight vanishes; nothing for the others."""
+    st = make([200] * 16, [200] * 16, 16, 16, d, dtype)
+    want = run(fcv, st)
+    sees = torch.zeros(3200, 16, dtype=torch.bool)
+    for b, head, key in ((0, 0, 0), (1, 3, 63), (2, 5, 64), (2, 7, 94), (2, 7, 129), (15, 15, 199), (9, 2, 190)):
+        st["pages"][st["table"][b, key // 64], head].view(-1)[-F.PAGE + key % 64] = 255
+        sees[200 * b + key:200 * b + 200, head] = True
+    got = run(fcv, st)
+    assert torch.equal(got.isnan().all(-1).cpu(), sees) and torch.equal(got.isnan().any(-1).cpu(), sees)
+    assert torch.equal(got.cpu()[~sees], want.cpu()[~sees])
+
+
+def test_huge_values_do_not_touch_others(fcv):
+    """Values of 2^100 that a row does not see, or sees with a weight of next to nothing; such ones in front of
+    the ones that count, behind them and in one page with them."""
+    d = 64
+    st = make([200] * 16, [330] * 16, 16, 16, d, torch.bfloat16)
+    g = torch.Generator().manual_seed(5)
+    n = st["pages"].shape[0]
+    k = torch.randn(n, 16, F.PAGE, d, generator=g)
+    v = torch.randn(n, 16, F.PAGE, d, generator=g)
+    k[..., 0] = 0
+    st["q"][..., 0] = d ** 0.5
+    for b in range(16):
+        for key in ((140,), (329,), (131, 200, 330 - 66), tuple(range(192, 256)))[b % 4]:
+            v[st["table"][b, key // 64], :, key % 64] *= 2.0 ** 100
+            if b % 8 >= 4:
+                k[st["table"][b, key // 64], :, key % 64, 0] = -192.0  # a weight of some 2^-277
+        if b >= 12:
+            for key in (0, 5, 70):
+                v[st["table"][b, key // 64], :, key % 64] *= 2.0 ** 110
+                k[st["table"][b, key // 64], :, key % 64, 0] = -160.0
+    st["pages"] = fp4_bars.pack(k, v, torch.bfloat16)
+    compare(*run(fcv, st, return_lse=True), st, "huge")
