@@ -25,7 +25,8 @@ namespace {
 
 constexpr int kPage = FCV_FP4_PAGE;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// bf16's values are held at 2^-24 times their size: sums of 2^24 of its largest values do not pass fp32's.
+// bf16's values are held at 2^-24 times their size: sums of 2^24 of its largest values do not pass fp32's.  What
+// that costs are bits of results below 2^-64.
 template <class E>
 constexpr float kHeld = std::is_same<E, Bf16>::value ? 0x1p-24f : 1.0f;
 
@@ -174,6 +175,11 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
 #pragma unroll
         for (int j = 0; j < kJ; ++j) s[t] = E::mfma16(fp4_octet<E>(r.k[t][j], ks), fq[j], s[t]);
         __builtin_amdgcn_sched_barrier(0);  // conversions of one tile at a time: registers
+      }
+      if (!there) {  // whatever the queries hold
+        asm volatile("");
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
     };
     // `masked`: some rows do not see all of the page's keys
@@ -717,10 +723,11 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       }
     }
     l = swap32_sum(l);
-    {  // back to the units of the other kernel's sums
-      const float f = poison * (kOne ? scale_of((uint32_t)mine) * (kHeld<E> / (1 << kTop)) : 1.0f);
+    {  // back to the units of the other kernel's sums, in two steps that do not leave fp32's range
+      const float f = kOne ? poison * (kHeld<E> / (1 << kTop)) : poison;
+      const float g = kOne ? scale_of((uint32_t)mine) : 1.0f;
 #pragma unroll
-      for (int d = 0; d < kDT; ++d) o[d] *= f;
+      for (int d = 0; d < kDT; ++d) o[d] = o[d] * f * g;
     }
     if (there) {
       const int64_t at = (int64_t)(first + token) * p.n_heads + head;

@@ -160,7 +160,8 @@ int fcv_fp4_read(const FcvFp4Read* args, hipStream_t stream);
  * rows for every sequence.  max_q and max_length bound the new tokens and the keys of a sequence: they
  * shape the launch, and a batch that passes them is computed all the same, more slowly.  Pages may be
  * shared between sequences.  tokens * n_heads is below 2^24, n_pages at most 2^24.  Numbers of the
- * pages are rounded to q's type (exact within the limits above for pages written in that type). */
+ * pages are rounded to q's type (exact within the limits above for pages written in that type); results
+ * below 2^-64 lose bits, because sums of bf16's largest values have to fit fp32. */
 typedef struct FcvFp4Attention {
   const void* q;          /* [tokens][n_heads][head_dim], strides q_row, q_head */
   const uint8_t* pages;

@@ -305,3 +305,18 @@ def test_refusals(fcv):
     buf = torch.zeros(3, 8, 64, dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError, match="out overlaps q"):
         call(q=buf[:2], out=buf[1:])
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [5, 1, 9], [700, 300, 600]])
+@pytest.mark.parametrize("d", [64, 128])
+def test_queries_without_numbers_and_without_pages(fcv, news, d):
+    """A padded slot: no page behind its length, and whatever its queries hold."""
+    st = make(news, [1000] * 3, 16, 4, d, torch.bfloat16)
+    clean = run(fcv, st)
+    st["table"][1] = -1
+    first, end = st["cu_q"][1:3].tolist()
+    st["q"][first:end, 0::2] = math.nan
+    st["q"][first:end, 1::2] = math.inf
+    out, lse = run(fcv, st, return_lse=True)
+    assert bool((out[first:end] == 0).all()) and bool((lse[first:end] == -math.inf).all())
+    assert torch.equal(out[:first], clean[:first]) and torch.equal(out[end:], clean[end:])
