@@ -262,3 +262,18 @@ def test_refusals(fcv):
     with pytest.raises(ValueError, match="out overlaps codes"):
         f(x, flat[:4 * 48].view(4, 48), s[:4],
           out=flat[16:16 + 32].view(torch.float16).view(4, 4))
+
+
+@pytest.mark.parametrize("m", [3, 40, 300, 1100])
+def test_rows_of_weights_far_apart(fcv, m):
+    """The largest row strides: a tile's offsets pass 2^31."""
+    n, k = 300, 256
+    x, c, s, b, _ = make(m, k, n, torch.bfloat16, bias=torch.bfloat16)
+    far = torch.empty(300 * 2 ** 24, dtype=torch.uint8, device=DEV)
+    codes = far.as_strided((n, 128), (2 ** 24 - 16, 1))
+    codes.copy_(c)
+    want = fcv.fused_linear_fp4(x, c, s, b)
+    assert torch.equal(fcv.fused_linear_fp4(x, codes, s, b), want)
+    scales = far.as_strided((n, 8), (2 ** 24 - 4, 1))
+    scales.copy_(s)
+    assert torch.equal(fcv.fused_linear_fp4(x, c, scales, b), want)

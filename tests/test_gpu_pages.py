@@ -133,3 +133,36 @@ def test_book(fcv):
     assert all(max(book.table([s])[0].tolist()) < used for s in truth)
     write(other, 60)
     look()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_offsets_that_pass_32_bits(fcv, d):
+    """Pages and heads gigabytes apart: every operator as over a dense pool."""
+    hk, hq, n = 2, 8, 6
+    g = torch.Generator().manual_seed(d)
+    dense = fcv.new_fp4_pages(n, hk, d, device=DEV)
+    size = dense.shape[2]
+    flat = torch.empty(5 * 2 ** 30 + 2 ** 29 + size, dtype=torch.uint8, device=DEV)
+    far = flat.as_strided((n, hk, size), (2 ** 30, 2 ** 29, 1))
+    far.zero_()
+    tokens = 300
+    qkv = torch.randn(tokens, (hq + 2 * hk) * d, generator=g).to(DEV, torch.bfloat16)
+    rows = (torch.randperm(n * 64, generator=g)[:tokens]).int().to(DEV)
+    angle = torch.rand(tokens, d // 2, generator=g).to(DEV)
+    cos, sin = angle.cos(), angle.sin()
+    pos = torch.arange(tokens, dtype=torch.int32, device=DEV)
+    q = [fcv.qk_norm_rope_fp4(qkv, pos, cos, sin, pool, rows, n_heads=hq) for pool in (dense, far)]
+    assert torch.equal(q[0], q[1]) and torch.equal(dense, far)
+    for a, b in zip(fcv.read_fp4_pages(dense, rows, dtype=torch.bfloat16),
+                    fcv.read_fp4_pages(far, rows, dtype=torch.bfloat16)):
+        assert torch.equal(a, b)
+    table = torch.tensor([[5, 0, 4, 1, 3, 2]], dtype=torch.int32, device=DEV)
+    lengths = torch.tensor([n * 64 - 5], dtype=torch.int32, device=DEV)
+    for count in (1, 3, tokens):  # each form of the attention
+        many = q[0][:count].repeat(1 if count < tokens else 24, 1, 1)
+        batch = 1 if count < tokens else 24
+        got = [fcv.paged_attention_fp4(many, pool, table.expand(batch, -1), lengths.expand(batch).contiguous())
+               for pool in (dense, far)]
+        assert torch.equal(got[0], got[1])
+    fcv.copy_pages(far.transpose(0, 1), [5, 0], [1, 4])  # a head as a layer: its bytes lie together
+    assert torch.equal(far[1], dense[5]) and torch.equal(far[4], dense[0])
