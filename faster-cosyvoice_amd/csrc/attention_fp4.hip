@@ -38,6 +38,7 @@ struct AttendArgs {
   int each;                  // rows of every sequence without cu_q
   int row_tiles;             // tiles of 16 rows of a sequence's longest query range
   int splits, pages_per;     // ranges of keys, and the pages of one
+  int order_shift;           // of sequence_of, or -1: sequences in their order
   float* part;               // [splits][tokens][n_heads][D]
   float* part_ml;            // [splits][tokens][n_heads][2]
 };
@@ -58,6 +59,54 @@ __device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
   typedef __bf16 b2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b});
+}
+
+// The sequence of a workgroup's slot: of every kOrdered sequences the one of that rank by falling length (in
+// steps of 2^order_shift; equal ones in their order), so that the longest start first and the short ones fill the
+// ends.  Every wave selects it for itself, by ballots: the largest key that more than `rank` of the sequences
+// reach, then one of those that have it.
+constexpr int kOrdered = 1024, kKeyBits = 8;
+__device__ __forceinline__ int sequence_of(const AttendArgs& a, int slot) {
+  if (a.order_shift < 0) return slot;
+  constexpr int kChunks = kOrdered / 64;
+  const int lane = threadIdx.x & 63;
+  const int first = slot / kOrdered * kOrdered, count = min(a.p.batch - first, kOrdered);
+  int rank = slot - first;
+  int key[kChunks];
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    key[c] = -1;
+    if (64 * c >= count) continue;
+    if (64 * c + lane < count)
+      key[c] = min(max(a.p.lengths[first + 64 * c + lane], 0) >> a.order_shift, (1 << kKeyBits) - 1);
+  }
+  auto reach = [&](int k) {  // how many have a key of k or more
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      if (64 * c >= count) break;
+      n += __popcll(__ballot(key[c] >= k));
+    }
+    return n;
+  };
+  int k = 0;
+#pragma unroll
+  for (int bit = kKeyBits - 1; bit >= 0; --bit)
+    if (reach(k | 1 << bit) > rank) k |= 1 << bit;
+  rank -= reach(k + 1);
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    if (64 * c >= count) break;
+    const uint64_t those = __ballot(key[c] == k);
+    const int n = __popcll(those);
+    if (rank < n) {
+      const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(those >> 32),
+                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)those, 0));
+      return first + 64 * c + __builtin_ctzll(__ballot(key[c] == k && below == rank));
+    }
+    rank -= n;
+  }
+  return slot;
 }
 
 // What a lane reads of a page.
@@ -84,7 +133,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
   const uint32_t col = lane & 15, blk = lane >> 4;
   int b, first, n;  // the sequence, its first row of q, its queries
   const int kv = blockIdx.x % p.n_kv_heads, tile = blockIdx.x / p.n_kv_heads % a.row_tiles;
-  b = blockIdx.x / p.n_kv_heads / a.row_tiles;
+  b = sequence_of(a, blockIdx.x / p.n_kv_heads / a.row_tiles);
   // What the whole workgroup asks for first, in one go.  Nothing writes it while the kernel runs: scalar loads.
   typedef const int32_t __attribute__((address_space(4))) * Uniform;
   const Uniform table = (Uniform)(uintptr_t)(p.table + (int64_t)b * p.table_row);
@@ -407,7 +456,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 31, fh = lane >> 5;
   const int kv = blockIdx.x % p.n_kv_heads, turn = blockIdx.x / p.n_kv_heads % a.row_tiles;
-  const int b = blockIdx.x / p.n_kv_heads / a.row_tiles;
+  const int b = sequence_of(a, blockIdx.x / p.n_kv_heads / a.row_tiles);
   typedef const int32_t __attribute__((address_space(4))) * Uniform;  // nothing writes these: scalar loads
   const Uniform table = (Uniform)(uintptr_t)(p.table + (int64_t)b * p.table_row);
   int first, n;
@@ -862,6 +911,7 @@ struct Plan {
   int rows;  // of a tile
   int64_t row_tiles;
   int splits, pages_per;
+  int order_shift;
 };
 
 Plan plan_of(const FcvFp4Attention& p) {
@@ -880,11 +930,18 @@ Plan plan_of(const FcvFp4Attention& p) {
   const int64_t most = (int64_t)p.max_pages * kPage;
   const int pages = (int)std::max<int64_t>((std::min<int64_t>(p.max_length, most) + kPage - 1) / kPage, 1);
   // Ranges of pages: two workgroups a CU; a workgroup's beginning and end cost about 5 us.  32 heads of 128 over
-  // 8, 64 sequences of 1000 to 8000 keys (512 workgroups): one, two, three and four ranges take 83, 90, 87 and
-  // 92 us; 14 over 2 of 64, 64 of 500 to 4000: one, two, four and eight 20, 16, 15.5 and 16.5; one of 7000 keys
-  // in ranges of 4, 8 and 16 pages 8.2, 8.8 and 10.6.
+  // 8, single tokens behind 1000 to 7000 keys: 64 sequences (512 workgroups) take 67, 67, 68 and 74 us in one,
+  // two, three and four ranges, 24 (192) 46, 38, 34 and 40; 14 over 2 of 64, 64 of 500 to 4000: one, two, four
+  // and eight 20, 16, 15.5 and 16.5; one of 7000 keys in ranges of 4, 8 and 16 pages 8.2, 8.8 and 10.6.
   // Up to 16 pages one range: it costs a microsecond there (8.5 instead of 7.6 for 600 keys) and saves a launch.
-  const int64_t want = pages <= 16 ? 1 : std::max<int64_t>(1, 2 * kCus / blocks);
+  // Two where one leaves CUs with half of what others have: 36 sequences (288) 62 us in one and 48 in two,
+  // 44 (352) 61 and 48, 48 (384) 63 and 58; but behind 300 to 3000 keys 44 take 31 in one and 38 in two.
+  int64_t want = pages <= 16 ? 1 : std::max<int64_t>(1, 2 * kCus / blocks);
+  if (blocks > kCus && blocks < 2 * kCus) {
+    auto filled = [](int64_t n) { return (double)n / (double)((n + kCus - 1) / kCus * kCus); };
+    const double us = (double)blocks * pages * kPage * (p.head_dim + p.head_dim / 32 + 1) / 5.0e6;
+    if (us / filled(blocks) - us / filled(2 * blocks) > 22.0) want = 2;
+  }
   int per = (int)std::max<int64_t>((pages + want - 1) / want, 4);
   if (rows == kTileRows) {
     // Time in pages of a workgroup that shares its CU; one that has it alone takes 0.63 of it, and a tile's
@@ -905,7 +962,14 @@ Plan plan_of(const FcvFp4Attention& p) {
       }
     }
   }
-  return Plan{rows, tiles, (pages + per - 1) / per, per};
+  const int splits = (pages + per - 1) / per;
+  // The longest sequences first, where their workgroups are long: 64 of 2000 to 8000 keys 84 us in their own
+  // order, 76 so; 100 of 1000 to 7000 115 and 96; 30 x 100 to 300 tokens behind 500 to 3000, 14 over 2 of 64,
+  // 128 and 101.  It costs a workgroup about a microsecond: 8 of 500 to 7000 in ranges of 14 pages 17.0 and 18.4.
+  int shift = -1;
+  if (p.batch > 1 && per >= 32 && blocks * splits > kCus)
+    for (shift = 6; pages * (int64_t)kPage >> shift >= 1 << kKeyBits; ++shift) {}
+  return Plan{rows, tiles, splits, per, shift};
 }
 
 size_t workspace_bytes(const FcvFp4Attention& p, const Plan& plan) {
@@ -952,7 +1016,7 @@ extern "C" int fcv_fp4_attention(const FcvFp4Attention* args, void* workspace, s
   float* part = static_cast<float*>(workspace);
   const AttendArgs a{*args, args->n_heads / args->n_kv_heads, args->tokens / args->batch,
                      (int)plan.row_tiles, plan.splits,
-                     plan.pages_per, part,
+                     plan.pages_per, plan.order_shift, part,
                      part ? part + (size_t)plan.splits * args->tokens * args->n_heads * args->head_dim
                           : nullptr};
   if (args->dtype == FCV_LM_F16)

@@ -320,3 +320,18 @@ def test_queries_without_numbers_and_without_pages(fcv, news, d):
     out, lse = run(fcv, st, return_lse=True)
     assert bool((out[first:end] == 0).all()) and bool((lse[first:end] == -math.inf).all())
     assert torch.equal(out[:first], clean[:first]) and torch.equal(out[end:], clean[end:])
+
+
+@pytest.mark.parametrize("batch,heads,n_kv,d", [(300, 4, 1, 64), (70, 16, 4, 64), (1100, 2, 1, 64), (40, 32, 8, 128)])
+def test_sequences_of_many_lengths(fcv, batch, heads, n_kv, d):
+    """Batches that are taken longest first: equal lengths among them, none, one past the table, and more
+    sequences than are ordered together."""
+    say(f"[attend fp4] order {batch} {heads}/{n_kv} x {d}")
+    g = torch.Generator().manual_seed(batch)
+    keys = torch.randint(0, 60, (batch,), generator=g)
+    keys[0], keys[batch // 2], keys[-1] = 2300, 2300, 2310
+    keys[3:20:3] = 0
+    st = make([1] * batch, keys.tolist(), heads, n_kv, d, torch.bfloat16)
+    check(fcv, st, "many lengths")
+    st["lengths"][batch // 3], st["lengths"][5] = 1 << 30, -7
+    check(fcv, st, "bounds", max_length=2310)
