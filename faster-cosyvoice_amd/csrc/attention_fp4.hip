@@ -417,17 +417,19 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
 // m follows a row's maximum only where it has risen by kSlack (a power of two: weights up to 2^1.75), so that
 // few pages scale the sums; the other tiles' m is the maximum.
 //
-// Bound: instructions.  8 texts of 300 behind 500 to 3000 keys, 32 heads of 128 over 8, run at 0.57 PFLOP/s
-// (bf16, 168 us; 0.53 in fp16): the matrix pipes are busy for two fifths of it, and some 600 other instructions
-// to a wave's page take their turns with the products of the CU's other workgroup.
+// Bound: instructions.  4000 tokens of 32 heads of 128 over 8 run at 0.76 PFLOP/s in bf16 (173 us) and 0.62 in
+// fp16, 4 texts of 300 to 1024 behind 4096 keys at 0.72 (189 us) and 0.58, 7000 of 14 heads of 64 over 2 at 0.54:
+// the matrix pipes are busy for a third of it (27 % of the time, CUs 80 %: texts), and some 300 vector
+// instructions to a wave's page, 32 of them exponentials at a quarter of the rate, take their turns with the
+// products of the CU's other workgroup.
 //
 // bf16.  Results are off by 2^-8 from their rounding, and one fp16 number, off by 2^-11, is all that a weight
 // times its value's scale goes in as, times 2^kTop and over 2^u (u as a scale byte): one below 2^-28 of
 // 2^u loses bits, one below 2^-39 is 0.  u is the row's, and as large as the page's largest scale, or as the
-// row's largest product of a weight and a scale with kRoom over it where that is less: values that a row hides, or
-// weighs next to nothing, cost the others no bit, however large.  A row's u follows its m's rise (`owed`) once
-// that is more than kRoom.  LDS holds the scales over the largest scale of all pages so far; the factor
-// between the two goes into the exponent, and out of l's terms again.
+// row's largest product of a weight and a scale with kRoom over it where that is less: values that a row hides,
+// or weighs next to nothing, do not set it.  A row's u follows its m's rise (`owed`) once that is more than
+// kRoom.  LDS holds the scales over the largest scale of all pages so far; the factor between the two goes into
+// the exponent, and out of l's terms again.
 // fp16.  Weights go in as two bf16 numbers as above.
 //
 // A value without a scale (its byte is 255) lies in LDS as zeros, and rows that see it become NaN at their end.
@@ -445,6 +447,9 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
   using P = Page<D>;
   constexpr int kRows = kTileRows, kSteps = D / 16, kDT = D / 32;
   constexpr bool kOne = std::is_same<E, Bf16>::value;  // one fp16 number a weight
+  // products before the other workgroup's vector instructions: 4000 tokens of 32 heads of 128 182 -> 173 us, but
+  // 7000 of 14 of 64 164 -> 173
+  constexpr bool kFirst = D == 128;
   using V = typename std::conditional<kOne, Half, Bf16>::type;
   __shared__ __attribute__((aligned(16))) short sk[2][kPage * D];
   __shared__ __attribute__((aligned(16))) short sv[2][D * kPage];
@@ -723,6 +728,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       };
       load_vf(0);
       weights(0);
+      if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         if (st < 3) load_vf(st + 1);
@@ -764,8 +770,11 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
         unpack(buf ^ 1, page + 1, next >= 0);
         load(after);
         if (sees_it) {
+          if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
           scores(buf);
+          if constexpr (kFirst) __builtin_amdgcn_s_setprio(0);
           take(page, buf);
+          if constexpr (kFirst) __builtin_amdgcn_s_setprio(0);
         }
         id = next;
         next = after;
@@ -918,7 +927,7 @@ Plan plan_of(const FcvFp4Attention& p) {
   const int group = p.n_heads / p.n_kv_heads;
   const int64_t most_rows = (int64_t)std::min(p.max_q, p.tokens) * group;
   // Tiles of 128 rows where they fill the card, which takes more of heads of 64, whose pages are short.  Heads of
-  // 128, 32 over 8, by tiles of 128 and of 16 rows: 4000 tokens (1000 tiles) 176 and 304 us, 2000 (500) 63 and
+  // 128, 32 over 8, by tiles of 128 and of 16 rows: 4000 tokens (1000 tiles) 173 and 304 us, 2000 (500) 63 and
   // 98, 8 x 128 behind a cache (256) 80 and 98, 1000 (250) 34 and 36, 4 x 128 (128) 79 and 54.  Heads of 64,
   // 14 over 2: 7000 (766) 161 and 229, 16 x 300 (544) 112 and 106, 8 x 300 (272) 77 and 64, 2000 (220) 52 and 28.
   const int64_t many = (most_rows + kTileRows - 1) / kTileRows * p.batch * p.n_kv_heads;
@@ -967,7 +976,7 @@ Plan plan_of(const FcvFp4Attention& p) {
   // order, 76 so; 100 of 1000 to 7000 115 and 96; 30 x 100 to 300 tokens behind 500 to 3000, 14 over 2 of 64,
   // 128 and 101.  It costs a workgroup about a microsecond: 8 of 500 to 7000 in ranges of 14 pages 17.0 and 18.4.
   int shift = -1;
-  if (p.batch > 1 && per >= 32 && blocks * splits > kCus)
+  if (p.batch >= (rows == kTileRows ? 8 : 2) && per >= 32 && blocks * splits > kCus)
     for (shift = 6; pages * (int64_t)kPage >> shift >= 1 << kKeyBits; ++shift) {}
   return Plan{rows, tiles, splits, per, shift};
 }
