@@ -132,7 +132,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void linear_fp4_few_kernel(const
 // ---- many rows: operands by copies into LDS ---------------------------------------------------------
 //
 // The ring of slices of linear.hip: x as it lies there, W's slice in 4 bits (a quarter of the LDS and of the
-// copies) and four scales a row.  A lane of the 32 x 32 x 16 instruction has one group in 64 of K: its codes are
+// copies) and a row's four scales of 128 elements.  Rows of scales start on any byte: both words that the four lie
+// in are copied, and shifted together where they are used.  A lane of the 32 x 32 x 16 instruction has one group in 64 of K: its codes are
 // one read, and become fragments a step ahead of the products that take them.
 template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int BK_>
 struct Fp4Tile {
@@ -142,17 +143,17 @@ struct Fp4Tile {
   static constexpr int kChunks = BK / 8, kXRows = 64 / kChunks;       // 16-byte chunks of a row of x; rows of a copy
   static constexpr int kGroups = BK / 32, kWRows = 64 / kGroups;      // and of a row of codes
   static constexpr int kXCopies = BM / kXRows / kWaves;
-  static constexpr int kWParts = BN / kWRows, kSParts = BN / 64;
+  static constexpr int kWParts = BN / kWRows, kSParts = 2 * (BN / 64);
   static constexpr int kWCopies = kWParts > kWaves ? kWParts / kWaves : 1;
   static constexpr int kCopies = kXCopies + kWCopies + 1;
-  static constexpr int kW = BM * BK * 2, kS = kW + BN * BK / 2, kStage = kS + BN * 4;  // bytes
+  static constexpr int kW = BM * BK * 2, kS = kW + BN * BK / 2, kStage = kS + BN * 8;  // bytes
   static constexpr int kLds = STAGES * kStage;
   static constexpr int kGroupM = 1024 / BM > 0 ? 1024 / BM : 1;
   static constexpr int kPerCu = 160 * 1024 / kLds;
   static constexpr int kWavesPerSimd = kPerCu * kWaves >= 8 ? 2 : 1;
   // small tiles: a whole slice's operands are read at once, under the products of the slice before
   static constexpr bool kWhole = TM * TN <= 2;
-  static_assert(BM % (kXRows * kWaves) == 0 && kSParts >= 1 && kSParts <= kWaves, "copy split");
+  static_assert(BM % (kXRows * kWaves) == 0 && kSParts <= kWaves, "copy split");
   static_assert((STAGES - 2) * kCopies < 64, "copies in flight");
 };
 
@@ -195,7 +196,11 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
                                                  (int64_t)slice0 * BK);
   const char* wb =
       reinterpret_cast<const char*>(f.codes + (int64_t)n0 * f.ld_codes + (int64_t)slice0 * (BK / 2));
-  const char* sb = reinterpret_cast<const char*>(f.scales + (int64_t)n0 * f.ld_scales);
+  const uintptr_t s_first = (uintptr_t)f.scales + (int64_t)n0 * f.ld_scales;
+  const char* sb = reinterpret_cast<const char*>(s_first & ~(uintptr_t)3);
+  auto scale_at = [&](int row) {  // of the tile, in bytes from sb
+    return (uint32_t)(s_first & 3) + (uint32_t)min(row, p.n - 1 - n0) * (uint32_t)f.ld_scales;
+  };
   const int crow = lane / C::kChunks, cpos = lane % C::kChunks;
   uint32_t x_off[C::kXCopies], w_off[C::kWCopies];
 #pragma unroll
@@ -211,7 +216,12 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
     const int row = (w_part + i) * C::kWRows + grow;
     w_off[i] = (uint32_t)min(row, p.n - 1 - n0) * (uint32_t)f.ld_codes + swz_w<BK>(row, gpos) * 16;
   }
-  const uint32_t s_off = (uint32_t)min(s_part * 64 + lane, p.n - 1 - n0) * (uint32_t)f.ld_scales;
+  const uint32_t s_at = scale_at(s_part / 2 * 64 + lane);
+  const uint32_t s_off = (s_at & ~3u) + (s_part & 1) * 4;
+  // the last span's groups; a second word without one of them is not read (it may lie behind the scales)
+  const int last_span = (p.k - 1) / kSpan;
+  const int last_groups = (p.k + FCV_FP4_GROUP - 1) / FCV_FP4_GROUP - 4 * last_span;
+  const uint32_t s_last = (s_at & ~3u) + ((s_part & 1) && (int)(s_at & 3) + last_groups > 4 ? 4 : 0);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)smem;
   const uint32_t lds_x = lds0 + wave * C::kXCopies * 1024;
   const uint32_t lds_w = lds0 + C::kW + w_part * 1024;
@@ -228,7 +238,8 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
     for (int c = 0; c < C::kCopies; ++c) {
       if (c < c0 || c >= c1) continue;
       if (c == 0) {
-        lds_dma4(sb + slice * BK / kSpan * 4, s_off, lds_s + at);
+        const int span = slice * BK / kSpan;
+        lds_dma4(sb + span * 4, span == last_span ? s_last : s_off, lds_s + at);
       } else if (c < 1 + C::kWCopies) {
         const int i = c - 1;
         if (last) {
@@ -264,7 +275,8 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
   constexpr int kSets = C::kWhole ? 2 : 1;
   s16x8 fx[C::kWhole ? 2 * KS : 2][TM], fw[2][TN];
   u32x4 wc[kSets][TN][kHalves];
-  uint32_t ws[kSets][TN];
+  uint32_t ws[TN][2], ss[kSets][TN];  // scales as they lie, and in their places
+  const uint32_t s_shift = (uint32_t)(s_first + (uint32_t)fr * (uint32_t)f.ld_scales) % 4 * 8;  // rows 32 apart alike
   auto load_w = [&](int set, int st) {
     const char* w = smem + st * C::kStage + C::kW;
     const char* s = smem + st * C::kStage + C::kS;
@@ -275,7 +287,9 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
       for (int u = 0; u < kHalves; ++u)
         wc[set][j][u] =
             *reinterpret_cast<const u32x4*>(w + row * (BK / 2) + swz_w<BK>(row, 2 * u + fh) * 16);
-      ws[set][j] = *reinterpret_cast<const uint32_t*>(s + row * 4);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        ws[j][u] = *reinterpret_cast<const uint32_t*>(s + row / 64 * 512 + u * 256 + row % 64 * 4);
     }
   };
   // step ks: elements 8 (ks % 4) .. + 7 of group 2 (ks / 4) + fh
@@ -288,12 +302,20 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
           sx + row * BK + swz<BK>(row, ks / 4 * 8 + 4 * fh + ks % 4) * 8);
     }
   };
+  // the scales of slice kt; what lies past K is 1
+  auto place = [&](int set, int kt) {
+    const bool last = (slice0 + kt) * BK / kSpan == last_span && last_groups < 4;
+    const uint32_t keep = last ? (1u << (8 * last_groups)) - 1 : ~0u;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      ss[set][j] = (__builtin_amdgcn_alignbit(ws[j][1], ws[j][0], s_shift) & keep) | (0x7f7f7f7fu & ~keep);
+  };
   // `odd`: the slice is the second one of its span (BK 64)
   auto convert = [&](int buf, int set, int ks, int odd) {
     const int shift = ((ks / 4 + odd) * 2 + fh) * 8;
 #pragma unroll
     for (int j = 0; j < TN; ++j)
-      fw[buf][j] = fp4_octet<E>(wc[set][j][ks / 4][ks % 4], scale_of((ws[set][j] >> shift) & 255));
+      fw[buf][j] = fp4_octet<E>(wc[set][j][ks / 4][ks % 4], scale_of((ss[set][j] >> shift) & 255));
   };
   auto parity = [&](int kt) { return BK == 64 ? (slice0 + kt) & 1 : 0; };
 #pragma unroll
@@ -310,8 +332,9 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) load_x(decltype(set)::value * KS + ks, ks, stage);
     };
-    auto mma_all = [&](auto set, int odd) {
+    auto mma_all = [&](auto set, int kt) {
       __builtin_amdgcn_sched_barrier(0);
+      const int odd = parity(kt);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         convert(ks & 1, decltype(set)::value, ks, odd);
@@ -332,10 +355,12 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
       stage = stage == S - 1 ? 0 : stage + 1;
       load_all(set);
       if (kt + S - 1 < KT) issue(kt + S - 1, freed, 0, C::kCopies);
-      mma_all(before, parity(kt - 1));
+      mma_all(before, kt - 1);
+      place(decltype(set)::value, kt);
     };
     if (S - 1 < KT) issue(S - 1, S - 1, 0, C::kCopies);
     load_all(even);
+    place(0, 0);
     for (kt = 1; kt < KT;) {
       step(odd, even);
       if (++kt == KT) break;
@@ -343,9 +368,9 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
       ++kt;
     }
     if (KT & 1)
-      mma_all(even, parity(KT - 1));
+      mma_all(even, KT - 1);
     else
-      mma_all(odd, parity(KT - 1));
+      mma_all(odd, KT - 1);
   } else {
     // rotated by one step as in linear.hip: a slice's last step runs from registers after the barrier that
     // publishes the next slice and frees the one before
@@ -393,6 +418,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
     copies(0);
     load_w(0, 0);
     load_x(0, 0, 0);
+    place(0, 0);
     convert(0, 0, 0, parity(0));
     head(0);
     for (kt = 1; kt < KT; ++kt) {
@@ -404,6 +430,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
       load_x(0, 0, stage);
       copies(0);
       mma(1);
+      place(0, kt);
       convert(0, 0, 0, parity(kt));
       head(stage);
     }
@@ -412,27 +439,13 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
   store_tile<E, C, C::kLds>(f.a, acc, reinterpret_cast<short*>(smem), split, n0, wn0, wm0, m0);
 }
 
-// Copies that make a call's operands fit the tiles: rows of x from any boundary to 16-byte ones with zeros up
-// to a multiple of 8, rows of scales to multiples of 4 bytes.  A thread has 8 elements of x or 4 scales.
-__global__ __launch_bounds__(256) void lay_out_kernel(const Fp4Args f, short* x, int64_t ldx, int64_t x_units,
-                                                      uint8_t* scales, int64_t ld_scales,
-                                                      int64_t scale_units) {
-  const FcvLmLinear& p = f.a.p;
-  const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  for (int64_t i = first; i < x_units; i += step) {
+// Copies rows of x from any boundary to 16-byte ones, with zeros up to a multiple of 8.  A thread has 8 elements.
+__global__ __launch_bounds__(256) void lay_out_kernel(const FcvLmLinear p, short* x, int64_t ldx, int64_t units) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < units; i += (int64_t)gridDim.x * 256) {
     const int64_t per = ldx / 8, row = i / per;
     const int k = (int)(i % per) * 8;
     *reinterpret_cast<s16x8*>(x + row * ldx + k) =
         row_chunk(static_cast<const short*>(p.x) + row * p.ldx, k, p.k);
-  }
-  for (int64_t u = first; u < scale_units; u += step) {
-    const int64_t per = ld_scales / 4, row = u / per;
-    const int g = (int)(u % per) * 4, groups = (p.k + FCV_FP4_GROUP - 1) / FCV_FP4_GROUP;
-    uint32_t w = 0x7f7f7f7fu;
-    for (int e = 0; e < 4; ++e)
-      if (g + e < groups)
-        w = (w & ~(255u << (8 * e))) | (uint32_t)f.scales[row * f.ld_scales + g + e] << (8 * e);
-    *reinterpret_cast<uint32_t*>(scales + row * ld_scales + g) = w;
   }
 }
 
@@ -507,8 +520,8 @@ int check(const FcvFp4Linear* p) {
 //   16384 39, 26 and 19; 32 x 4096 x 4096 11.8, 13.5 and 17.5, with K in 1, 2 and 4 ranges 11.8, 10.7 and 9.8.
 //   (x loaded in whole lines, W's words changing places between lanes instead: no faster.)
 // A cut K adds the join's 1.8 (3.5 to few rows: what the second launch takes of the host, which calls that
-// short wait for) and its sums' way, operands off their boundaries the pass that lays them out
-// (the same for every tile).
+// short wait for) and its sums' way, an x off its boundaries the pass that lays it out (the same
+// for every tile).
 enum Form { kFew, kTile64, kTile64x128, kTile128, kTile128x256, kTile256 };
 
 struct Shape {
@@ -528,11 +541,10 @@ struct Plan {
   Form form;
   int nt;              // of kFew: blocks of 16 rows of W
   int splits, spans;   // ranges of K, and the spans of 128 of one
-  bool lay_x, lay_s;   // operands that are laid out first
+  bool lay_x;          // x is laid out first
 };
 
 int part_ld(int n) { return (n + 3) / 4 * 4; }
-int64_t groups_of(const FcvFp4Linear& p) { return (p.k + FCV_FP4_GROUP - 1) / FCV_FP4_GROUP; }
 
 float join_us(const FcvFp4Linear& p, int splits) {
   return splits > 1 ? (p.m <= kFewMost ? 3.5f : 1.8f) + (float)p.m * (float)p.n * 8.0f * splits / 5.0e6f : 0.0f;
@@ -540,7 +552,6 @@ float join_us(const FcvFp4Linear& p, int splits) {
 
 Plan plan_of(const FcvFp4Linear& p) {
   const bool lay_x = !(aligned(p.x, 16) && (p.ldx % 8 == 0 || p.m == 1) && p.k % 8 == 0 && p.ldx < (1 << 22));
-  const bool lay_s = !(aligned(p.scales, 4) && (p.ld_scales % 4 == 0 || p.n == 1) && groups_of(p) % 4 == 0);
   const int spans = (p.k + kSpan - 1) / kSpan;
   Plan best{};
   float best_us = 3.0e38f;
@@ -549,7 +560,7 @@ Plan plan_of(const FcvFp4Linear& p) {
     if (us >= best_us) return;
     best_us = us;
     const int per = (spans + splits - 1) / splits;
-    best = Plan{form, nt, (spans + per - 1) / per, per, form != kFew && lay_x, form != kFew && lay_s};
+    best = Plan{form, nt, (spans + per - 1) / per, per, form != kFew && lay_x};
   };
   for (int splits : kSplits) {
     if (splits > 1 && spans < splits * kMinSpans) break;
@@ -577,10 +588,9 @@ Plan plan_of(const FcvFp4Linear& p) {
 }
 
 int64_t laid_ldx(const FcvFp4Linear& p) { return (p.k + 7) / 8 * 8; }
-int64_t laid_ld_scales(const FcvFp4Linear& p) { return (groups_of(p) + 3) / 4 * 4; }
 size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 
-// The workspace: sums of the ranges, then x and the scales laid out.
+// The workspace: sums of the ranges, then x laid out.
 size_t part_bytes(const FcvFp4Linear& p, const Plan& plan) {
   return plan.splits > 1 ? round_up((size_t)plan.splits * p.m * part_ld(p.n) * 4) : 0;
 }
@@ -588,8 +598,7 @@ size_t x_bytes(const FcvFp4Linear& p, const Plan& plan) {
   return plan.lay_x ? round_up((size_t)p.m * laid_ldx(p) * 2) : 0;
 }
 size_t workspace_bytes(const FcvFp4Linear& p, const Plan& plan) {
-  return part_bytes(p, plan) + x_bytes(p, plan) +
-         (plan.lay_s ? round_up((size_t)p.n * laid_ld_scales(p)) : 0);
+  return part_bytes(p, plan) + x_bytes(p, plan);
 }
 
 template <class E, class C>
@@ -624,17 +633,12 @@ void launch(const FcvFp4Linear& p, const Plan& plan, void* workspace, hipStream_
                       quad(p.bias, p.bias_dtype, 0),
                plan.splits, plan.spans, static_cast<float*>(workspace), part_ld(p.n)};
   Fp4Args f{a, p.codes, p.scales, p.ld_codes, p.ld_scales};
-  if (plan.lay_x || plan.lay_s) {
-    char* at = static_cast<char*>(workspace) + part_bytes(p, plan);
-    short* x = reinterpret_cast<short*>(at);
-    uint8_t* scales = reinterpret_cast<uint8_t*>(at + x_bytes(p, plan));
-    const int64_t x_units = plan.lay_x ? p.m * (laid_ldx(p) / 8) : 0;
-    const int64_t s_units = plan.lay_s ? p.n * (laid_ld_scales(p) / 4) : 0;
-    const int64_t blocks = std::min<int64_t>((std::max(x_units, s_units) + 255) / 256, 1 << 20);
-    hipLaunchKernelGGL(lay_out_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, f, x, laid_ldx(p),
-                       x_units, scales, laid_ld_scales(p), s_units);
-    if (plan.lay_x) f.a.p.x = x, f.a.p.ldx = laid_ldx(p), f.a.p.k = (int32_t)laid_ldx(p);
-    if (plan.lay_s) f.scales = scales, f.ld_scales = laid_ld_scales(p);
+  if (plan.lay_x) {
+    short* x = reinterpret_cast<short*>(static_cast<char*>(workspace) + part_bytes(p, plan));
+    const int64_t units = p.m * (laid_ldx(p) / 8);
+    const int64_t blocks = std::min<int64_t>((units + 255) / 256, 1 << 20);
+    hipLaunchKernelGGL(lay_out_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, f.a.p, x, laid_ldx(p), units);
+    f.a.p.x = x, f.a.p.ldx = laid_ldx(p), f.a.p.k = (int32_t)laid_ldx(p);
   }
   switch (plan.form) {
     case kFew:

@@ -32,7 +32,7 @@ def test_few_rows_keep_to_one_launch_where_weights_are_many(fcv):
 
 
 def test_workspaces(fcv):
-    """Sums of the ranges, and what is laid out first: rows of x off their boundaries, scales off theirs."""
+    """Sums of the ranges, and rows of x off their boundaries, which are laid out first; scales lie anywhere."""
     lib = fcv._lib.load()
 
     def need(m, k, n, **kw):
@@ -47,7 +47,7 @@ def test_workspaces(fcv):
 
     assert need(1, 4096, 4096) == 0 and need(4096, 4096, 4096) == 0 and need(0, 4096, 4096) == 0
     assert need(4096, 4096, 4096, x=BIG + 2) == up(4096 * 4096 * 2)
-    assert need(4096, 4100, 4096) == up(4096 * 4104 * 2) + up(4096 * 132)
-    assert need(4096, 4128, 4096) == up(4096 * 132) and need(4096, 4096, 4096, scales=BIG + 1) == up(4096 * 128)
+    assert need(4096, 4100, 4096) == up(4096 * 4104 * 2)
+    assert need(4096, 4128, 4096) == 0 and need(4096, 4096, 4096, scales=BIG + 1) == 0
     form, ranges = plan(fcv, 64, 4096, 4096)
     assert ranges > 1 and need(64, 4096, 4096) == up(ranges * 64 * 4096 * 4)

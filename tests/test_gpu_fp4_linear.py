@@ -277,3 +277,17 @@ def test_rows_of_weights_far_apart(fcv, m):
     scales = far.as_strided((n, 8), (2 ** 24 - 4, 1))
     scales.copy_(s)
     assert torch.equal(fcv.fused_linear_fp4(x, c, scales, b), want)
+
+
+@pytest.mark.parametrize("m,k,n", [(40, 96, 70), (100, 2112, 200), (300, 416, 300), (700, 160, 600), (2100, 1184, 1030)])
+@pytest.mark.parametrize("start", [0, 1, 2, 3])
+def test_scales_on_any_byte(fcv, m, k, n, start):
+    """Rows of 3, 13, 66, 5 and 37 scales from every byte of a word, at odd strides; NaN around them."""
+    x, c, s, b, _ = make(m, k, n, torch.bfloat16)
+    want = fcv.fused_linear_fp4(x, c, s)
+    check(want, x, c, s, None, None, None, torch.bfloat16, "dense")
+    for pad in (0, 5, 7):
+        wide = torch.full((n * (s.shape[1] + pad) + 16,), 255, dtype=torch.uint8, device=DEV)
+        view = wide[4 + start:4 + start + n * (s.shape[1] + pad)].view(n, -1)[:, :s.shape[1]]
+        view.copy_(s)
+        assert torch.equal(fcv.fused_linear_fp4(x, c, view), want), pad
