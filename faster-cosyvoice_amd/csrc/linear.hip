@@ -90,8 +90,8 @@ __global__ __launch_bounds__(256) void linear_any_kernel(const Args a) {
       *reinterpret_cast<f32x4*>(a.part + ((int64_t)blockIdx.y * p.m + m) * a.part_ld + n) = v;
       continue;
     }
-    const bool vec = a.vec && n + 3 < p.n;
-    finish4<E>(p, vec, m, n, v, bias4<E>(p, vec, n), residual4<E>(p, vec, m, n));
+    const bool whole = n + 3 < p.n;
+    finish4<E>(p, a.vec, m, n, v, bias4<E>(p, whole, n), residual4<E>(p, whole, m, n));
   }
 }
 
@@ -352,8 +352,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few_kernel(const Args a
     *reinterpret_cast<f32x4*>(a.part + ((int64_t)blockIdx.y * p.m + m) * a.part_ld + n) = v;
     return;
   }
-  const bool vec = a.vec && n + 3 < p.n;
-  finish4<E>(p, vec, m, n, v, bias4<E>(p, vec, n), residual4<E>(p, vec, m, n));
+  const bool whole = n + 3 < p.n;
+  finish4<E>(p, a.vec, m, n, v, bias4<E>(p, whole, n), residual4<E>(p, whole, m, n));
 }
 
 // ---- host ---------------------------------------------------------------------------------------

@@ -13,7 +13,7 @@ namespace {
 
 struct Args {
   FcvLmLinear p;
-  bool vec;                 // four columns of y, the residual and the bias are one aligned access
+  bool vec;                 // four columns of y, the residual and the bias are on the boundary of four
   int splits, slices;       // ranges of K, and the 64-wide slices of one
   float* part;              // [splits][m][part_ld] sums of the ranges
   int part_ld;
@@ -58,19 +58,23 @@ __device__ __forceinline__ float element(const void* p, bool f32, int64_t i) {
   return f32 ? static_cast<const float*>(p)[i] : E::to_f32(static_cast<const short*>(p)[i]);
 }
 
+// Four elements from any element's boundary: the same instruction as an aligned access.
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef s16x4 s16x4_any __attribute__((aligned(2)));
+
 template <class E>
 __device__ __forceinline__ f32x4 load4(const void* p, bool f32, int64_t i) {
-  if (f32) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
-  const s16x4 b = *reinterpret_cast<const s16x4*>(static_cast<const short*>(p) + i);
+  if (f32) return *reinterpret_cast<const f32x4_any*>(static_cast<const float*>(p) + i);
+  const s16x4 b = *reinterpret_cast<const s16x4_any*>(static_cast<const short*>(p) + i);
   return f32x4{E::to_f32(b[0]), E::to_f32(b[1]), E::to_f32(b[2]), E::to_f32(b[3])};
 }
 
 template <class E>
 __device__ __forceinline__ void store4(void* p, bool f32, int64_t i, const f32x4& v) {
   if (f32)
-    *reinterpret_cast<f32x4*>(static_cast<float*>(p) + i) = v;
+    *reinterpret_cast<f32x4_any*>(static_cast<float*>(p) + i) = v;
   else
-    *reinterpret_cast<s16x4*>(static_cast<short*>(p) + i) =
+    *reinterpret_cast<s16x4_any*>(static_cast<short*>(p) + i) =
         s16x4{E::from_f32(v[0]), E::from_f32(v[1]), E::from_f32(v[2]), E::from_f32(v[3])};
 }
 
@@ -87,17 +91,20 @@ __device__ __forceinline__ void finish1(const FcvLmLinear& p, int m, int n, floa
     static_cast<short*>(p.y)[at] = E::from_f32(z);
 }
 
-// Four columns n .. n + 3 of row m from their sums: those below N one at a time, or all of them
-// where they are one aligned access (`vec`).
+// Four columns n .. n + 3 of row m from their sums: at once, or those below N one at a time.  What is not
+// there is not added where an access is off its boundary (`vec` false), so that a sum of -0 stays one as in
+// finish1.
 template <class E>
 __device__ __forceinline__ void finish4(const FcvLmLinear& p, bool vec, int m, int n, f32x4 v,
                                         const f32x4& bias, const f32x4& residual) {
-  if (vec) {
-    v = act4(v + bias, p.activation) + residual;
+  if (n + 3 < p.n) {
+    if (vec || p.bias) v += bias;
+    v = act4(v, p.activation);
+    if (vec || p.residual) v += residual;
     store4<E>(p.y, p.y_dtype == FCV_LM_F32, (int64_t)m * p.ldy + n, v);
     return;
   }
-  const int count = min(4, p.n - n);
+  const int count = p.n - n;
 #pragma unroll 1
   for (int e = 0; e < count; ++e) {
     finish1<E>(p, m, n + e, v[0]);
@@ -106,13 +113,13 @@ __device__ __forceinline__ void finish4(const FcvLmLinear& p, bool vec, int m, i
 }
 
 template <class E>
-__device__ __forceinline__ f32x4 bias4(const FcvLmLinear& p, bool vec, int n) {
-  return vec && p.bias ? load4<E>(p.bias, p.bias_dtype == FCV_LM_F32, n) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+__device__ __forceinline__ f32x4 bias4(const FcvLmLinear& p, bool whole, int n) {
+  return whole && p.bias ? load4<E>(p.bias, p.bias_dtype == FCV_LM_F32, n) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
 template <class E>
-__device__ __forceinline__ f32x4 residual4(const FcvLmLinear& p, bool vec, int m, int n) {
-  return vec && p.residual ? load4<E>(p.residual, p.residual_dtype == FCV_LM_F32, (int64_t)m * p.ldr + n)
+__device__ __forceinline__ f32x4 residual4(const FcvLmLinear& p, bool whole, int m, int n) {
+  return whole && p.residual ? load4<E>(p.residual, p.residual_dtype == FCV_LM_F32, (int64_t)m * p.ldr + n)
                     : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
@@ -202,7 +209,6 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[C:
   float* stg = reinterpret_cast<float*>(smem) + wave * 32 * kPitch;
   const int rr = lane / kLanes, rc = (lane % kLanes) * 4;
   const int col = n0 + wn0 + rc;
-  const bool inside = col < p.n;
   auto park = [&](int i) {
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -230,66 +236,46 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[C:
     }
     return;
   }
-  if (__all(a.vec && (!inside || col + 3 < p.n))) {
-    with_act(p.activation, [&](auto kind) {
-      const f32x4 bias = bias4<E>(p, inside, col);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int row0 = m0 + wm0 + i * 32 + rr;
-        f32x4 r[kPasses];
-        // a block's residuals are asked for together, before its stores
-#pragma unroll
-        for (int q = 0; q < kPasses; ++q)
-          r[q] = residual4<E>(p, inside, min(row0 + q * kPassRows, p.m - 1), col);
-        park(i);
-        f32x4 v[kPasses];
-#pragma unroll
-        for (int q = 0; q < kPasses; ++q)
-          v[q] = *reinterpret_cast<const f32x4*>(mine + q * kPassRows * kPitch);
-        wave_fence();
-#pragma unroll
-        for (int q = 0; q < kPasses; ++q) {
-          const f32x4 z = act4<decltype(kind)::value>(v[q] + bias) + r[q];
-          const int row = row0 + q * kPassRows;
-          if (row < p.m && inside) store4<E>(p.y, p.y_dtype == FCV_LM_F32, (int64_t)row * p.ldy + col, z);
-        }
-      }
-    });
-    return;
-  }
-  // rows off their boundaries, or N no multiple of four: a column a lane, neighbouring lanes along a row
-  static_assert(64 % kCols == 0, "a lane keeps its column");
-  const int n = n0 + wn0 + lane % kCols;
-  const float bias1 = p.bias && n < p.n ? element<E>(p.bias, p.bias_dtype == FCV_LM_F32, n) : 0.0f;
+  // where N ends inside a lane's four columns, the one to three below it have a pass of their own
+  const bool whole = col + 3 < p.n;
+  const int left = p.n - n0 - wn0, edge = left > 0 && left < kCols ? left & 3 : 0;
   with_act(p.activation, [&](auto kind) {
+    const f32x4 bias = bias4<E>(p, whole, col);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
+      const int row0 = m0 + wm0 + i * 32 + rr;
+      f32x4 r[kPasses];
+      // a block's residuals are asked for together, before its stores
+#pragma unroll
+      for (int q = 0; q < kPasses; ++q)
+        r[q] = residual4<E>(p, whole, min(row0 + q * kPassRows, p.m - 1), col);
       park(i);
-      const int row0 = m0 + wm0 + i * 32 + lane / kCols;
-#pragma unroll 1
-      for (int q0 = 0; q0 < kCols / 2; q0 += 8) {  // 8 of the block's passes of 64 / kCols rows
-        float r[8];
+      f32x4 v[kPasses];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int row = row0 + (q0 + q) * (64 / kCols);
-          r[q] = p.residual && row < p.m && n < p.n
-                     ? element<E>(p.residual, p.residual_dtype == FCV_LM_F32, (int64_t)row * p.ldr + n)
-                     : 0.0f;
-        }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int row = row0 + (q0 + q) * (64 / kCols);
-          const float v = stg[(row - m0 - wm0 - i * 32) * kPitch + lane % kCols];
-          const float z = act<decltype(kind)::value>(v + bias1) + r[q];
-          if (row >= p.m || n >= p.n) continue;
-          const int64_t at = (int64_t)row * p.ldy + n;
+      for (int q = 0; q < kPasses; ++q)
+        v[q] = *reinterpret_cast<const f32x4*>(mine + q * kPassRows * kPitch);
+      if (edge) {
+        const int row = m0 + wm0 + i * 32 + fr;
+        for (int e = fh; e < edge && row < p.m; e += 2) {
+          const int at = left - edge + e, n = n0 + wn0 + at;
+          const float b = p.bias ? element<E>(p.bias, p.bias_dtype == FCV_LM_F32, n) : 0.0f;
+          const float z = act<decltype(kind)::value>(stg[fr * kPitch + at] + b) +
+                          (p.residual ? element<E>(p.residual, p.residual_dtype == FCV_LM_F32,
+                                                   (int64_t)row * p.ldr + n)
+                                      : 0.0f);
           if (p.y_dtype == FCV_LM_F32)
-            static_cast<float*>(p.y)[at] = z;
+            static_cast<float*>(p.y)[(int64_t)row * p.ldy + n] = z;
           else
-            static_cast<short*>(p.y)[at] = E::from_f32(z);
+            static_cast<short*>(p.y)[(int64_t)row * p.ldy + n] = E::from_f32(z);
         }
       }
       wave_fence();
+#pragma unroll
+      for (int q = 0; q < kPasses; ++q) {
+        const f32x4 z = act4<decltype(kind)::value>(v[q] + bias) + r[q];
+        const int row = row0 + q * kPassRows;
+        if (row < p.m && whole) store4<E>(p.y, p.y_dtype == FCV_LM_F32, (int64_t)row * p.ldy + col, z);
+      }
     }
   });
 }
@@ -314,8 +300,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const Args a) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) v += u[s];
   }
-  const bool vec = a.vec && col + 3 < p.n;
-  finish4<E>(p, vec, row, col, v, bias4<E>(p, vec, col), residual4<E>(p, vec, row, col));
+  const bool whole = col + 3 < p.n;
+  finish4<E>(p, a.vec, row, col, v, bias4<E>(p, whole, col), residual4<E>(p, whole, row, col));
 }
 
 inline int element_size(int dtype) { return dtype == FCV_LM_F32 ? 4 : 2; }

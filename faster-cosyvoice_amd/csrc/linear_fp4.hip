@@ -124,8 +124,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void linear_fp4_few_kernel(const
       *reinterpret_cast<f32x4*>(f.a.part + ((int64_t)blockIdx.y * p.m + m) * f.a.part_ld + n) = v;
       continue;
     }
-    const bool vec = f.a.vec && n + 3 < p.n;
-    finish4<E>(p, vec, m, n, v, bias4<E>(p, vec, n), residual4<E>(p, vec, m, n));
+    const bool whole = n + 3 < p.n;
+    finish4<E>(p, f.a.vec, m, n, v, bias4<E>(p, whole, n), residual4<E>(p, whole, m, n));
   }
 }
 
