@@ -514,7 +514,8 @@ int check(const FcvFp4Linear* p) {
 // Which kernel, and into how many ranges K is cut: the least of estimates in us, fits to measurements.
 // Tiles:  rounds (spans span_us + tile_us) + 2.9,   rounds = blocks over the CUs, `per_cu` each, rounded up;
 //   span_us of full rounds at K 4096 (alone: one block a CU of those that share one).  32 x 4096 x 16384 by
-//   tiles of 64 x 64 23, by few rows 19.
+//   tiles of 64 x 64 23, by few rows 19.  By tiles of 128 x 256, 192 x 256 and 256 x 256 9184 x 1024 x 2048 take
+//   61, 54 and 64 us, 2048 x 4096 x 4096 72, 84 and 88, 8192 x 4096 x 8192 545, 542 and 464.
 // Few rows, up to 32:  2.9 + what W takes, 3.5 TB/s from all CUs or 18 B/ns to one, + 21 ns for each KB of x
 //   that a CU reads.  In us by blocks of 16, 32 and 64 rows of W: 1 x 4096 x 4096 5.3, 7.2 and 11; 32 x 4096 x
 //   16384 39, 26 and 19; 32 x 4096 x 4096 11.8, 13.5 and 17.5, with K in 1, 2 and 4 ranges 11.8, 10.7 and 9.8.
@@ -522,7 +523,7 @@ int check(const FcvFp4Linear* p) {
 // A cut K adds the join's 1.8 (3.5 to few rows: what the second launch takes of the host, which calls that
 // short wait for) and its sums' way, an x off its boundaries the pass that lays it out (the same
 // for every tile).
-enum Form { kFew, kTile64, kTile64x128, kTile128, kTile128x256, kTile256 };
+enum Form { kFew, kTile64, kTile64x128, kTile128, kTile128x256, kTile192x256, kTile256 };
 
 struct Shape {
   Form form;
@@ -532,6 +533,7 @@ struct Shape {
 constexpr Shape kShapes[] = {
     {kTile64, 64, 64, 1, 0.60f, 0.62f, 1.2f},    {kTile64x128, 64, 128, 2, 0.76f, 1.25f, 1.5f},
     {kTile128, 128, 128, 2, 1.50f, 2.24f, 1.5f}, {kTile128x256, 128, 256, 1, 2.08f, 2.08f, 2.0f},
+    {kTile192x256, 192, 256, 1, 2.75f, 2.75f, 3.0f},
     {kTile256, 256, 256, 1, 3.56f, 3.56f, 4.0f}};
 constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16};
 constexpr int kMinSpans = 2;  // of a range
@@ -651,6 +653,7 @@ void launch(const FcvFp4Linear& p, const Plan& plan, void* workspace, hipStream_
     case kTile64x128: launch_tiles<E, Fp4Tile<64, 128, 2, 2, 3, 128>>(f, stream); break;
     case kTile128: launch_tiles<E, Fp4Tile<128, 128, 2, 2, 3, 64>>(f, stream); break;
     case kTile128x256: launch_tiles<E, Fp4Tile<128, 256, 2, 4, 3, 64>>(f, stream); break;
+    case kTile192x256: launch_tiles<E, Fp4Tile<192, 256, 2, 4, 3, 64>>(f, stream); break;
     case kTile256: launch_tiles<E, Fp4Tile<256, 256, 2, 4, 3, 64>>(f, stream); break;
   }
   if (a.splits > 1) {

@@ -83,7 +83,7 @@ size_t fcv_fp4_linear_workspace_bytes(const FcvFp4Linear* args);
 int fcv_fp4_linear(const FcvFp4Linear* args, void* workspace, size_t workspace_bytes,
                    hipStream_t stream);
 /* Which kernel a call takes and into how many ranges it cuts k, for logs and tests.  form: 0 up to 32 rows,
- * else tiles of 1 64 x 64, 2 64 x 128, 3 128 x 128, 4 128 x 256, 5 256 x 256. */
+ * else tiles of 1 64 x 64, 2 64 x 128, 3 128 x 128, 4 128 x 256, 5 192 x 256, 6 256 x 256. */
 int fcv_fp4_linear_plan(const FcvFp4Linear* args, int32_t* form, int32_t* ranges);
 
 /* Pages: a pool [pages][n_kv_heads][page bytes], strides page_stride and head_stride in bytes,

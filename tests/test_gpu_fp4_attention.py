@@ -335,3 +335,15 @@ def test_sequences_of_many_lengths(fcv, batch, heads, n_kv, d):
     check(fcv, st, "many lengths")
     st["lengths"][batch // 3], st["lengths"][5] = 1 << 30, -7
     check(fcv, st, "bounds", max_length=2310)
+
+
+def test_ordered_sequences_in_ranges(fcv):
+    """Longest first, their pages in ranges: few long sequences among short ones, new tokens of one to five."""
+    g = torch.Generator().manual_seed(17)
+    news = torch.randint(1, 6, (32,), generator=g).tolist()
+    keys = torch.randint(5, 300, (32,), generator=g).tolist()
+    keys[7], keys[20], keys[31] = 4500, 4401, 4500
+    st = make(news, keys, 16, 8, 64, torch.float16)
+    out, lse = check(fcv, st, "ranges", max_q=5)
+    again = run(fcv, st, max_q=5, max_length=300)  # a bound that the long ones pass
+    compare(again, lse, st, "passed")

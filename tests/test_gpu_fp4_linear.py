@@ -63,7 +63,7 @@ def test_sizes(fcv, m, k, n, dtype):
 # tiles of every shape, K ending inside a slice, rows and columns inside a tile
 TILES = [(77, 904, 601), (600, 1000, 4096), (2000, 4104, 2000), (19000, 200, 381), (2048, 1032, 4096),
          (4600, 1000, 2000), (4096, 1000, 4090), (4090, 1000, 4100), (8, 4104, 130), (300, 4104, 70),
-         (709, 4101, 67), (2717, 3277, 787), (2740, 7883, 149), (2708, 3426, 1455)]
+         (709, 4101, 67), (2717, 3277, 787), (2740, 7883, 149), (2708, 3426, 1455), (3069, 4194, 1301)]
 
 
 @pytest.mark.parametrize("m,k,n", TILES)
