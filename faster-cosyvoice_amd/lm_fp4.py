@@ -50,11 +50,11 @@ def _pack(layout: struct.Struct, *args) -> bytes:
 
 def _bytes_matrix(t: torch.Tensor, name: str, rows: int, columns: int, like: torch.Tensor):
     """Address and row stride of a matrix of bytes."""
-    if t.dtype != torch.uint8 or t.device != like.device or t.shape != (rows, columns) \
-            or (columns > 1 and t.stride(1) != 1):
+    if t.dtype is not torch.uint8 or t.shape != (rows, columns) or t.get_device() != like.get_device() \
+            or (columns > 1 and t.stride()[1] != 1):
         raise ValueError(f"{name} must be a uint8 matrix {(rows, columns)} on {like.device} whose rows "
                          f"are contiguous, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr(), t.stride(0) if rows > 1 else columns
+    return t.data_ptr(), t.stride()[0] if rows > 1 else columns
 
 
 def quantize_fp4(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -92,10 +92,10 @@ def fused_linear_fp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     ``fused_linear``'s.  Rows of codes start on 16-byte boundaries; those of ``x`` may lie at any stride
     (many rows go faster where they start on 16-byte boundaries and K is a multiple of 8)."""
     code = _dtype(x, "x")
-    device = x.device
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must be rows of at least one element, got {tuple(x.shape)}")
-    k = x.shape[-1]
+    size = x.shape
+    if not size or size[-1] < 1:
+        raise ValueError(f"x must be rows of at least one element, got {tuple(size)}")
+    k = size[-1]
     groups = (k + GROUP - 1) // GROUP
     if codes.dim() != 2 or codes.shape[0] < 1:
         raise ValueError(f"codes must be a matrix of bytes, got {tuple(codes.shape)}")
@@ -106,10 +106,10 @@ def fused_linear_fp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}")
-    shape = (m, n) if x.dim() == 2 else (*x.shape[:-1], n)
+    shape = (m, n) if len(size) == 2 else (*size[:-1], n)
     given = out is not None
     if not given:
-        if out_dtype is None or out_dtype == x.dtype:
+        if out_dtype is None or out_dtype is x.dtype:
             out_code = code
         elif out_dtype == torch.float32:
             out_code = _F32
@@ -158,9 +158,9 @@ def fused_linear_fp4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     fn = _entry("fcv_fp4_linear", 3)
     if need:
         ws = x.new_empty(need, dtype=torch.uint8)
-        _launch(fn, device.index, args, ws.data_ptr(), need)
+        _launch(fn, x.get_device(), args, ws.data_ptr(), need)
     else:
-        _launch(fn, device.index, args, None, 0)
+        _launch(fn, x.get_device(), args, None, 0)
     return out
 
 
@@ -180,12 +180,13 @@ def new_fp4_pages(n_pages: int, n_kv_heads: int, head_dim: int, *, layers: int |
 
 def _pool(pages: torch.Tensor, device: torch.device):
     """Pages, key heads, head dim and strides of a layer's pool."""
-    if pages.dtype != torch.uint8 or pages.device != device or pages.dim() != 3 \
-            or pages.shape[2] not in _HEAD_DIMS or pages.numel() == 0 or pages.stride(2) != 1:
+    if pages.dtype is not torch.uint8 or pages.device != device or pages.dim() != 3 \
+            or pages.shape[2] not in _HEAD_DIMS or pages.numel() == 0 or pages.stride()[2] != 1:
         raise ValueError("pages must be a uint8 tensor [pages, kv heads, page bytes] of new_fp4_pages on "
                          f"{device}, got {pages.dtype} {tuple(pages.shape)} on {pages.device}")
     n_pages, n_kv, size = pages.shape
-    return n_pages, n_kv, _HEAD_DIMS[size], pages.stride(0), pages.stride(1)
+    page_stride, head_stride, _ = pages.stride()
+    return n_pages, n_kv, _HEAD_DIMS[size], page_stride, head_stride
 
 
 def _reach(pages: torch.Tensor) -> int:
@@ -299,22 +300,24 @@ def paged_attention_fp4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
     ``[T, heads]``."""
     code = _dtype(q, "q")
     n_pages, n_kv, dim, page_stride, head_stride = _pool(pages, q.device)
-    if q.dim() != 3 or q.shape[2] != dim or q.shape[1] % n_kv or q.shape[1] < 1:
+    size = q.shape
+    if len(size) != 3 or size[2] != dim or size[1] % n_kv or size[1] < 1:
         raise ValueError(f"q must be [tokens, heads, {dim}] with heads a multiple of {n_kv}, got "
-                         f"{tuple(q.shape)}")
-    if q.stride(2) != 1:
+                         f"{tuple(size)}")
+    qs = q.stride()
+    if qs[2] != 1:
         raise ValueError("q's last dimension must be contiguous")
-    tokens, heads, _ = q.shape
+    tokens, heads, _ = size
     batch = lengths.numel()
     if batch < 1:
         raise ValueError("lengths is empty")
     len_ptr = _indices(lengths, "lengths", batch, q)
-    if table.dtype != torch.int32 or table.device != q.device or table.dim() != 2 \
-            or table.shape[0] != batch or table.shape[1] < 1 \
-            or (table.shape[1] > 1 and table.stride(1) != 1):
+    sizes, ts = table.shape, table.stride()
+    if table.dtype is not torch.int32 or table.device != q.device or len(sizes) != 2 \
+            or sizes[0] != batch or sizes[1] < 1 or (sizes[1] > 1 and ts[1] != 1):
         raise ValueError(f"table must be an int32 matrix of {batch} rows on {q.device} whose rows are "
-                         f"contiguous, got {table.dtype} {tuple(table.shape)} on {table.device}")
-    max_pages = table.shape[1]
+                         f"contiguous, got {table.dtype} {tuple(sizes)} on {table.device}")
+    max_pages = sizes[1]
     cu_ptr = 0 if cu_q is None else _indices(cu_q, "cu_q", batch + 1, q)
     if cu_q is None:
         if tokens % batch:
@@ -325,7 +328,7 @@ def paged_attention_fp4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
         max_q = max(tokens - batch + 1, 1)
     given = out is not None
     if not given:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(size)
     elif out.dtype != q.dtype or out.device != q.device or out.shape != q.shape \
             or out.stride(2) != 1:
         raise ValueError(f"out must be a {q.dtype} tensor {tuple(q.shape)} on {q.device}, its last "
@@ -335,7 +338,7 @@ def paged_attention_fp4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if tokens == 0:
         return (out, lse) if return_lse else out
-    qs, os = q.stride(), out.stride()
+    os = out.stride()
     q_ptr, out_ptr, pages_ptr = q.data_ptr(), out.data_ptr(), pages.data_ptr()
     if given:
         rows = (tokens - 1, heads - 1)
@@ -345,7 +348,7 @@ def paged_attention_fp4(q: torch.Tensor, pages: torch.Tensor, table: torch.Tenso
         _check_apart(out, out_ptr, 2 * (rows[0] * os[0] + rows[1] * os[1] + dim), inputs)
     args = _pack(_ATTENTION, q_ptr, pages_ptr, table.data_ptr(), len_ptr, cu_ptr, out_ptr,
                  0 if lse is None else lse.data_ptr(), qs[0], qs[1], os[0], os[1], page_stride,
-                 head_stride, table.stride(0) if batch > 1 else max_pages, tokens, batch, heads,
+                 head_stride, ts[0] if batch > 1 else max_pages, tokens, batch, heads,
                  n_kv, dim, n_pages, max_pages, max_q,
                  PAGE * max_pages if max_length is None else max_length, code,
                  dim ** -0.5 if scale is None else scale)
