@@ -210,17 +210,17 @@ def qk_norm_rope_fp4(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tens
     given, which may be their own columns of ``qkv`` and overlaps nothing else."""
     code = _dtype(qkv, "qkv")
     n_pages, n_kv, dim, page_stride, head_stride = _pool(pages, qkv.device)
-    if qkv.dim() != 2 or n_heads < 1 or qkv.shape[1] != (n_heads + 2 * n_kv) * dim:
-        raise ValueError(f"qkv must be [tokens, {(n_heads + 2 * n_kv) * dim}], got "
-                         f"{tuple(qkv.shape)}")
-    tokens, qkv_row = _rows(qkv, "qkv", qkv.shape[1])
+    width = (n_heads + 2 * n_kv) * dim
+    if qkv.dim() != 2 or n_heads < 1 or qkv.shape[1] != width:
+        raise ValueError(f"qkv must be [tokens, {width}], got {tuple(qkv.shape)}")
+    tokens, qkv_row = _rows(qkv, "qkv", width)
     pos_ptr = _indices(positions, "positions", tokens, qkv)
     row_ptr = _indices(cache_rows, "cache_rows", tokens, qkv)
+    index, table = qkv.get_device(), cos.shape
     for t, name in ((cos, "cos"), (sin, "sin")):
-        if t.dtype != torch.float32 or t.device != qkv.device or t.dim() != 2 \
+        if t.dtype is not torch.float32 or t.get_device() != index or t.dim() != 2 \
                 or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float32 table on {qkv.device}")
-    table = cos.shape
     if table != sin.shape or table[0] < 1:
         raise ValueError(f"cos {tuple(table)} and sin {tuple(sin.shape)} must be equal tables")
     w_code, qw_ptr, kw_ptr = code, 0, 0
@@ -244,16 +244,16 @@ def qk_norm_rope_fp4(qkv: torch.Tensor, positions: torch.Tensor, cos: torch.Tens
     if tokens == 0:
         return out
     qkv_ptr, out_ptr, pages_ptr = qkv.data_ptr(), out.data_ptr(), pages.data_ptr()
-    q_row = out.stride(0) if tokens > 1 else n_heads * dim
+    q_row = n_heads * dim if not given or tokens == 1 else out.stride(0)
     if given:
         inputs = [("pages", pages, pages_ptr, _reach(pages))]
         if out_ptr != qkv_ptr or (tokens > 1 and q_row != qkv_row):
-            inputs.append(("qkv", qkv, qkv_ptr, 2 * ((tokens - 1) * qkv_row + qkv.shape[1])))
+            inputs.append(("qkv", qkv, qkv_ptr, 2 * ((tokens - 1) * qkv_row + width)))
         _check_apart(out, out_ptr, 2 * ((tokens - 1) * q_row + n_heads * dim), inputs)
     args = _pack(_APPEND, qkv_ptr, pos_ptr, row_ptr, cos.data_ptr(), sin.data_ptr(), qw_ptr, kw_ptr,
                  out_ptr, pages_ptr, qkv_row, q_row, page_stride, head_stride, tokens, n_heads,
                  n_kv, dim, 2 * table[1], table[0], n_pages, code, w_code, bool(interleaved), eps)
-    _launch(_entry("fcv_fp4_append", 1), qkv.device.index, args)
+    _launch(_entry("fcv_fp4_append", 1), index, args)
     return out
 
 
