@@ -51,11 +51,6 @@ __device__ __forceinline__ float across_max(float v) {  // over the lane blocks 
 }
 __device__ __forceinline__ float across_sum(float v) { return swap32_sum(swap16_sum(v)); }
 
-template <int kCtrl>
-__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xF, 0xF, false);
-}
-
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
   typedef __bf16 b2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b});
@@ -414,28 +409,16 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
 // 16-bit numbers once, in LDS: keys [64][D], values [D][64] in the order of the S^T tiles' rows, so that a
 // lane's weights are its right operand again.  Two pages' room: one barrier a page, with the next page's
 // conversions beside this one's first product, and a step's weights between the products of the one before.
-// m follows a row's maximum only where it has risen by kSlack (a power of two: weights up to 2^1.75), so that
-// few pages scale the sums; the other tiles' m is the maximum.
+// m is set kSlack above a row's maximum, and again only where a score passes it (weights are 2^-1.75 to 1 of the
+// row's largest), so that few pages scale the sums; the other tiles' m is the maximum.
 //
-// Bound: instructions.  4000 tokens of 32 heads of 128 over 8 run at 0.76 PFLOP/s in bf16 (173 us) and 0.62 in
-// fp16, 4 texts of 300 to 1024 behind 4096 keys at 0.72 (189 us) and 0.58, 7000 of 14 heads of 64 over 2 at 0.54:
-// the matrix pipes are busy for a third of it (27 % of the time, CUs 80 %: texts), and some 300 vector
-// instructions to a wave's page, 32 of them exponentials at a quarter of the rate, take their turns with the
-// products of the CU's other workgroup.
-//
-// bf16.  Results are off by 2^-8 from their rounding, and one fp16 number, off by 2^-11, is all that a weight
-// times its value's scale goes in as, times 2^kTop and over 2^u (u as a scale byte): one below 2^-28 of
-// 2^u loses bits, one below 2^-39 is 0.  u is the row's, and as large as the page's largest scale, or as the
-// row's largest product of a weight and a scale with kRoom over it where that is less: values that a row hides,
-// or weighs next to nothing, do not set it.  A row's u follows its m's rise (`owed`) once that is more than
-// kRoom.  LDS holds the scales over the largest scale of all pages so far; the factor between the two goes into
-// the exponent, and out of l's terms again.
-// fp16.  Weights go in as two bf16 numbers as above.
+// Bound: instructions.  4000 tokens of 32 heads of 128 over 8 run at 0.65 PFLOP/s (200 us), 4 texts of 300 to 1024
+// behind 4096 keys at 0.60 (210 us), 7000 of 14 heads of 64 over 2 at 0.48 (181 us), in bf16 and fp16 alike.  A
+// weight in one 16-bit number, half of the second product, would take 181 instead of 210 us for the texts, but its
+// rounding shows where values cancel, and fp16's range does not hold weights times any scale.
 //
 // A value without a scale (its byte is 255) lies in LDS as zeros, and rows that see it become NaN at their end.
-constexpr int kTop = 14;
 constexpr float kSlack = 1.75f;
-constexpr int kRoom = 8;
 template <int D>
 __device__ __forceinline__ int key_chunk(int row, int c) {  // 16 rows read at one chunk touch all banks
   return D == 128 ? c ^ (row & 15) : c ^ ((row >> 1) & 7);
@@ -446,16 +429,13 @@ template <class E, int D>
 __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArgs a) {
   using P = Page<D>;
   constexpr int kRows = kTileRows, kSteps = D / 16, kDT = D / 32;
-  constexpr bool kOne = std::is_same<E, Bf16>::value;  // one fp16 number a weight
-  // products before the other workgroup's vector instructions: 4000 tokens of 32 heads of 128 182 -> 173 us, but
-  // 7000 of 14 of 64 164 -> 173
+  // products before the other workgroup's vector instructions: 4 texts of 32 heads of 128 210 -> 204 us, but 7000
+  // tokens of 14 of 64 179 -> 186
   constexpr bool kFirst = D == 128;
-  using V = typename std::conditional<kOne, Half, Bf16>::type;
   __shared__ __attribute__((aligned(16))) short sk[2][kPage * D];
   __shared__ __attribute__((aligned(16))) short sv[2][D * kPage];
   __shared__ __attribute__((aligned(16))) f32x4 svs[2][2][kPage / 8];  // the values' scales, by half waves
-  // of a page: the scale byte that its values' are told over (kOne), and which keys' values have no scale
-  __shared__ __attribute__((aligned(16))) uint32_t about[2][4];
+  __shared__ __attribute__((aligned(8))) uint32_t without[2][2];  // which keys' values have no scale
   const FcvFp4Attention& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -508,8 +488,6 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
     float poison = 1.0f;  // or NaN, of the row
-    float owed = 0.0f;
-    int unit = 0, mine = 1;     // kOne: the largest scale byte of the pages so far, and that of the row's sums
 
     // a thread's share of a page: D / 4 codes of a key, 16 bytes of a byte row of the values
     uint32_t kw[D / 32], ks, vsw = 0;
@@ -532,7 +510,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       if (tid < kPage / 4)
         vsw = *reinterpret_cast<const uint32_t*>(page + P::kValueScales + (uint32_t)tid * 4);
     };
-    auto unpack = [&](int buf, int page, bool here) {
+    auto unpack = [&](int buf) {
       const int key = tid / 4;
 #pragma unroll
       for (int j = 0; j < D / 32; ++j)
@@ -548,10 +526,10 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
           const uint32_t wo = (w0 >> 4 & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
           *reinterpret_cast<s16x8*>(
               &sv[buf][2 * pair * kPage + value_chunk(2 * pair, 2 * step + h) * 8]) =
-              fp4_octet<V>(we, kOne ? 1.0f : kHeld<E>);
+              fp4_octet<Bf16>(we, kHeld<E>);
           *reinterpret_cast<s16x8*>(
               &sv[buf][(2 * pair + 1) * kPage + value_chunk(2 * pair + 1, 2 * step + h) * 8]) =
-              fp4_octet<V>(wo, kOne ? 1.0f : kHeld<E>);
+              fp4_octet<Bf16>(wo, kHeld<E>);
         }
       }
       if (tid < kPage / 4) {  // 16 lanes of one row, four keys each
@@ -563,26 +541,10 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
           bad[j] = (uint32_t)__ballot(byte[j] == 255);
           byte[j] = byte[j] == 255 ? 0 : byte[j];
         }
-        if constexpr (kOne) {
-          const int left = here ? length - page * kPage - 4 * tid : 0;  // keys that are the sequence's
-          uint32_t top = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (j >= left) byte[j] = 0;
-            top = max(top, (uint32_t)byte[j]);
-          }
-          top = max(top, dpp_u<0xB1>(top));
-          top = max(top, dpp_u<0x4E>(top));
-          top = max(top, dpp_u<0x141>(top));
-          top = max(top, dpp_u<0x140>(top));
-          unit = max(unit, (int)top);
-          if (tid == 0) about[buf][3] = top;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) byte[j] = max(byte[j] + 127 + kTop - unit, 0);
+        if (tid == 0) {
+          without[buf][0] = bad[0] | bad[1] << 16;
+          without[buf][1] = bad[2] | bad[3] << 16;
         }
-        if (tid == 0)
-          for (int j = 0; j < 3; ++j)
-            about[buf][j] = j == 0 ? (uint32_t)unit : bad[2 * j - 2] | bad[2 * j - 1] << 16;
         svs[buf][tid % 2][tid / 2] =
             f32x4{scale_of(byte[0]), scale_of(byte[1]), scale_of(byte[2]), scale_of(byte[3])};
       }
@@ -620,7 +582,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
               *reinterpret_cast<const s16x8*>(&sv[buf][r * kPage + value_chunk(r, 2 * st + fh) * 8]);
         }
       };
-      const u32x4 facts = *reinterpret_cast<const u32x4*>(about[buf]);
+      const u32x2 none = *reinterpret_cast<const u32x2*>(without[buf]);
       if (!__all(limit >= (page + 1) * kPage)) {  // hidden keys have no score
         asm volatile("");  // a branch: the compiler would do this for every page
         const int seen = limit - page * kPage - 4 * fh;
@@ -630,12 +592,12 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
           for (int j = 0; j < 4; ++j)
             if (8 * g + j >= seen) s[g / 4][g % 4 * 4 + j] = -__builtin_inff();
       }
-      const uint32_t bad = __builtin_amdgcn_readfirstlane(facts[1] | facts[2]);
+      const uint32_t bad = __builtin_amdgcn_readfirstlane(none[0] | none[1]);
       if (bad != 0) {  // a value without a scale is in LDS as zeros: NaN for the rows that see it
         const int seen = limit - page * kPage;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t lanes = facts[1 + j / 2] >> (16 * (j % 2)) & 0xffffu;
+          const uint32_t lanes = none[j / 2] >> (16 * (j % 2)) & 0xffffu;
           const int n = min(max((seen - j + 3) >> 2, 0), 16);
           if (lanes & ((1u << n) - 1)) poison = __builtin_nanf("");
         }
@@ -650,56 +612,15 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
                                                         false);
         top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * scale;
       }
-      float shrink = 1.0f;  // of the sums
-      if (__any(top > m + kSlack)) {
-        const float next = fmaxf(m, top);
-        const float rise = next == -__builtin_inff() ? 0.0f : next - m;
+      if (__any(top > m)) {
+        const float next = top > m ? top + kSlack : m;
+        const float shrink = top > m ? hw_exp2(m - next) : 1.0f;  // of the sums
         m = next;
-        l *= hw_exp2(-rise);
-        float down = 0.0f;
-        if constexpr (kOne) {
-          owed += fminf(rise, 256.0f);
-          if (owed > kRoom) {
-            const int was = mine;
-            mine = min(mine, max(mine - (int)owed, max((int)facts[0] - 125, 1)));
-            down = (float)(was - mine);
-            owed = 0.0f;
-          }
-        }
-        shrink = hw_exp2(down - rise);
-      }
-      float base = m == -__builtin_inff() ? 0.0f : m, back = 1.0f;  // back: out of l's terms
-      if constexpr (kOne) {
-        const int all = __builtin_amdgcn_readfirstlane(facts[0]);
-        const int here = __builtin_amdgcn_readfirstlane(facts[3]);
-        if (__any(max(here, all - 125) > mine && m > -__builtin_inff())) {
-          // the row's largest weight with its value's scale, as a scale byte
-          float most = -__builtin_inff();
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const f32x4 v = svs[buf][fh][g];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float byte = (float)(__float_as_uint(v[j]) >> 23);
-              most = fmaxf(most, fmaf(s[g / 4][g % 4 * 4 + j], scale, byte));
-            }
-          }
-          const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false,
-                                                          false);
-          most = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) - base + (all - 127 - kTop);
-          const int want = min(here, (int)fmaxf(most, -512.0f) + kRoom), was = mine;
-          mine = max(max(mine, want), all - 125);
-          owed = mine > was ? 0.0f : owed;
-          shrink *= scale_of((uint32_t)max(127 + was - mine, 0));
-        }
-        // the weights' scales are over `all`: 2^(all - mine) goes in through the exponent, and out of l's
-        base -= (float)(all - mine);
-        back = hw_exp2((float)(mine - all));
-      }
-      if (__any(shrink != 1.0f)) {
+        l *= shrink;
 #pragma unroll
         for (int d = 0; d < kDT; ++d) o[d] *= shrink;
       }
+      const float base = m == -__builtin_inff() ? 0.0f : m;
       u32x4 hi[2], lo[2];
       auto weights = [&](int st) {  // of 16 keys: words 2 st and 2 st + 1 of the lane's eight
         // the scales of the lane's keys: 8 g + 4 fh + j is element j of vs[g % 2]
@@ -713,17 +634,13 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
           for (int i = 0; i < 2; ++i) {
             const int g = 2 * st + i;
             const float e = hw_exp2(fmaf(s[g / 4][g % 4 * 4 + j], scale, -base));
-            l = kOne ? fmaf(e, back, l) : l + e;
+            l += e;
             w[i] = e * vs[i][j];
           }
-          if constexpr (kOne) {
-            hi[st & 1][j] = __builtin_bit_cast(uint32_t, f2h2(w[0], w[1]));
-          } else {
-            const uint32_t u = bf16_pair(w[0], w[1]);
-            hi[st & 1][j] = u;
-            lo[st & 1][j] =
-                bf16_pair(w[0] - __uint_as_float(u << 16), w[1] - __uint_as_float(u & 0xffff0000u));
-          }
+          const uint32_t u = bf16_pair(w[0], w[1]);
+          hi[st & 1][j] = u;
+          lo[st & 1][j] =
+              bf16_pair(w[0] - __uint_as_float(u << 16), w[1] - __uint_as_float(u & 0xffff0000u));
         }
       };
       load_vf(0);
@@ -736,15 +653,15 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
         // this step's products, and between them the next one's weights
 #pragma unroll
         for (int d = 0; d < kDT; ++d) {
-          o[d] = V::mfma32(vf[st & 1][d], __builtin_bit_cast(s16x8, hi[st & 1]), o[d]);
-          if constexpr (!kOne) o[d] = V::mfma32(vf[st & 1][d], __builtin_bit_cast(s16x8, lo[st & 1]), o[d]);
+          o[d] = Bf16::mfma32(vf[st & 1][d], __builtin_bit_cast(s16x8, hi[st & 1]), o[d]);
+          o[d] = Bf16::mfma32(vf[st & 1][d], __builtin_bit_cast(s16x8, lo[st & 1]), o[d]);
         }
         if (st < 3) {
           weights(st + 1);
 #pragma unroll
-          for (int i = 0; i < (kOne ? 1 : 2) * kDT; ++i) {
+          for (int i = 0; i < 2 * kDT; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
-            __builtin_amdgcn_sched_group_barrier(0x002, (kOne ? 36 : 60) / ((kOne ? 1 : 2) * kDT), 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 60 / (2 * kDT), 0);
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -758,7 +675,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       };
       int id = number(page0), next = number(page0 + 1);
       load(id);
-      unpack(0, page0, id >= 0);
+      unpack(0);
       load(next);
       for (int page = page0; page < page1; ++page) {
         const int buf = (page - page0) & 1;
@@ -767,7 +684,7 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
         const bool sees_it = id >= 0 && page * kPage < reach;
         if (sees_it)
           for (int j = 0; j < 2; ++j) load_kf(buf, j);
-        unpack(buf ^ 1, page + 1, next >= 0);
+        unpack(buf ^ 1);
         load(after);
         if (sees_it) {
           if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
@@ -781,12 +698,8 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_tile_kernel(const AttendArg
       }
     }
     l = swap32_sum(l);
-    {  // back to the units of the other kernel's sums, in two steps that do not leave fp32's range
-      const float f = kOne ? poison * (kHeld<E> / (1 << kTop)) : poison;
-      const float g = kOne ? scale_of((uint32_t)mine) : 1.0f;
 #pragma unroll
-      for (int d = 0; d < kDT; ++d) o[d] = o[d] * f * g;
-    }
+    for (int d = 0; d < kDT; ++d) o[d] *= poison;
     if (there) {
       const int64_t at = (int64_t)(first + token) * p.n_heads + head;
       if (a.splits > 1) {
@@ -927,9 +840,10 @@ Plan plan_of(const FcvFp4Attention& p) {
   const int group = p.n_heads / p.n_kv_heads;
   const int64_t most_rows = (int64_t)std::min(p.max_q, p.tokens) * group;
   // Tiles of 128 rows where they fill the card, which takes more of heads of 64, whose pages are short.  Heads of
-  // 128, 32 over 8, by tiles of 128 and of 16 rows: 4000 tokens (1000 tiles) 173 and 304 us, 2000 (500) 63 and
-  // 98, 8 x 128 behind a cache (256) 80 and 98, 1000 (250) 34 and 36, 4 x 128 (128) 79 and 54.  Heads of 64,
-  // 14 over 2: 7000 (766) 161 and 229, 16 x 300 (544) 112 and 106, 8 x 300 (272) 77 and 64, 2000 (220) 52 and 28.
+  // 128, 32 over 8, by tiles of 128 and of 16 rows: 4000 tokens (1000 tiles) 202 and 329 us, 2000 (500) 73 and
+  // 96, 8 x 128 behind 4000 keys (256) 119 and 156, 1000 (250) 36 and 36, 4 x 128 behind 2000 (128) 54 and 47.
+  // Heads of 64, 14 over 2: 7000 (766) 180 and 230, 20 x 300 behind 3000 keys (680) 163 and 179, 16 x 300 (544)
+  // 153 and 135, 8 x 300 (272) 101 and 75, 2000 (220) 55 and 30.
   const int64_t many = (most_rows + kTileRows - 1) / kTileRows * p.batch * p.n_kv_heads;
   const int rows = most_rows <= 8 ? 8 : many < (p.head_dim == 128 ? kCus : 5 * kCus / 2) ? 16 : kTileRows;
   const int64_t all = std::max<int64_t>((most_rows + rows - 1) / rows, 1);
@@ -955,8 +869,8 @@ Plan plan_of(const FcvFp4Attention& p) {
   if (rows == kTileRows) {
     // Time in pages of a workgroup that shares its CU; one that has it alone takes 0.63 of it, and a tile's
     // sums of one range cost 0.02.  8 x 128 tokens of 32 heads of 128 over 8 (256 tiles) behind 16000 keys take
-    // 410 us in one range, 331, 343 and 353 in two, three and four, behind 4000 keys 110 and 113; 10 x 128 (320)
-    // behind 8000 288, 264 and 249; 500 tiles behind 8000 273 and 308, 640 behind 16000 906, 805 and 838.
+    // 430 us in one range, 381, 412 and 393 in two, three and four, behind 4000 keys 119 and 121; 10 x 128 (320)
+    // behind 8000 309, 303 and 286; 520 tiles behind 8000 501, 450 and 428, 640 behind 16000 1052, 933 and 958.
     // Tiles whose keys are new ones too have lengths of their own, and the short ones fill the ends.
     const int most_ranges = p.max_q <= p.max_length / 2 ? 3 : 1;
     double best = 0.0;
@@ -974,7 +888,7 @@ Plan plan_of(const FcvFp4Attention& p) {
   const int splits = (pages + per - 1) / per;
   // The longest sequences first, where their workgroups are long: 64 of 2000 to 8000 keys 84 us in their own
   // order, 76 so; 100 of 1000 to 7000 115 and 96; 30 x 100 to 300 tokens behind 500 to 3000, 14 over 2 of 64,
-  // 128 and 101.  It costs a workgroup about a microsecond: 8 of 500 to 7000 in ranges of 14 pages 17.0 and 18.4.
+  // 168 and 131.  It costs a workgroup about a microsecond: 8 of 500 to 7000 in ranges of 14 pages 17.0 and 18.4.
   int shift = -1;
   if (p.batch >= (rows == kTileRows ? 8 : 2) && per >= 32 && blocks * splits > kCus)
     for (shift = 6; pages * (int64_t)kPage >> shift >= 1 << kKeyBits; ++shift) {}
