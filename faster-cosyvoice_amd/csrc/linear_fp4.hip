@@ -20,7 +20,15 @@ struct Fp4Args {
   Args a;  // the epilogue's fields, x, the ranges of K
   const uint8_t *codes, *scales;
   int64_t ld_codes, ld_scales;
+  int32_t k;  // of the weights: a.p.k may be that of an x laid out
 };
+
+// The codes of a word that holds elements at .. at + 7 of a row of k: those past k as zeros.  x is 0 there, but a
+// scale can make an infinity of a code, and NaN of its product.
+__device__ __forceinline__ uint32_t codes_below(uint32_t w, int at, int k) {
+  const int n = min(max(k - at, 0), 8);
+  return n == 8 ? w : w & ((1u << (4 * n)) - 1);
+}
 
 // ---- few rows: the weights straight into registers -------------------------------------------------
 //
@@ -97,6 +105,13 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void linear_fp4_few_kernel(const
       const int span = span0 + i * kFewWaves;
       if (span >= end) break;
       if (i + 1 < kAhead && span + kFewWaves < end) load_x((i + 1) & 1, span + kFewWaves);
+      if ((span + 1) * kSpan > p.k && p.k % FCV_FP4_GROUP) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            w[i][u][j] = codes_below(w[i][u][j], span * kSpan + fb * FCV_FP4_GROUP + 8 * j, p.k);
+      }
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         const float scale = scale_of(s[i][u]);
@@ -163,7 +178,9 @@ __device__ __forceinline__ int swz_w(int r, int g) {
   return BK == 128 ? g ^ ((r >> 2) & 3) : g ^ ((r >> 3) & 1);
 }
 
-template <class E, class C>
+// kCut: K ends inside a group, whose other codes are cleared.  As a branch of one kernel that took 3 to 8 % of calls
+// without such a group (2000 x 4096 x 2000 48.2 -> 50.4 us).
+template <class E, class C, bool kCut>
 __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile_kernel(const Fp4Args f) {
   constexpr int BM = C::BM, BN = C::BN, TM = C::TM, TN = C::TN, S = C::STAGES, BK = C::BK;
   __shared__ __attribute__((aligned(1024))) char smem[C::kLds];
@@ -262,6 +279,22 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
     }
   };
 
+  // slice kt is in LDS: codes past K in the last one's last group become 0
+  auto trim = [&](int kt, int st) {
+    if constexpr (kCut) {
+      if (kt != KT - 1 || slice0 + KT != all) return;
+      const int left = f.k - (slice0 + kt) * BK, g = left / FCV_FP4_GROUP;
+      for (int row = threadIdx.x; row < BN; row += C::kThreads) {
+        u32x4* at = reinterpret_cast<u32x4*>(smem + st * C::kStage + C::kW + row * (BK / 2) + swz_w<BK>(row, g) * 16);
+        u32x4 w = *at;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = codes_below(w[q], 8 * q, left % FCV_FP4_GROUP);
+        *at = w;
+      }
+      __syncthreads();
+    }
+  };
+
   f32x16 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -324,6 +357,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
   wait_ahead<C::kCopies, S - 2>(KT - 1);
   __syncthreads();
   int kt = 0, stage = 0;
+  trim(kt, stage);
   if constexpr (C::kWhole) {
     // as in linear.hip: slice kt's operands are asked for after the barrier that publishes it and used after
     // the next one
@@ -353,6 +387,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
       __syncthreads();
       const int freed = stage;
       stage = stage == S - 1 ? 0 : stage + 1;
+      trim(kt, stage);
       load_all(set);
       if (kt + S - 1 < KT) issue(kt + S - 1, freed, 0, C::kCopies);
       mma_all(before, kt - 1);
@@ -426,6 +461,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void linear_fp4_tile
       wait_ahead<C::kCopies, S - 2>(KT - 1 - kt);
       __syncthreads();
       stage = next;
+      trim(kt, stage);
       load_w(0, stage);
       load_x(0, 0, stage);
       copies(0);
@@ -606,8 +642,11 @@ size_t workspace_bytes(const FcvFp4Linear& p, const Plan& plan) {
 template <class E, class C>
 void launch_tiles(const Fp4Args& f, hipStream_t stream) {
   const int64_t tiles = (int64_t)((f.a.p.m + C::BM - 1) / C::BM) * ((f.a.p.n + C::BN - 1) / C::BN);
-  hipLaunchKernelGGL((linear_fp4_tile_kernel<E, C>), dim3((unsigned)(tiles * f.a.splits)),
-                     dim3(C::kThreads), 0, stream, f);
+  const dim3 grid((unsigned)(tiles * f.a.splits)), block(C::kThreads);
+  if (f.k % FCV_FP4_GROUP)
+    hipLaunchKernelGGL((linear_fp4_tile_kernel<E, C, true>), grid, block, 0, stream, f);
+  else
+    hipLaunchKernelGGL((linear_fp4_tile_kernel<E, C, false>), grid, block, 0, stream, f);
 }
 
 template <class E, int MT>
@@ -634,7 +673,7 @@ void launch(const FcvFp4Linear& p, const Plan& plan, void* workspace, hipStream_
   const Args a{e, quad(p.y, p.y_dtype, p.ldy) && quad(p.residual, p.residual_dtype, p.ldr) &&
                       quad(p.bias, p.bias_dtype, 0),
                plan.splits, plan.spans, static_cast<float*>(workspace), part_ld(p.n)};
-  Fp4Args f{a, p.codes, p.scales, p.ld_codes, p.ld_scales};
+  Fp4Args f{a, p.codes, p.scales, p.ld_codes, p.ld_scales, p.k};
   if (plan.lay_x) {
     short* x = reinterpret_cast<short*>(static_cast<char*>(workspace) + part_bytes(p, plan));
     const int64_t units = p.m * (laid_ldx(p) / 8);
