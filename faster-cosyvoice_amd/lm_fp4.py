@@ -34,11 +34,12 @@ PAGE = 64    # FCV_FP4_PAGE, tokens of a page
 GROUP = 32   # FCV_FP4_GROUP, elements of a weight row or a key that share a scale
 _HEAD_DIMS = {PAGE * (d + d // 32 + 1): d for d in (64, 128)}  # by the bytes of a page's head
 
-_QUANTIZE = struct.Struct("@3Q3q3i")
+# 4x: the struct's own tail, which the library copies with the rest
+_QUANTIZE = struct.Struct("@3Q3q3i4x")
 _LINEAR = struct.Struct("@6Q5q8i")
-_APPEND = struct.Struct("@9Q4q10if")
-_READ = struct.Struct("@4Q4q5i")
-_ATTENTION = struct.Struct("@7Q7q10if")
+_APPEND = struct.Struct("@9Q4q10if4x")
+_READ = struct.Struct("@4Q4q5i4x")
+_ATTENTION = struct.Struct("@7Q7q10if4x")
 
 
 def _pack(layout: struct.Struct, *args) -> bytes:
