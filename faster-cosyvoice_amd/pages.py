@@ -30,8 +30,6 @@ def copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
     if pages.dim() < 3 or not pages.is_cuda:
         raise ValueError("pages must be a tensor [layers, pages, ...] on the GPU, got "
                          f"{tuple(pages.shape)} on {pages.device}")
-    if len(src) != len(dst):
-        raise ValueError(f"{len(src)} sources and {len(dst)} destinations")
     layers, n_pages = pages.shape[:2]
     size = pages.element_size()
     step = 1
@@ -39,16 +37,19 @@ def copy_pages(pages: torch.Tensor, src: list[int], dst: list[int]) -> None:
         if n > 1 and stride != step:
             raise ValueError(f"a page's bytes must be contiguous, got strides {pages.stride()}")
         step *= n
+    if isinstance(src, (bytes, bytearray)) or isinstance(dst, (bytes, bytearray)):
+        raise ValueError("src and dst must be lists of page numbers, not bytes")  # an array's own integers
     try:
         lists = array("i", src), array("i", dst)
     except OverflowError as e:
         raise ValueError(f"a page is outside the pool of {n_pages}") from e
     except TypeError as e:
         raise ValueError(f"src and dst must be lists of page numbers: {e}") from e
+    if len(lists[0]) != len(lists[1]):
+        raise ValueError(f"{len(lists[0])} sources and {len(lists[1])} destinations")
     _launch(_lib.load().fcv_copy_pages, pages.device.index, pages.data_ptr(), layers,
             pages.stride(0) * size, n_pages, pages.stride(1) * size if n_pages > 1 else step * size,
-            step * size, lists[0].buffer_info()[0],
-            lists[1].buffer_info()[0], len(src))
+            step * size, lists[0].buffer_info()[0], lists[1].buffer_info()[0], len(lists[0]))
 
 
 class CachePages:

@@ -1,0 +1,54 @@
+"""What ``copy_pages`` hands the library, on the CPU: as many page numbers as it says."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+
+class Pool:
+    """As much of a pool on the GPU as ``copy_pages`` looks at."""
+
+    is_cuda, shape, device = True, (2, 8, 64), type("device", (), {"index": 0})
+
+    def dim(self):
+        return 3
+
+    def element_size(self):
+        return 1
+
+    def stride(self, i=None):
+        return (512, 64, 1) if i is None else (512, 64, 1)[i]
+
+    def data_ptr(self):
+        return 1 << 40
+
+
+@pytest.fixture
+def calls(fcv, monkeypatch):
+    got = []
+    module = __import__("faster_cosyvoice_amd.pages", fromlist=["x"])
+
+    def launch(fn, index, *args):
+        src, dst, count = args[-3:]
+        got.append((count, [list((ctypes.c_int32 * count).from_address(a)) if count else [] for a in (src, dst)]))
+
+    monkeypatch.setattr(module, "_launch", launch)
+    return got
+
+
+def test_lists(fcv, calls):
+    fcv.copy_pages(Pool(), [0, 1], (6, 7))
+    fcv.copy_pages(Pool(), range(3), iter([5, 6, 7]))
+    fcv.copy_pages(Pool(), [], [])
+    assert calls == [(2, [[0, 1], [6, 7]]), (3, [[0, 1, 2], [5, 6, 7]]), (0, [[], []])]
+
+
+@pytest.mark.parametrize("src,dst", [(b"\1\0\0\0", b"\2\0\0\0"), (bytearray(4), [2, 3, 4, 5]), (b"\0\0\0\0", [5]),
+                                     ("0", "1"), ([0], [1, 2]), (range(2), iter([5])), (5, 6)])
+def test_refusals(fcv, calls, src, dst):
+    """Bytes are the machine's integers to an array: four of them are one page number, not four."""
+    with pytest.raises(ValueError):
+        fcv.copy_pages(Pool(), src, dst)
+    assert calls == []
