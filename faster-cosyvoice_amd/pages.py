@@ -64,7 +64,7 @@ class CachePages:
         book.close(request); book.compact()
 
     Copies run on the current stream when a method needs them: calls on one stream are in order.  A pool
-    that is full raises ``RuntimeError`` and changes nothing.  Driven from one thread."""
+    that is full raises ``RuntimeError`` and changes nothing, as any error does.  Driven from one thread."""
 
     def __init__(self, pages: torch.Tensor):
         if pages.dim() < 3:
@@ -111,37 +111,50 @@ class CachePages:
         session, on the pool's device.  A last page that is shared and partly filled is copied first."""
         if len(sessions) != len(counts) or len(set(sessions)) != len(sessions):
             raise ValueError("one count for each of different sessions")
-        users, need = list(self._users), 0
-        for session, count in zip(sessions, counts):  # nothing changes where the pool is too small
+        plan, need = [], 0
+        left: dict[int, int] = {}  # users of a shared last page, without those that copy it
+        for session, count in zip(sessions, counts):
             held, length = self._session(session), self._length[session]
             if count < 0:
                 raise ValueError(f"a negative count: {count}")
-            need += (length + count + PAGE - 1) // PAGE - len(held)
-            if count and length % PAGE and users[held[-1]] > 1:
-                users[held[-1]] -= 1
-                need += 1
+            copied = False
+            if count and length % PAGE:
+                users = left.get(held[-1], self._users[held[-1]])
+                copied = users > 1
+                left[held[-1]] = users - copied
+            more = (length + count + PAGE - 1) // PAGE - len(held)
+            plan.append((session, count, copied, more))
+            need += copied + more
         if need > len(self._free):
             raise RuntimeError(f"{need} pages are needed, {len(self._free)} of {len(self._users)} "
                                "are free")
-        src, dst, rows = [], [], []
-        for session, count in zip(sessions, counts):
-            held, length = self._held[session], self._length[session]
-            if count and length % PAGE and self._users[held[-1]] > 1:
-                src.append(held[-1])
-                self._users[held[-1]] -= 1
-                held[-1] = self._take()
-                dst.append(held[-1])
-            while len(held) * PAGE < length + count:
-                held.append(self._take())
-            rows += [held[i // PAGE] * PAGE + i % PAGE for i in range(length, length + count)]
-            self._length[session] = length + count
-        self._copy(src, dst)
-        return torch.tensor(rows, dtype=torch.int32, device=self.pages.device)
-
-    def _take(self) -> int:
-        page = heapq.heappop(self._free)
-        self._users[page] = 1
-        return page
+        taken = [heapq.heappop(self._free) for _ in range(need)]
+        try:  # nothing else changes before the copy is on its way and the rows are there
+            fresh = iter(taken)
+            src, dst, rows, held_now = [], [], [], []
+            for session, count, copied, more in plan:
+                held, length = list(self._held[session]), self._length[session]
+                if copied:
+                    src.append(held[-1])
+                    held[-1] = next(fresh)
+                    dst.append(held[-1])
+                held += [next(fresh) for _ in range(more)]
+                rows += [held[i // PAGE] * PAGE + i % PAGE for i in range(length, length + count)]
+                held_now.append(held)
+            self._copy(src, dst)
+            out = torch.tensor(rows, dtype=torch.int32, device=self.pages.device)
+        except BaseException:
+            for page in taken:
+                heapq.heappush(self._free, page)
+            raise
+        for (session, count, _, _), held in zip(plan, held_now):
+            self._held[session] = held
+            self._length[session] += count
+        for page in src:
+            self._users[page] -= 1
+        for page in taken:
+            self._users[page] = 1
+        return out
 
     def close(self, session: int) -> None:
         """Ends a session; pages that no other has are free again."""

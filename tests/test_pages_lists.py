@@ -52,3 +52,28 @@ def test_refusals(fcv, calls, src, dst):
     with pytest.raises(ValueError):
         fcv.copy_pages(Pool(), src, dst)
     assert calls == []
+
+
+def test_a_copy_that_fails_changes_nothing(fcv):
+    """The book stays as it was where the pages cannot be copied (here: a pool that is not on the GPU)."""
+    import torch
+
+    book = fcv.CachePages(torch.zeros(1, 12, 16))
+    voice, other = book.open(), book.open()
+    book.extend([other, voice], [64, 100])
+    kids = [book.fork(voice) for _ in range(2)]
+    everyone = [voice, other, *kids]
+    before = (book.table(everyone).tolist(), book.lengths(everyone).tolist(), book.free)
+    for sessions, counts in (([kids[0]], [1]), ([other, kids[0], kids[1], voice], [70, 1, 200, 2])):
+        with pytest.raises(ValueError, match="GPU"):
+            book.extend(sessions, counts)
+        assert (book.table(everyone).tolist(), book.lengths(everyone).tolist(), book.free) == before
+    assert book.extend([other], [2]).tolist() == [3 * 64, 3 * 64 + 1]  # pages 0 to 2 are in use
+    book.close(kids[0])
+    book.close(kids[1])
+    assert book.extend([voice], [1]).tolist() == [2 * 64 + 36] and book.free == 8
+    book.close(other)
+    before = (book.table([voice]).tolist(), book.free)
+    with pytest.raises(ValueError, match="GPU"):
+        book.compact()
+    assert (book.table([voice]).tolist(), book.free) == before
