@@ -215,6 +215,7 @@ SIGNATURES = {
     "fcv_fp4_append": (c_int32, [POINTER(FcvFp4Append), c_void_p]),
     "fcv_fp4_read": (c_int32, [POINTER(FcvFp4Read), c_void_p]),
     "fcv_fp4_attention_workspace_bytes": (c_size_t, [POINTER(FcvFp4Attention)]),
+    "fcv_fp4_attention_plan": (c_int32, [POINTER(FcvFp4Attention)] + [POINTER(c_int32)] * 4),
     "fcv_fp4_attention": (c_int32, [POINTER(FcvFp4Attention), c_void_p, c_size_t, c_void_p]),
     "fcv_copy_pages": (c_int32, [c_void_p, c_int32, c_int64, c_int32, c_int64, c_int64,
                                  c_void_p, c_void_p, c_int32, c_void_p]),

@@ -923,6 +923,19 @@ extern "C" size_t fcv_fp4_attention_workspace_bytes(const FcvFp4Attention* args)
   return fcv::lm::workspace_bytes(*args, fcv::lm::plan_of(*args));
 }
 
+extern "C" int fcv_fp4_attention_plan(const FcvFp4Attention* args, int32_t* rows, int32_t* tiles, int32_t* ranges,
+                                      int32_t* ordered) {
+  if (int rc = fcv::lm::check(args)) return rc;
+  FCV_CHECK(rows && tiles && ranges && ordered, FCV_ERR_INVALID, "null argument");
+  FCV_CHECK(args->tokens > 0, FCV_ERR_INVALID, "no rows: nothing is launched");
+  const fcv::lm::Plan plan = fcv::lm::plan_of(*args);
+  *rows = plan.rows;
+  *tiles = (int32_t)plan.row_tiles;
+  *ranges = plan.splits;
+  *ordered = plan.order_shift >= 0;
+  return FCV_OK;
+}
+
 extern "C" int fcv_fp4_attention(const FcvFp4Attention* args, void* workspace, size_t workspace_bytes,
                                  hipStream_t stream) {
   using namespace fcv::lm;

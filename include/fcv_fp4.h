@@ -194,6 +194,11 @@ typedef struct FcvFp4Attention {
 size_t fcv_fp4_attention_workspace_bytes(const FcvFp4Attention* args);
 int fcv_fp4_attention(const FcvFp4Attention* args, void* workspace, size_t workspace_bytes,
                       hipStream_t stream);
+/* How a call is launched, for logs and tests: tiles of 8, 16 or 128 rows (a row is a query's head), how many of
+ * them a sequence's key head has (a batch that passes max_q gives each several in turn), into how many ranges its
+ * pages are cut, and whether the longest sequences are taken first (1) or each in its place (0). */
+int fcv_fp4_attention_plan(const FcvFp4Attention* args, int32_t* rows, int32_t* tiles, int32_t* ranges,
+                           int32_t* ordered);
 
 /* Page src_host[i] of every layer is copied to page dst_host[i], for i < count: a fork (one source, many
  * destinations) or a compaction.  No page is a destination twice, or both a source and a destination.
