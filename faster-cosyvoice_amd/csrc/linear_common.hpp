@@ -14,7 +14,7 @@ namespace {
 struct Args {
   FcvLmLinear p;
   bool vec;                 // four columns of y, the residual and the bias are on the boundary of four
-  int splits, slices;       // ranges of K, and the 64-wide slices of one
+  int splits, slices;       // ranges of K, and the slices of one: of 64, or of 128 over 4-bit weights
   float* part;              // [splits][m][part_ld] sums of the ranges
   int part_ld;
 };
