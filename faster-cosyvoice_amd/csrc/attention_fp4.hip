@@ -409,8 +409,8 @@ __global__ __launch_bounds__(256, 2) void attend_fp4_kernel(const AttendArgs a) 
 // 16-bit numbers once, in LDS: keys [64][D], values [D][64] in the order of the S^T tiles' rows, so that a
 // lane's weights are its right operand again.  Two pages' room: one barrier a page, with the next page's
 // conversions beside this one's first product, and a step's weights between the products of the one before.
-// m is set kSlack above a row's maximum, and again only where a score passes it (weights are 2^-1.75 to 1 of the
-// row's largest), so that few pages scale the sums; the other tiles' m is the maximum.
+// m is set kSlack above a row's maximum, and again only where a score passes it, so that few pages scale the sums:
+// the row's largest weight lies between 2^-1.75 and 1.  The other tiles' m is the maximum.
 //
 // Bound: instructions.  4000 tokens of 32 heads of 128 over 8 run at 0.65 PFLOP/s (200 us), 4 texts of 300 to 1024
 // behind 4096 keys at 0.60 (210 us), 7000 of 14 heads of 64 over 2 at 0.48 (181 us), in bf16 and fp16 alike.  A
